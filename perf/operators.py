@@ -139,7 +139,10 @@ def _values(case, pieces, value):
     hd = case["hd"]
     if case["bits"] == 16:
         return _unpack(case, pieces, value).contiguous().view(F16).float()
-    scale = pieces[..., : hd // 2].contiguous().view(F16).float().reshape(*pieces.shape[:-1], 16, hd // 32, 1)
+    scale = pieces[..., : hd // 2]
+    if value:
+        scale = scale.unflatten(-1, (4, hd // 32, 2, 2)).movedim(-2, -4).transpose(-1, -2).flatten(-4)
+    scale = scale.contiguous().view(F16).float().reshape(*pieces.shape[:-1], 16, hd // 32, 1)
     quads = _unpack(case, pieces[..., hd // 2:], value).int()
     codes = torch.stack([(quads >> (4 * i)) & 15 for i in range(4)], -1).float() - 8.0
     return (codes.reshape(*codes.shape[:-2], hd // 32, 32) * scale).reshape(*codes.shape[:-2], hd)
@@ -248,7 +251,10 @@ def _store(s, pool, piece, slot, x, value):
     d = top / -8.0
     codes = torch.where(d == 0, 8.0, (blocks / torch.where(d == 0, 1.0, d) + 8.5).trunc().clamp(0, 15)).int()
     quads = codes.reshape(*x.shape[:-1], hd // 4, 4) << torch.tensor([0, 4, 8, 12], device="cuda")
-    at_d = piece[..., None] * words + (slot * (hd // 32))[:, None, None] + torch.arange(hd // 32, device="cuda")
+    block = torch.arange(hd // 32, device="cuda")
+    at_d = (slot // 2 % 4 * (hd // 8) + slot // 8 * 2 + slot % 2)[:, None, None] + 4 * block if value else (
+        slot * (hd // 32))[:, None, None] + block
+    at_d = piece[..., None] * words + at_d
     pool[at + hd // 2] = quads.sum(-1).to(torch.int16)
     pool[at_d] = d.half().view(torch.int16).squeeze(-1)
     got = (pool[at + hd // 2].int()[..., None] >> torch.tensor([0, 4, 8, 12], device="cuda")) & 15
@@ -391,7 +397,12 @@ def _exact_attn(case, s):
             got = pool[piece[..., None] * words + word[pos % 16][:, None]]
             if case["bits"] == 16:
                 return got.view(F16).double()
-            d = pool[piece[..., None] * words + (pos % 16 * (hd // 32))[:, None, None] + torch.arange(hd, device="cuda") // 32]
+            in_piece, block = pos % 16, torch.arange(hd, device="cuda") // 32
+            if value:
+                at_d = 2 * (in_piece // 8)[:, None] + (in_piece % 2)[:, None] + 4 * (block + (in_piece // 2 % 4)[:, None] * (hd // 32))
+            else:
+                at_d = in_piece[:, None] * (hd // 32) + block
+            d = pool[piece[..., None] * words + at_d[:, None]]
             return d.view(F16).double() * (((got.int() >> shift[pos % 16][:, None].int()) & 15) - 8)
 
         k, v = rows_of(s["k"], False), rows_of(s["v"], True)
