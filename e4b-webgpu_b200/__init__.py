@@ -13,5 +13,6 @@ from .config import ModelConfig  # noqa: F401
 from .device import Buffer, Device  # noqa: F401
 from .engine import DeviceStatusError, Engine  # noqa: F401
 from .batch import BatchEngine  # noqa: F401
+from .paged import PagedKV  # noqa: F401
 
-__all__ = ["Engine", "DeviceStatusError", "BatchEngine", "Device", "Buffer", "ModelConfig", "E4BError", "config", "gguf", "ops", "synth", "lib"]
+__all__ = ["Engine", "DeviceStatusError", "BatchEngine", "PagedKV", "Device", "Buffer", "ModelConfig", "E4BError", "config", "gguf", "ops", "synth", "lib"]

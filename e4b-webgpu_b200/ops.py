@@ -121,6 +121,29 @@ def attcomb(dev: Device, part_o, part_ml, out_h, out_f, lse, *, Q_HEADS, HEAD_DI
     dev.call("e4b_attcomb", _p(part_o), _p(part_ml), _p(out_h), _p(out_f), _p(lse), Q_HEADS, HEAD_DIM, CHUNKS)
 
 
+def headprep_paged(dev: Device, kv, qkv, qw, kw, q_out, *, QH, ROPE_ANGLES, THETA, EPS=1e-6, NORM=1, KEQV=0, XF16=0,
+                   STRIDE=0, NPARTS=1, ROWS):
+    """kernels/headprep.wgsl into a paged cache (paged.PagedKV): f16 or 4-bit pages, a position per sequence"""
+    dev.call("e4b_headprep_paged", kv.ref, _p(qkv), _p(qw), _p(kw), _p(q_out), QH, ROPE_ANGLES, THETA, EPS, NORM, KEQV,
+             XF16, STRIDE, NPARTS, ROWS)
+
+
+def kvread_paged(dev: Device, kv, k_out, v_out, *, F32=0, ROWS):
+    """The cached keys / values at the rows' positions as plain rows (f16, or f32 with F32=1)"""
+    dev.call("e4b_kvread_paged", kv.ref, _p(k_out), _p(v_out), F32, ROWS)
+
+
+def attn_paged(dev: Device, kv, q, out_h, out_f, lse, scratch, *, Q_HEADS, WINDOW=0, SINKS=0, SCALE=1.0, XFO=0, ROWS):
+    """Attention of the rows over a paged cache, with an optional window and sinks"""
+    dev.call("e4b_attn_paged", kv.ref, _p(q), _p(out_h), _p(out_f), _p(lse), _p(scratch), Q_HEADS, WINDOW, SINKS, SCALE,
+             XFO, ROWS)
+
+
+def paged_advance(dev: Device, kv):
+    """lens[s] += the rows of the call just made, on the device"""
+    dev.call("e4b_paged_advance", kv.ref)
+
+
 def geglumul(dev: Device, a, b, y, *, N):
     dev.call("e4b_geglumul", _p(a), _p(b), _p(y), N)
 

@@ -1,0 +1,68 @@
+"""Paged KV cache of sequences of unequal length, in f16 or 4 bits (host side).
+
+`PagedKV` is the descriptor (e4b_paged_kv, include/e4b_b200.h) that
+`ops.headprep_paged`, `ops.attn_paged`, `ops.kvread_paged` and
+`ops.paged_advance` take.  It holds device addresses: buffers that the caller
+owns, or ones that it allocates on the device when they are not given.  Which
+page belongs to which sequence is the caller's to decide (`set_tables` uploads
+a page table).
+"""
+from __future__ import annotations
+
+import ctypes
+
+import numpy as np
+
+from ._lib import lib
+
+
+class PagedStruct(ctypes.Structure):
+    """e4b_paged_kv (include/e4b_b200.h)"""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "pages", "lens", "rows")] + \
+        [(n, ctypes.c_int) for n in ("bits", "page", "n_pages", "max_pages", "nseq", "kv_heads", "head_dim")]
+
+
+class PagedKV:
+    """A paged cache of one layer; `ref` is what the C entry points take."""
+
+    def __init__(self, dev, *, BITS, PAGE, PAGES, MAX_PAGES, SEQS, KV_HEADS, HEAD_DIM, k=None, v=None, pages=None,
+                 lens=None, rows=None):
+        pool = lib().e4b_paged_pool_bytes(BITS, PAGE, PAGES, KV_HEADS, HEAD_DIM)
+        if pool == 0:
+            raise ValueError(f"paged cache: bad sizes bits={BITS} page={PAGE} pages={PAGES} kv_heads={KV_HEADS} "
+                             f"head_dim={HEAD_DIM}")
+        self.dev, self.pool_bytes, self.owned = dev, pool, []
+        self.nseq, self.max_pages = SEQS, MAX_PAGES
+
+        def buf(given, nbytes, name):
+            if given is not None:
+                return int(given)
+            self.owned.append(dev.alloc(nbytes, name))
+            return self.owned[-1].ptr
+
+        self.struct = PagedStruct(buf(k, pool, "paged k"), buf(v, pool, "paged v"),
+                                  buf(pages, SEQS * MAX_PAGES * 4, "page table"), buf(lens, SEQS * 4, "lengths"),
+                                  None if rows is None else int(rows), BITS, PAGE, PAGES, MAX_PAGES, SEQS, KV_HEADS,
+                                  HEAD_DIM)
+        self.ref = ctypes.addressof(self.struct)
+
+    def set_tables(self, pages=None, lens=None, rows=None):
+        """Upload the page table [SEQS][MAX_PAGES] and / or the lengths; `rows`: device address of the rows table
+        (0: one row per sequence)."""
+        if pages is not None:
+            a = np.ascontiguousarray(pages, np.uint32)
+            if a.shape != (self.nseq, self.max_pages):
+                raise ValueError(f"paged cache: page table {a.shape}, expected {(self.nseq, self.max_pages)}")
+            self.dev.write(self.struct.pages, a)
+        if lens is not None:
+            a = np.ascontiguousarray(lens, np.uint32)
+            if a.shape != (self.nseq,):
+                raise ValueError(f"paged cache: lengths {a.shape}, expected {(self.nseq,)}")
+            self.dev.write(self.struct.lens, a)
+        if rows is not None:
+            self.struct.rows = int(rows) or None
+
+    def free(self):
+        for b in self.owned:
+            self.dev.free(b)
+        self.owned = []

@@ -498,6 +498,77 @@ E4B_API int e4b_attdec_seq(e4b_ctx* ctx, const float* q, const uint16_t* kcache,
                            int HD, int window, int cachemode, int ring, int max_chunks, float scale, int cache_slots,
                            int nseq, int xfo);
 
+/* ---- paged KV cache: sequences of unequal length, f16 or 4-bit storage (no
+ * counterpart in the reference, whose caches are one contiguous f16 region per
+ * layer).  A pool holds n_pages pages of `page` slots; pages[s][j] (u32) is the
+ * page with slots j*page.. of sequence s, read only where the call needs a slot
+ * of it.  Slot t of a sequence holds its token at position t.  lens[s] is the
+ * number of tokens cached BEFORE the rows of a call: with a rows table the
+ * call's rows rows[s] .. rows[s+1]-1 (ascending, rows[0] = 0) are sequence s's
+ * tokens at positions lens[s], lens[s]+1, ..; a sequence may have none, and
+ * rows from rows[nseq] on (padding up to n_rows) are neither read nor written.
+ * rows = NULL: one row per sequence, n_rows = nseq.  lens, rows and pages are
+ * device memory, so a recorded plan follows them; e4b_paged_advance adds a
+ * call's row counts to lens.
+ *
+ * Storage, per page and KV head, in pieces of 16 slots (bytes: 32*HD for f16,
+ * 9*HD for 4 bits), ordered for the matrix unit's operands; i = slot/8*2 +
+ * slot%2, t = slot/2%4 within the piece:
+ *   f16 keys    [dim/32][slot][dim%32]
+ *   f16 values  [dim/64][i][dim%64/8][t][dim%8]
+ *   4 bits: HD/32 f16 scales per slot, keys [slot][dim/32], values
+ *     [t][dim/32][slot/8][slot%2]; then 16-bit words of the codes of 4
+ *     consecutive dims (the lowest dim in the lowest bits), with nb = min(4, HD/32)
+ *     keys    [dim/32/nb][slot][dim%32/8][dim/32%nb][dim%8/4]
+ *     values  [i][dim%32/4][t][dim/32]
+ * A 4-bit block is 32 dims of the f16 value that an f16 cache would hold, under
+ * the q4_0 rule: m = the first element of the largest magnitude, d = m / -8,
+ * code = trunc(x / d + 8.5) in 0..15, standing for f16(d) * (code - 8); a block
+ * with an infinity or NaN reads back as NaN.
+ *
+ * A position at or past max_pages*page, or a page id >= n_pages, sets
+ * E4B_ST_BADINDEX in the device status word; the slot is then not written, and
+ * counts as not visible (reads as zeros).  So does a row count past n_rows.
+ * head_dim 64, 128 or 256; pools 16-byte aligned; nseq <= 4096. */
+typedef struct {
+  void* k; /* page pools, e4b_paged_pool_bytes each */
+  void* v;
+  const uint32_t* pages; /* [nseq][max_pages] */
+  const uint32_t* lens;  /* [nseq] */
+  const uint32_t* rows;  /* [nseq + 1], or NULL */
+  int bits, page, n_pages, max_pages, nseq, kv_heads, head_dim;
+} e4b_paged_kv;
+E4B_API size_t e4b_paged_pool_bytes(int bits, int page, int n_pages, int kv_heads, int head_dim); /* 0: bad sizes */
+/* e4b_headprep (kernels/headprep.wgsl:19-87) into a paged cache: rows of q|k|v
+ * (f32, or f16 with x_f16; row_stride elements apart, 0 = the row's width;
+ * nparts > 1: the sum of nparts [n_rows][row_stride] f32 partials, in order).
+ * norm = 1: q and k heads RMS-normalised with qw / kw, v without a weight; 0: as
+ * they are (qw, kw unused).  RoPE on pairs (p, p + HD/2), p < rope_angles, at the
+ * row's position, its angle in 64 bits.  q_out f32 [n_rows][QH][HD] (QH = 0: none);
+ * K and V rows go to the cache (v = the k slice when keqv).  qkv 16-byte aligned
+ * (f16: 8), row_stride % 4 == 0. */
+E4B_API int e4b_headprep_paged(e4b_ctx* ctx, const e4b_paged_kv* kv, const void* qkv, const float* qw,
+                               const float* kw, float* q_out, int QH, int rope_angles, float theta, float eps,
+                               int norm, int keqv, int x_f16, int row_stride, int nparts, int n_rows);
+/* The cached keys / values at the rows' positions, as plain rows [n_rows][KVH][HD]
+ * of f16 (out_f32 = 1: f32, exact); k_out or v_out may be NULL. */
+E4B_API int e4b_kvread_paged(e4b_ctx* ctx, const e4b_paged_kv* kv, void* k_out, void* v_out, int out_f32, int n_rows);
+/* Attention of the rows over the paged cache (their own K/V already appended):
+ * the row at position p sees slots t <= p, with window > 0 only those with
+ * t > p - window or t < sinks.  q f32 [n_rows][QH][HD]; out_h f16 (fragment order
+ * when xfo) and / or out_f f32 [n_rows][QH*HD], lse f32 [n_rows][QH] or NULL; a row
+ * that sees nothing gives zeros and lse = -inf.  Products carry f32 precision
+ * (q and p as f16 hi + lo), sums are f32.  Pages wholly between the sinks and
+ * the window are not read and need no valid id.  scratch: e4b_paged_scratch_bytes(),
+ * 16-byte aligned, zeroed once before its first use (each call leaves it ready
+ * for the next) and not shared by calls that may overlap.  QH/KVH <= 8. */
+E4B_API size_t e4b_paged_scratch_bytes(void);
+E4B_API int e4b_attn_paged(e4b_ctx* ctx, const e4b_paged_kv* kv, const float* q, uint16_t* out_h, float* out_f,
+                           float* lse, void* scratch, int QH, int window, int sinks, float scale, int xfo, int n_rows);
+/* lens[s] += the sequence's rows of the call (1 without a rows table): the cache
+ * is ready for the next rows.  Writes through kv->lens. */
+E4B_API int e4b_paged_advance(e4b_ctx* ctx, const e4b_paged_kv* kv);
+
 /* ------------------------------------------------------------ argmax / feed */
 /* kernels/argmax2.wgsl:8-48 (both stages): out[0] = index of the largest x (ties
  * -> lowest index), out[1] = its f32 bits.  part: scratch of 2*parts u32. */
