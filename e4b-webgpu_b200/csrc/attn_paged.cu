@@ -2,37 +2,43 @@
 // optional sliding window and sinks: split-KV on the tensor cores.
 //
 // Unit = (sequence, group of query rows, KV head).  A unit's work is the pieces
-// of 16 slots that its sequence's rows can see; the pieces of all units, one
-// after the other, are cut into equal runs, one per CTA, so ragged lengths and
-// few long sequences alike fill the machine.  A CTA's warps take a run's pieces
-// in turn; each warp streams its own (one bulk copy for the keys, one for the
-// values, through a ring of its own) and keeps its own softmax state, so the
-// main loop has no CTA barrier.  At a unit's end the warps' states are merged in
-// shared memory; a unit cut between CTAs leaves partials in the scratch, which
-// the last CTA to arrive merges in CTA order (the same bits every time).
+// of 16 slots that its rows can see; the work of all units, one after the other,
+// is cut into equal runs, one per CTA, so ragged lengths and few long sequences
+// alike fill the machine.  In a CTA a producer warp streams the run's pieces (one
+// bulk copy for the keys, one for the values) through a ring of stages, a lane
+// per stage, into the next units too.  The consumer warps form WS x WC: WC warps
+// share a piece, each with its own query rows, and WS such groups take pieces in
+// turn.  A unit of one row has WC = 1, one of a prompt's chunk WC = W; a stage is
+// free after W arrivals, so its WC users arrive W / WC times each.  Every warp
+// keeps its own softmax state; at a unit's end the WS states are merged in shared
+// memory.  A unit cut between CTAs leaves partials in the scratch, which the last
+// CTA to arrive merges in CTA order (the same bits every time).
 //
 // Products, per piece and 8 MMA columns (m16n8k16, f32 accumulators):
 //   S[slot][col]  = K[slot][:] . q[:][col]      A = keys,   B = q
 //   O[dim][col]  += V[slot][dim] p[slot][col]   A = values, B = p
-// The 8 columns are 4 query heads as f16 hi and lo parts (columns 0-3, 4-7), so
-// q and p carry f32 precision at the MMA cost of one f16 pass.
-// 4 bits: A holds the codes n as f16 subnormals, n * 2^-24 (a code in the low
-// bits of a half) or 16 n * 2^-24 (one place up; q is divided by 16 there, the
-// value's sum at the end), so decoding is one AND per pair.  The -8 enters as the
-// accumulator's start (keys: -8 sum q per block) and as an MMA with a constant A
-// (values).  A key block's scale multiplies its block's dot product in f32; a
-// value block's scale multiplies p, again as hi + lo.
+// The 8 columns are 4 query heads of one row as f16 hi and lo parts (columns 0-3,
+// 4-7), so q and p carry f32 precision at the MMA cost of one f16 pass.
+// 4-bit keys: A holds the codes n as f16 subnormals, n * 2^-24 (a code in the low
+// bits of a half) or 16 n * 2^-24 (one place up; q is divided by 16 there), so
+// decoding is one AND per pair; a block's scale d multiplies its dot product in
+// f32, and the code's -8 is one more MMA per piece, sum_b d_b (-8 sum q_b).
+// The MMA aligns a subnormal by its exponent field, which costs it up to 7 of the
+// sum's 24 bits: no loss for 15-bit products of one magnitude (q's), but 6e-6 of
+// the result where p spreads over many, so 4-bit values are decoded to normal f16
+// n - 8.  A value block's scale multiplies p, again as hi + lo; p is kept as
+// p * 2^14 unless a scale of the piece is 2 or more, so that the lo parts stay
+// clear of f16's subnormals.
 #include "paged.cuh"
 #include "stream.cuh"
 
 namespace {
 using namespace e4b;
 
-constexpr int kMaxCtas = 256;
-constexpr int kCols = 8;             // query heads of a unit at most (2 n-tiles of 4)
+constexpr int kMaxCtas = 160;
 constexpr uint32_t kLowCodes = 0x000F000Fu, kHighCodes = 0x00F000F0u;
-constexpr uint32_t kMinus8Low = 0x80088008u, kMinus8High = 0x80808080u;  // -8 * 2^-24, -8 * 16 * 2^-24
-constexpr float kTwo24 = 16777216.f, kTwo20 = 1048576.f;
+constexpr float kTwo24 = 16777216.f;
+constexpr float kLift = 14.f;        // p is held as p * 2^14 (see above)
 
 struct AttnP {
   PagedDev d;
@@ -41,90 +47,137 @@ struct AttnP {
   float* out_f;
   float* lse;
   uint32_t* arrived;                 // [kMaxCtas], zero at rest
-  float* parts;                      // [2 * CTAs][kCols][HD + 2]
-  int QH, G, per_unit, xfo;          // per_unit: query rows of a unit
+  float* parts;                      // [2 * CTAs][columns][HD], then (max, sum) per column
+  int QH, G, xfo;
   uint32_t window, sinks;
   float scale;
 };
 
-constexpr size_t kPartFloats = (size_t)kCols * (256 + 2);
+constexpr int kMaxCols = 64;         // columns (row, head) of a unit at most
+constexpr size_t kPartFloats = (size_t)kMaxCols * (256 + 2);
+
+constexpr int kConsumerRegs = 224, kProducerRegs = 56;
 
 template <int BITS, int HD, int NT>
 struct Shape {
   static constexpr int NB = HD / 32;
   static constexpr int PB = BITS == 16 ? 32 * HD : 9 * HD;
   static constexpr int STAGE = 2 * PB;
-  // warps and ring depth: about 150-200 KB in flight per SM
-  static constexpr int W = BITS == 16 && HD == 256 ? 4 : 8;
-  static constexpr int ST = BITS == 16 ? (HD == 64 ? 5 : (NT == 2 ? 2 : 3)) : (HD == 256 ? (NT == 2 ? 3 : 4) : 8);
-  static constexpr int THREADS = 32 * W;
-  static constexpr size_t RING = (size_t)W * ST * STAGE;
+  // consumer warps: with one n-tile a warp needs 168 registers, so 12 warps fit an SM;
+  // with two it needs more, which the producer's warpgroup gives up (setmaxnreg):
+  // 8 * 32 * 224 + 4 * 32 * 56 = 384 * 168, what the block was launched with
+  static constexpr int W = NT == 1 ? (BITS == 16 && HD == 256 ? 10 : 11) : 8;
+  // ring depth: a multiple of W, so a stage's uses within a unit belong to the same
+  // warps (a warp then never waits for a phase before the stage's last one is done)
+  static constexpr int S = NT == 1 ? W * (BITS == 16 ? (HD == 256 ? 1 : (HD == 128 ? 2 : 4)) : (HD == 256 ? 2 : (HD == 128 ? 4 : 6)))
+                                   : W * (BITS == 16 ? (HD == 256 ? 1 : (HD == 128 ? 2 : 4)) : (HD == 64 ? 8 : 4));
+  static constexpr int LN = S <= 32 ? S : (NT == 1 ? 22 : 32);          // producer lanes; S is a multiple
+  static constexpr int THREADS = 384, CT = 32 * W;
+  static constexpr int TILES = W * NT;                                  // n-tiles of a unit at most
+  static constexpr size_t RING = (size_t)S * STAGE;
+  // q fragments [TILES][NB][32] while a unit's pieces pass, then the warps' O [W][NT*4][HD]
   static constexpr size_t MERGE = (size_t)W * NT * 4 * HD * 4;
-  static constexpr size_t QFRAG = (size_t)NT * NB * 32 * 16;
-  static constexpr size_t SMEM = RING + MERGE + QFRAG + 128;
+  static constexpr size_t SMEM = RING + MERGE;
+  static_assert((size_t)TILES * NB * 32 * 16 <= MERGE, "q fragments fit the merge buffer");
 };
 
-// One sequence's rows of the call and the pieces they see.
+// Rows and heads of a unit in n-tiles: a row of up to 4 heads is one tile, of up
+// to 8 heads two; a warp has NT tiles.
+template <int W, int NT>
+struct Rows {
+  int per_warp;                      // rows of a warp
+  E4B_DEV explicit Rows(int G) : per_warp(G > 4 ? NT / 2 : NT) {}
+  E4B_DEV uint32_t per_unit() const { return per_warp * W; }
+  // warps that share a piece, for a unit of r rows: a power of two
+  E4B_DEV uint32_t sharing(uint32_t r) const {
+    uint32_t wc = 1;
+    while (wc * per_warp < r) wc *= 2;
+    return wc;
+  }
+};
+
+// One sequence's rows of the call, the pieces they see and what they cost.
 struct SeqWork {
   uint32_t p0, nq;                   // first row's position, rows
-  uint32_t groups, np;
   PieceRange range;
+  uint32_t full, tail_wc;            // units of W sharing warps, sharing warps of the last unit (0: none)
+  uint64_t cost;                     // sum over units and KV heads of pieces * sharing warps
 };
+template <int W, int NT>
 E4B_DEV SeqWork seq_work(const AttnP& p, int s) {
+  const Rows<W, NT> rows(p.G);
   SeqWork w;
   uint32_t r0 = (uint32_t)s, r1 = r0 + 1;
   if (p.d.rows) r0 = p.d.rows[s], r1 = min(p.d.rows[s + 1], (uint32_t)p.d.n_rows);
   w.nq = r1 > r0 ? r1 - r0 : 0u;
-  // positions past the table are clamped: such slots are never visible (cap)
-  const uint64_t last = (uint64_t)p.d.lens[s] + w.nq;
-  w.p0 = min(p.d.lens[s], 0xfffffff0u - w.nq);
-  w.groups = (w.nq + p.per_unit - 1) / p.per_unit;
-  w.np = 0;
+  const uint32_t len = p.d.lens[s];
+  w.p0 = min(len, 0xfffffff0u - w.nq);
+  w.cost = 0;
+  w.full = w.tail_wc = 0;
   if (w.nq) {
-    if (last > p.d.cap && threadIdx.x == 0) set_status(p.d.status, E4B_ST_BADINDEX);
+    // positions past the table are clamped: no such slot is visible
+    if ((uint64_t)len + w.nq > p.d.cap) set_status(p.d.status, E4B_ST_BADINDEX);
     const uint32_t p1 = min(w.p0 + w.nq - 1, p.d.cap - 1);
     w.range = piece_range(min(w.p0, p1), p1, p.window, p.sinks);
-    w.np = w.range.count;
+    w.full = w.nq / rows.per_unit();
+    const uint32_t rest = w.nq % rows.per_unit();
+    w.tail_wc = rest ? rows.sharing(rest) : 0u;
+    w.cost = (uint64_t)w.range.count * p.d.KVH * ((uint64_t)w.full * W + w.tail_wc);
   }
   return w;
 }
 
-// Walks a CTA's run [g, end) of pieces, unit by unit.
+E4B_DEV uint64_t udiv(uint64_t a, uint32_t b) {
+  return (a >> 32) == 0 ? (uint64_t)((uint32_t)a / b) : a / b;
+}
+
+// Walks a CTA's run [g, end) of the work, unit by unit.
+template <int W, int NT>
 struct Walk {
-  uint64_t g, end, base;             // base: first piece of the current sequence
+  uint64_t g, end, base;             // base: where the current sequence's work begins
   int s;
   SeqWork w;
-  uint32_t kvh, group, k0, k1;       // current segment: pieces k0..k1-1 of the unit
-  uint64_t unit0;                    // first piece of the unit
+  uint64_t unit0, unit1;             // the unit's work
+  uint32_t kvh, wc, nrows;           // KV head, sharing warps, rows
   uint32_t pmin, pmax;               // positions of the unit's rows
+  PieceSpan span;                    // this CTA's pieces of it
   E4B_DEV bool next(const AttnP& p) {
     if (g >= end) return false;
-    const uint32_t KVH = p.d.KVH;
-    uint64_t total = (uint64_t)w.np * w.groups * KVH;
-    while (g >= base + total) {
-      base += total;
+    while (g >= base + w.cost) {
+      base += w.cost;
       if (++s >= p.d.nseq) {         // the lengths changed under the call
         g = end;
         return false;
       }
-      w = seq_work(p, s);
-      total = (uint64_t)w.np * w.groups * KVH;
+      w = seq_work<W, NT>(p, s);
     }
-    const uint64_t unit = (g - base) / w.np;
-    unit0 = base + unit * w.np;
-    k0 = (uint32_t)(g - unit0);
-    k1 = (uint32_t)min((uint64_t)w.np, k0 + (end - g));
-    kvh = (uint32_t)(unit % KVH);
-    group = (uint32_t)(unit / KVH);
-    pmin = w.p0 + group * p.per_unit;
-    pmax = min(pmin + p.per_unit, w.p0 + w.nq) - 1;
-    g += k1 - k0;
+    const Rows<W, NT> rows(p.G);
+    const uint32_t KVH = p.d.KVH, np = w.range.count;
+    const uint64_t off = g - base, full_cost = (uint64_t)np * W * w.full * KVH;
+    uint32_t group, unit;
+    if (off < full_cost) {
+      wc = W;
+      unit = (uint32_t)udiv(off, np * W);
+      unit0 = base + (uint64_t)unit * np * W;
+      group = unit / KVH;
+      kvh = unit % KVH;
+      nrows = rows.per_unit();
+    } else {
+      wc = w.tail_wc;
+      kvh = (uint32_t)udiv(off - full_cost, np * wc);
+      unit0 = base + full_cost + (uint64_t)kvh * np * wc;
+      group = w.full;
+      nrows = w.nq - group * rows.per_unit();
+    }
+    unit1 = unit0 + (uint64_t)np * wc;
+    pmin = w.p0 + group * rows.per_unit();
+    pmax = pmin + nrows - 1;
+    const uint64_t stop = min(unit1, end);
+    const uint32_t k0 = ((uint32_t)(g - unit0) + wc - 1) / wc, k1 = ((uint32_t)(stop - unit0) + wc - 1) / wc;
+    const uint32_t p1 = min(pmax, p.d.cap - 1);
+    span = piece_span(w.range, k0, k1, min(pmin, p1), p1, p.window, p.sinks);
+    g = stop;
     return true;
-  }
-  // Does a row of the unit see a slot of the piece?
-  E4B_DEV bool needs(const AttnP& p, uint32_t piece) const {
-    const uint32_t t0 = piece * kPieceSlots;
-    return t0 <= pmax && (p.window == 0 || t0 < p.sinks || pmin < p.window || t0 + kPieceSlots - 1 > pmin - p.window);
   }
 };
 
@@ -143,10 +196,30 @@ E4B_DEV uint32_t hmul2(uint32_t a, uint32_t b) {
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
+// a * b - c
+E4B_DEV uint32_t hfms2(uint32_t a, uint32_t b, uint32_t c) {
+  const __half2 r = __hfma2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b),
+                            __hneg2(*reinterpret_cast<__half2*>(&c)));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
 E4B_DEV uint32_t pack2(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
+}
+// D = A B, from a zero accumulator.
+E4B_DEV void mma16816_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+// The pair of codes in bits 0..3 (4..7) of each half, as f16 n - 8: OR-ed under the
+// exponent of 1024 they read 1024 + n (1024 + 16 n), from which one instruction
+// takes 1032 (and divides by 16).
+E4B_DEV uint32_t low_codes(uint32_t x) { return hsub2((x & kLowCodes) | 0x64006400u, 0x64086408u); }
+E4B_DEV uint32_t high_codes(uint32_t x) {
+  return hfma2((x & kHighCodes) | 0x64006400u, 0x2C002C00u, 0xD480D480u);   // / 16, - 72
 }
 E4B_DEV uint4 lds128(const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); }
 template <int WORDS>
@@ -161,144 +234,172 @@ E4B_DEV void lds_words(uint32_t (&w)[WORDS], const uint8_t* p) {
     w[0] = *reinterpret_cast<const uint32_t*>(p);
   }
 }
+E4B_DEV void mbar_arrive_n(uint64_t* b, uint32_t n) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(b)), "r"(n) : "memory");
+}
 
 template <int BITS, int HD, int NT>
 __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, 1) k_attn_paged(const AttnP p) {
   using Sh = Shape<BITS, HD, NT>;
-  constexpr int NB = Sh::NB, PB = Sh::PB, W = Sh::W, ST = Sh::ST, THREADS = Sh::THREADS, COLS = NT * 4;
-  constexpr int TILES = HD / 16;     // m16 tiles of O
+  constexpr int NB = Sh::NB, PB = Sh::PB, W = Sh::W, S = Sh::S, LN = Sh::LN, CT = Sh::CT, LC = NT * 4;
+  static_assert(S % W == 0 && S % LN == 0 && LN <= 32 && S <= Sh::THREADS, "ring");
+  constexpr int OT = HD / 16;        // m16 tiles of O
+  using Unit = Walk<W, NT>;
   extern __shared__ __align__(128) uint8_t smem[];
   uint8_t* ring = smem;
-  float* merge = reinterpret_cast<float*>(smem + Sh::RING);            // [W][COLS][HD]
-  uint4* qfrag = reinterpret_cast<uint4*>(smem + Sh::RING + Sh::MERGE);  // [NT][NB][32]
-  __shared__ uint64_t bars[W * ST];
-  __shared__ int loaded[W * ST];
-  __shared__ uint64_t sums[THREADS];
-  __shared__ float qstart[NT * NB * 8], qfac[COLS];     // -8 sum q per block and column; score factor
-  __shared__ float ml[W * COLS * 2], weight[kMaxCtas], fin[2];
+  float* merge = reinterpret_cast<float*>(smem + Sh::RING);            // [W][LC][HD]
+  uint4* qfrag = reinterpret_cast<uint4*>(smem + Sh::RING);            // [TILES][NB][32]
+  __shared__ uint64_t landed[S], freed[S];
+  __shared__ int usable[S];
+  __shared__ uint64_t warp_sum_[Sh::THREADS / 32];
+  __shared__ uint2 qzero[BITS == 4 ? Sh::TILES * 32 : 1];               // B of the -8 term: -8 sum q per block, hi and lo
+  __shared__ float qfac[Sh::TILES * 4];
+  __shared__ float ml[W * LC * 2], weight[W][kMaxCtas];
   __shared__ int last_one;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
 
-  if (tid < W * ST) mbar_init(&bars[tid], 1);
+  if (tid < S) {
+    mbar_init(&landed[tid], 1);
+    mbar_init(&freed[tid], W);
+  }
   if (tid == 0) fence_barrier_init();
+  if constexpr (BITS == 4)
+    for (int i = tid; i < Sh::TILES * 32; i += Sh::THREADS) qzero[i] = make_uint2(0u, 0u);
   pdl_wait();
 
-  // ---- the run of this CTA: pieces of all units, cut evenly
+  // ---- the run of this CTA: the work of all units, cut evenly
   uint64_t mine = 0;
-  const int per = (p.d.nseq + THREADS - 1) / THREADS;
-  for (int s = tid * per; s < min(p.d.nseq, (tid + 1) * per); s++) {
-    const SeqWork w = seq_work(p, s);
-    mine += (uint64_t)w.np * w.groups * p.d.KVH;
+  const int per = (p.d.nseq + Sh::THREADS - 1) / Sh::THREADS;
+  for (int s = tid * per; s < min(p.d.nseq, (tid + 1) * per); s++) mine += seq_work<W, NT>(p, s).cost;
+  if (blockIdx.x == 0) live_rows(p.d);                   // records a row count past n_rows
+  uint64_t upto = mine;                                  // inclusive sum over the threads
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint64_t v = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += v;
   }
-  sums[tid] = mine;
-  live_rows(p.d);                    // records a row count past n_rows
+  if (lane == 31) warp_sum_[warp] = upto;
   __syncthreads();
-  for (int o = 1; o < THREADS; o <<= 1) {
-    const uint64_t v = tid >= o ? sums[tid - o] : 0;
-    __syncthreads();
-    sums[tid] += v;
-    __syncthreads();
+  uint64_t before = 0, T = 0;
+#pragma unroll
+  for (int i = 0; i < Sh::THREADS / 32; i++) {
+    if (i < warp) before += warp_sum_[i];
+    T += warp_sum_[i];
   }
-  const uint64_t T = sums[THREADS - 1];
-  const uint64_t want = (T + W - 1) / W;                // at least a piece per warp
+  upto += before;
+  const uint64_t want = udiv(T + W - 1, W);              // at least a piece per warp
   const uint32_t C = want < gridDim.x ? (uint32_t)want : gridDim.x;
   const uint32_t cta = blockIdx.x;
   if (cta >= C) return;
-  Walk seg;
-  seg.g = T * cta / C;
-  seg.end = T * (cta + 1) / C;
-  {
-    int lo = 0, hi = THREADS - 1;    // first thread whose sequences reach past seg.g
-    while (lo < hi) {
-      const int mid = (lo + hi) / 2;
-      if (sums[mid] > seg.g) hi = mid;
-      else lo = mid + 1;
-    }
-    seg.s = lo * per;
-    seg.base = lo ? sums[lo - 1] : 0;
-    seg.w = seq_work(p, seg.s);
-  }
+  Unit u;
+  u.g = udiv(T * cta, C);
+  u.end = udiv(T * (cta + 1), C);
+  // the thread whose sequences hold the run's start tells the others
+  __shared__ uint64_t start_base;
+  __shared__ int start_seq;
+  if (upto - mine <= u.g && u.g < upto) start_base = upto - mine, start_seq = tid * per;
+  __syncthreads();
+  u.base = start_base;
+  u.s = start_seq;
+  u.w = seq_work<W, NT>(p, u.s);
 
-  // ---- the warp's feed: runs ST pieces ahead, into the next segments too
-  Walk feed = seg;
-  bool more = true;
-  uint32_t fk = 0, fk1 = 0, piece_n = 0, page_n = 0;
-  const auto advance = [&]() {
-    for (;;) {
-      while (fk < fk1) {
-        piece_n = feed.w.range.at(fk);
-        fk += W;
-        if (feed.needs(p, piece_n)) {
-          const uint32_t slot = piece_n * kPieceSlots;
-          page_n = slot < p.d.cap ? p.d.pages[(size_t)feed.s * p.d.max_pages + slot / (uint32_t)p.d.page] : 0xffffffffu;
+  if (warp >= W) {
+    // ---- producer: lane i brings the CTA's pieces i, i + LN, .., piece j into stage j % S
+    if constexpr (NT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProducerRegs));
+    if (warp > W || lane >= LN) return;
+    constexpr uint32_t kLanes = LN == 32 ? 0xffffffffu : (1u << (LN & 31)) - 1u;
+    uint32_t j = lane, seg0 = 0, seg1 = 0, page = 0, piece = 0, in_page = 0;
+    bool more = true;
+    const auto find = [&]() {        // piece j of the run and its page
+      while (j >= seg1) {
+        if (!u.next(p)) {
+          more = false;
           return;
         }
+        seg0 = seg1;
+        seg1 += u.span.count;
       }
-      if (!feed.next(p)) {
-        more = false;
-        return;
+      piece = u.span.at(j - seg0);
+      const uint32_t slot = piece * kPieceSlots, nth = slot / (uint32_t)p.d.page;
+      in_page = slot - nth * (uint32_t)p.d.page;
+      page = slot < p.d.cap ? p.d.pages[(size_t)u.s * p.d.max_pages + nth] : 0xffffffffu;
+    };
+    find();
+    uint64_t since = 0;
+    uint32_t idle = 0;
+    while (__any_sync(kLanes, more)) {
+      const uint32_t st = j % S;
+      const bool ready = more && (j < (uint32_t)S || mbar_try_wait(&freed[st], ((j / S) & 1u) ^ 1u));
+      if (ready) {
+        const bool ok = page < p.d.n_pages;
+        usable[st] = ok;
+        if (ok) {
+          const uint64_t off = piece_offset(page, u.kvh, (int)in_page, p.d.KVH, p.d.page, PB);
+          uint8_t* dst = ring + (size_t)st * Sh::STAGE;
+          mbar_expect_tx(&landed[st], 2 * PB);
+          bulk_g2s(dst, p.d.k + off, PB, &landed[st]);
+          bulk_g2s(dst + PB, p.d.v + off, PB, &landed[st]);
+        } else {
+          set_status(p.d.status, E4B_ST_BADINDEX);
+          mbar_arrive(&landed[st]);
+        }
+        j += LN;
+        find();
       }
-      fk = feed.k0 + warp;
-      fk1 = feed.k1;
-    }
-  };
-  uint32_t issued = 0;
-  const auto issue = [&]() {         // the pending piece into the next stage
-    if (!more) return;
-    if (lane == 0) {
-      const uint32_t st = issued % ST;
-      const bool ok = page_n < p.d.n_pages;
-      loaded[warp * ST + st] = ok;
-      if (ok) {
-        const uint64_t off = piece_offset(page_n, feed.kvh, (int)(piece_n * kPieceSlots % (uint32_t)p.d.page), p.d.KVH,
-                                          p.d.page, PB);
-        uint8_t* dst = ring + (size_t)(warp * ST + st) * Sh::STAGE;
-        mbar_expect_tx(&bars[warp * ST + st], 2 * PB);
-        bulk_g2s(dst, p.d.k + off, PB, &bars[warp * ST + st]);
-        bulk_g2s(dst + PB, p.d.v + off, PB, &bars[warp * ST + st]);
+      if (__any_sync(kLanes, ready)) {
+        idle = 0;
       } else {
-        set_status(p.d.status, E4B_ST_BADINDEX);
-        mbar_arrive(&bars[warp * ST + st]);
+        __nanosleep(40);
+        if (idle == 0) since = globaltimer_ns();
+        if ((++idle & 255u) == 0 && __any_sync(kLanes, globaltimer_ns() - since > 2000000000ull)) {
+          set_status(p.d.status, E4B_ST_TIMEOUT);        // the consumers gave up
+          break;
+        }
       }
     }
-    issued++;
-    advance();
-  };
-  advance();
-  for (int i = 0; i < ST; i++) issue();
+    // nothing of this CTA is in flight when it ends
+    for (int k = 0; k < S / LN && j >= (uint32_t)(lane + LN); k++) {
+      j -= LN;
+      mbar_wait(&landed[j % S], (j / S) & 1u, p.d.status);
+    }
+    return;
+  }
 
-  uint32_t used = 0;                 // pieces that have landed
+  if constexpr (NT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kConsumerRegs));
+  const auto consumers = []() { asm volatile("bar.sync 1, %0;" ::"n"(CT) : "memory"); };
+  uint32_t j0 = 0;                   // the CTA's pieces before the unit's
   bool alive = true;                 // no wait has run out
   bool first = true;                 // the CTA's first segment
-  float O[NT][TILES][4];
-  uint4 qreg[NT == 1 ? NB : 1];
-  float creg[NT == 1 ? NB : 1][2];
+  float O[NT][OT][4];
 
-  while (seg.next(p)) {
-    const SeqWork& w = seg.w;
-    // ---- q of the unit as B fragments: HD/8 lanes take a column, a lane the 8 dims of one (block, t)
+  while (u.next(p)) {
+    const uint32_t WC = u.wc, WS = W / WC;
+    const int wc = warp % WC, ws = warp / WC;
+    const uint32_t row0 = (p.d.rows ? p.d.rows[u.s] : (uint32_t)u.s) + (u.pmin - u.w.p0);
+    // column c of the unit: tile c / 4 -> row of the unit, head
+    const auto col_row = [&](int c) { return p.G > 4 ? c >> 3 : c >> 2; };
+    const auto col_head = [&](int c) { return p.G > 4 ? c & 7 : c & 3; };
+    const auto col_live = [&](int c) { return col_head(c) < p.G && (uint32_t)col_row(c) < u.nrows; };
+    const int cols = WC * LC;
+
+    // ---- q as B fragments: HD/8 lanes take a column, a lane the 8 dims of one (block, t)
     {
       constexpr int LPC = HD / 8;
       const int sub = tid / LPC, l = tid % LPC, blk = l >> 2, tt = l & 3;
-      for (int c0 = 0; c0 < COLS; c0 += THREADS / LPC) {
-        const int c = c0 + sub;
-        const int nt = c >> 2, cc = c & 3;
-        const int head = p.G > 4 ? c : cc;
-        const uint32_t pos = seg.pmin + (p.G > 4 ? 0 : nt);
-        const bool on = c < COLS && head < p.G && pos <= seg.pmax;
+      for (int c0 = 0; c0 < cols; c0 += CT / LPC) {
+        const int c = c0 + sub, tile = c >> 2, cc = c & 3;
         float x[8];
 #pragma unroll
-        for (int j = 0; j < 8; j++) x[j] = 0.f;
-        if (on) {
-          const uint32_t row = (p.d.rows ? p.d.rows[seg.s] : (uint32_t)seg.s) + (pos - w.p0);
+        for (int i = 0; i < 8; i++) x[i] = 0.f;
+        if (c < cols && col_live(c)) {
           const float4* src = reinterpret_cast<const float4*>(
-              p.q + ((size_t)row * p.QH + seg.kvh * p.G + head) * HD + 8 * l);
+              p.q + ((size_t)(row0 + col_row(c)) * p.QH + u.kvh * p.G + col_head(c)) * HD + 8 * l);
           const float4 a = src[0], b = src[1];
           x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
         }
         float m = 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; j++) m = fmaxf(m, fabsf(x[j]));
+        for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(x[i]));
 #pragma unroll
         for (int o = 1; o < LPC; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
         // a power of two that brings the largest |q| into [2^14, 2^15): f16 hi + lo then
@@ -306,117 +407,106 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, 1) k_attn_paged(
         const int e = (int)(__float_as_uint(m) >> 23);   // biased exponent; 0: zero or subnormal, 255: inf
         const int up = e == 255 ? 0 : min(14 + 127 - e, 120);
         const float f = __uint_as_float((uint32_t)(up + 127) << 23);
-        float hi[8], lo[8], sh = 0.f, sl = 0.f;
+        float hi[8], lo[8], sum = 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-          const float v = x[j] * f;
-          hi[j] = __half2float(__float2half_rn(v));
-          lo[j] = __half2float(__float2half_rn(v - hi[j]));
-          sh += hi[j];
-          sl += lo[j];
+        for (int i = 0; i < 8; i++) {
+          const float v = x[i] * f;
+          hi[i] = __half2float(__float2half_rn(v));
+          lo[i] = __half2float(__float2half_rn(v - hi[i]));
+          sum += v;
         }
+        uint4 fh, fl;
         if constexpr (BITS == 4) {
-          sh += __shfl_xor_sync(0xffffffffu, sh, 1);
-          sl += __shfl_xor_sync(0xffffffffu, sl, 1);
-          sh += __shfl_xor_sync(0xffffffffu, sh, 2);
-          sl += __shfl_xor_sync(0xffffffffu, sl, 2);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+          constexpr float r = 1.f / 16.f;
+          fh = make_uint4(pack2(hi[0], hi[4]), pack2(hi[2], hi[6]), pack2(hi[1] * r, hi[5] * r), pack2(hi[3] * r, hi[7] * r));
+          fl = make_uint4(pack2(lo[0], lo[4]), pack2(lo[2], lo[6]), pack2(lo[1] * r, lo[5] * r), pack2(lo[3] * r, lo[7] * r));
+        } else {
+          fh = make_uint4(pack2(hi[0], hi[1]), pack2(hi[2], hi[3]), pack2(hi[4], hi[5]), pack2(hi[6], hi[7]));
+          fl = make_uint4(pack2(lo[0], lo[1]), pack2(lo[2], lo[3]), pack2(lo[4], lo[5]), pack2(lo[6], lo[7]));
         }
-        if (c < COLS) {
-          uint4 fh, fl;
+        if (c < cols) {
+          qfrag[(tile * NB + blk) * 32 + cc * 4 + tt] = fh;
+          qfrag[(tile * NB + blk) * 32 + (cc + 4) * 4 + tt] = fl;
           if constexpr (BITS == 4) {
-            constexpr float r = 1.f / 16.f;
-            fh = make_uint4(pack2(hi[0], hi[4]), pack2(hi[2], hi[6]), pack2(hi[1] * r, hi[5] * r), pack2(hi[3] * r, hi[7] * r));
-            fl = make_uint4(pack2(lo[0], lo[4]), pack2(lo[2], lo[6]), pack2(lo[1] * r, lo[5] * r), pack2(lo[3] * r, lo[7] * r));
+            // B[k][col] of -8 sum q / 2^8: k = block (hi part), 8 + block (lo part); the rest stays zero
             if (tt == 0) {
-              qstart[(nt * NB + blk) * 8 + cc] = sh * (-8.f / kTwo24);
-              qstart[(nt * NB + blk) * 8 + cc + 4] = sl * (-8.f / kTwo24);
+              uint16_t* z = reinterpret_cast<uint16_t*>(qzero + tile * 32 + cc * 4 + blk / 2) + (blk & 1);
+              const float v = sum * (-8.f / 256.f);
+              z[0] = f2h(v);
+              z[2] = f2h(v - h2f(z[0]));
             }
-          } else {
-            fh = make_uint4(pack2(hi[0], hi[1]), pack2(hi[2], hi[3]), pack2(hi[4], hi[5]), pack2(hi[6], hi[7]));
-            fl = make_uint4(pack2(lo[0], lo[1]), pack2(lo[2], lo[3]), pack2(lo[4], lo[5]), pack2(lo[6], lo[7]));
           }
-          qfrag[(nt * NB + blk) * 32 + cc * 4 + tt] = fh;
-          qfrag[(nt * NB + blk) * 32 + (cc + 4) * 4 + tt] = fl;
-          if (l == 0) qfac[c] = p.scale * 1.4426950408889634f * __uint_as_float((uint32_t)(127 - up) << 23) * (BITS == 4 ? kTwo24 : 1.f);
+          if (l == 0)
+            qfac[c] = p.scale * 1.4426950408889634f * __uint_as_float((uint32_t)(127 - up) << 23);
         }
       }
     }
-    __syncthreads();
-    float m[NT][2], lsum[NT][2], fac[NT][2];
+    consumers();
+    float top[NT][2], lsum[NT][2], fac[NT][2], lift = kLift;  // largest score so far; sum of p; score factor
     bool live[NT];
     uint32_t pos[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
-      pos[nt] = seg.pmin + (p.G > 4 ? 0 : nt);
-      live[nt] = pos[nt] <= seg.pmax;
+      const int tile = wc * NT + nt;
+      pos[nt] = u.pmin + col_row(tile * 4);
+      live[nt] = (uint32_t)col_row(tile * 4) < u.nrows && col_head(tile * 4) < p.G;
 #pragma unroll
-      for (int j = 0; j < 2; j++) {
-        m[nt][j] = -INFINITY;
-        lsum[nt][j] = 0.f;
-        fac[nt][j] = qfac[nt * 4 + 2 * (t & 1) + j];
+      for (int i = 0; i < 2; i++) {
+        top[nt][i] = -INFINITY;
+        lsum[nt][i] = 0.f;
+        fac[nt][i] = qfac[tile * 4 + 2 * (t & 1) + i];
       }
 #pragma unroll
-      for (int i = 0; i < TILES; i++)
+      for (int i = 0; i < OT; i++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) O[nt][i][j] = 0.f;
+        for (int k = 0; k < 4; k++) O[nt][i][k] = 0.f;
     }
-    if constexpr (NT == 1) {
-#pragma unroll
-      for (int b = 0; b < NB; b++) {
-        qreg[b] = qfrag[b * 32 + lane];
-        if constexpr (BITS == 4) creg[b][0] = qstart[b * 8 + 2 * t], creg[b][1] = qstart[b * 8 + 2 * t + 1];
-      }
-    }
+    const uint4* qf = qfrag + (size_t)wc * NT * NB * 32 + lane;
 
-    for (uint32_t k = seg.k0 + warp; k < seg.k1; k += W) {
-      const uint32_t piece = w.range.at(k);
-      if (!seg.needs(p, piece)) continue;
-      const uint32_t st = used % ST;
-      if (alive) alive = __all_sync(0xffffffffu, mbar_wait(&bars[warp * ST + st], (used / ST) & 1u, p.d.status));
-      if (alive) used++;
-      const bool here = alive && loaded[warp * ST + st] != 0;
-      const uint8_t* kp = ring + (size_t)(warp * ST + st) * Sh::STAGE;
+    const uint32_t turn = j0 % WS;   // group (j % WS) takes the CTA's piece j
+    for (uint32_t i = (uint32_t)ws >= turn ? ws - turn : ws + WS - turn; i < u.span.count; i += WS) {
+      const uint32_t j = j0 + i, st = j % S, t0 = u.span.at(i) * kPieceSlots;
+      if (alive) alive = __all_sync(0xffffffffu, mbar_wait(&landed[st], (j / S) & 1u, p.d.status));
+      const bool here = alive && usable[st] != 0;
+      const uint8_t* kp = ring + (size_t)st * Sh::STAGE;
       const uint8_t* vp = kp + PB;
-      const uint32_t t0 = piece * kPieceSlots;
 
       // ---- scores
       float s[NT][4];
-#pragma unroll
-      for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) s[nt][j] = 0.f;
       if constexpr (BITS == 4) {
         constexpr int RUN = NB < 4 ? NB : 4;
         uint32_t da[NB / 2], db[NB / 2];                 // scales of slots g, g + 8
         lds_words<NB / 2>(da, kp + g * NB * 2);
         lds_words<NB / 2>(db, kp + (g + 8) * NB * 2);
+        float z[NT][4];
+        const uint32_t dz0 = t < NB / 2 ? *reinterpret_cast<const uint32_t*>(kp + g * NB * 2 + t * 4) : 0u;
+        const uint32_t dz1 = t < NB / 2 ? *reinterpret_cast<const uint32_t*>(kp + (g + 8) * NB * 2 + t * 4) : 0u;
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+          const uint2 zb = qzero[(wc * NT + nt) * 32 + lane];
+          mma16816_zero(z[nt], dz0, dz1, dz0, dz1, zb.x, zb.y);
+#pragma unroll
+          for (int k = 0; k < 4; k++) s[nt][k] = 0.f;
+        }
 #pragma unroll
         for (int r = 0; r < NB / RUN; r++) {
           uint32_t wa[RUN], wb[RUN];
           lds_words<RUN>(wa, kp + HD + ((r * 16 + g) * 4 + t) * (RUN * 4));
           lds_words<RUN>(wb, kp + HD + ((r * 16 + g + 8) * 4 + t) * (RUN * 4));
 #pragma unroll
-          for (int i = 0; i < RUN; i++) {
-            const int b = r * RUN + i;
-            const uint32_t sa = wa[i] >> 8, sb = wb[i] >> 8;
+          for (int q = 0; q < RUN; q++) {
+            const int b = r * RUN + q;
+            const uint32_t sa = wa[q] >> 8, sb = wb[q] >> 8;
             const float d0 = h2f((uint16_t)(da[b / 2] >> (16 * (b & 1)))), d1 = h2f((uint16_t)(db[b / 2] >> (16 * (b & 1))));
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
               if (NT > 1 && !live[nt]) continue;
-              uint4 qb;
+              const uint4 qb = qf[(nt * NB + b) * 32];
               float acc[4];
-              if constexpr (NT == 1) {
-                qb = qreg[b];
-                acc[0] = acc[2] = creg[b][0];
-                acc[1] = acc[3] = creg[b][1];
-              } else {
-                qb = qfrag[(nt * NB + b) * 32 + lane];
-                const float2 c2 = *reinterpret_cast<const float2*>(&qstart[(nt * NB + b) * 8 + 2 * t]);
-                acc[0] = acc[2] = c2.x;
-                acc[1] = acc[3] = c2.y;
-              }
-              mma16816(acc, wa[i] & kLowCodes, wb[i] & kLowCodes, sa & kLowCodes, sb & kLowCodes, qb.x, qb.y);
-              mma16816(acc, wa[i] & kHighCodes, wb[i] & kHighCodes, sa & kHighCodes, sb & kHighCodes, qb.z, qb.w);
+              mma16816_zero(acc, wa[q] & kLowCodes, wb[q] & kLowCodes, sa & kLowCodes, sb & kLowCodes, qb.x, qb.y);
+              mma16816(acc, wa[q] & kHighCodes, wb[q] & kHighCodes, sa & kHighCodes, sb & kHighCodes, qb.z, qb.w);
               s[nt][0] = fmaf(d0, acc[0], s[nt][0]);
               s[nt][1] = fmaf(d0, acc[1], s[nt][1]);
               s[nt][2] = fmaf(d1, acc[2], s[nt][2]);
@@ -424,21 +514,50 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, 1) k_attn_paged(
             }
           }
         }
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+          for (int k = 0; k < 4; k++) s[nt][k] = fmaf(s[nt][k], kTwo24, z[nt][k] * 256.f);
       } else {
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+          for (int k = 0; k < 4; k++) s[nt][k] = 0.f;
 #pragma unroll
         for (int b = 0; b < NB; b++) {
           const uint4 wa = lds128(kp + (b * 16 + g) * 64 + t * 16), wb = lds128(kp + (b * 16 + g + 8) * 64 + t * 16);
 #pragma unroll
           for (int nt = 0; nt < NT; nt++) {
             if (NT > 1 && !live[nt]) continue;
-            uint4 qb;
-            if constexpr (NT == 1) qb = qreg[b];
-            else qb = qfrag[(nt * NB + b) * 32 + lane];
-            float acc[4] = {0.f, 0.f, 0.f, 0.f};
-            mma16816(acc, wa.x, wb.x, wa.y, wb.y, qb.x, qb.y);
+            const uint4 qb = qf[(nt * NB + b) * 32];
+            float acc[4];
+            mma16816_zero(acc, wa.x, wb.x, wa.y, wb.y, qb.x, qb.y);
             mma16816(acc, wa.z, wb.z, wa.w, wb.w, qb.z, qb.w);
 #pragma unroll
-            for (int j = 0; j < 4; j++) s[nt][j] += acc[j];
+            for (int k = 0; k < 4; k++) s[nt][k] += acc[k];
+          }
+        }
+      }
+
+      // ---- value scales of slots (2t, 2t+1) and (2t+8, 2t+9); one of 2 or more ends the lift of p
+      uint32_t dv[BITS == 4 ? NB : 1][2];
+      if constexpr (BITS == 4) {
+        uint32_t any = 0;
+#pragma unroll
+        for (int b = 0; b < NB; b += 2) {
+          const uint4 d4 = lds128(vp + (t * NB + b) * 8);
+          dv[b][0] = d4.x, dv[b][1] = d4.y, dv[b + 1][0] = d4.z, dv[b + 1][1] = d4.w;
+          any |= d4.x | d4.y | d4.z | d4.w;
+        }
+        if (__any_sync(0xffffffffu, (any & 0x40004000u) != 0) && lift != 0.f) {
+          lift = 0.f;
+#pragma unroll
+          for (int nt = 0; nt < NT; nt++) {
+            lsum[nt][0] *= 1.f / 16384.f, lsum[nt][1] *= 1.f / 16384.f;
+#pragma unroll
+            for (int o = 0; o < OT; o++)
+#pragma unroll
+              for (int k = 0; k < 4; k++) O[nt][o][k] *= 1.f / 16384.f;
           }
         }
       }
@@ -453,9 +572,9 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, 1) k_attn_paged(
         if (NT > 1 && !live[nt]) continue;
         float v[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          s[nt][j] += __shfl_xor_sync(0xffffffffu, s[nt][j], 2);     // hi + lo columns
-          v[j] = s[nt][j] * fac[nt][j & 1];
+        for (int k = 0; k < 4; k++) {
+          s[nt][k] += __shfl_xor_sync(0xffffffffu, s[nt][k], 2);     // hi + lo columns
+          v[k] = s[nt][k] * fac[nt][k & 1];
         }
         bool va = true, vb = true;
         if (!full[nt]) {
@@ -465,29 +584,30 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, 1) k_attn_paged(
           if (!vb) v[2] = v[3] = -INFINITY;
           keep[nt][0] = keep[nt][1] = 0;
 #pragma unroll
-          for (int j = 0; j < 4; j++)
-            if (here && slot_visible(t0 + 2 * t + (j & 1) + 8 * (j >> 1), pos[nt], p.window, p.sinks))
-              keep[nt][j >> 1] |= 0xffffu << (16 * (j & 1));
+          for (int k = 0; k < 4; k++)
+            if (here && slot_visible(t0 + 2 * t + (k & 1) + 8 * (k >> 1), pos[nt], p.window, p.sinks))
+              keep[nt][k >> 1] |= 0xffffu << (16 * (k & 1));
         }
-        const bool grow = v[0] > m[nt][0] || v[2] > m[nt][0] || v[1] > m[nt][1] || v[3] > m[nt][1];
+        const bool grow = v[0] > top[nt][0] || v[2] > top[nt][0] || v[1] > top[nt][1] || v[3] > top[nt][1];
         if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-          for (int j = 0; j < 2; j++) {
-            float n = fmaxf(v[j], v[j + 2]);
+          for (int k = 0; k < 2; k++) {
+            float n = fmaxf(v[k], v[k + 2]);
             n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, 4));
             n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, 8));
             n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, 16));
-            n = fmaxf(n, m[nt][j]);
-            const float a = n == m[nt][j] ? 1.f : ex2(m[nt][j] - n);
-            m[nt][j] = n;
-            lsum[nt][j] *= a;
+            n = fmaxf(n, top[nt][k]);
+            const float a = n == top[nt][k] ? 1.f : ex2(top[nt][k] - n);
+            top[nt][k] = n;
+            lsum[nt][k] *= a;
 #pragma unroll
-            for (int i = 0; i < TILES; i++) O[nt][i][j] *= a, O[nt][i][j + 2] *= a;
+            for (int o = 0; o < OT; o++) O[nt][o][k] *= a, O[nt][o][k + 2] *= a;
           }
         }
         float e[4];
+        const float ref[2] = {top[nt][0] - lift, top[nt][1] - lift};
 #pragma unroll
-        for (int j = 0; j < 4; j++) e[j] = ex2(v[j] - m[nt][j & 1]);
+        for (int k = 0; k < 4; k++) e[k] = ex2(v[k] - ref[k & 1]);
         if (!full[nt]) {
           if (!va) e[0] = e[1] = 0.f;
           if (!vb) e[2] = e[3] = 0.f;
@@ -495,15 +615,15 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, 1) k_attn_paged(
         lsum[nt][0] += e[0] + e[2];
         lsum[nt][1] += e[1] + e[3];
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-          const uint32_t h = pack2(e[2 * j], e[2 * j + 1]);
+        for (int k = 0; k < 2; k++) {
+          const uint32_t h = pack2(e[2 * k], e[2 * k + 1]);
           const float2 hf = __half22float2(*reinterpret_cast<const __half2*>(&h));
-          const uint32_t l = pack2(e[2 * j] - hf.x, e[2 * j + 1] - hf.y);
+          const uint32_t l = pack2(e[2 * k] - hf.x, e[2 * k + 1] - hf.y);
           if constexpr (BITS == 4) {
-            ph[nt][j] = transpose8x8(h);
-            pl[nt][j] = transpose8x8(l);
+            ph[nt][k] = transpose8x8(h);
+            pl[nt][k] = transpose8x8(l);
           } else {
-            ph[nt][j] = transpose8x8(t < 2 ? h : l);      // columns 0-3 hi, 4-7 lo
+            ph[nt][k] = transpose8x8(t < 2 ? h : l);      // columns 0-3 hi, 4-7 lo
           }
         }
       }
@@ -512,174 +632,187 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, 1) k_attn_paged(
       if constexpr (BITS == 4) {
         uint32_t vw[4][NB / 2];
 #pragma unroll
-        for (int i = 0; i < 4; i++) lds_words<NB / 2>(vw[i], vp + HD + (i * 32 + lane) * (NB * 2));
+        for (int k = 0; k < 4; k++) lds_words<NB / 2>(vw[k], vp + HD + (k * 32 + lane) * (NB * 2));
 #pragma unroll
         for (int b = 0; b < NB; b++) {
-          const uint2 d2 = *reinterpret_cast<const uint2*>(vp + (t * NB + b) * 8);
           const uint32_t sel = b & 1 ? 0x7632u : 0x5410u;
           const uint32_t x = __byte_perm(vw[0][b / 2], vw[1][b / 2], sel), y = __byte_perm(vw[2][b / 2], vw[3][b / 2], sel);
           const uint32_t xs = x >> 8, ys = y >> 8;
+          const uint32_t al[4] = {low_codes(x), low_codes(xs), low_codes(y), low_codes(ys)};
+          const uint32_t ah[4] = {high_codes(x), high_codes(xs), high_codes(y), high_codes(ys)};
 #pragma unroll
           for (int nt = 0; nt < NT; nt++) {
             if (NT > 1 && !live[nt]) continue;
             uint32_t bb[2];
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
-              uint32_t d = j ? d2.y : d2.x;
-              if (!full[nt]) d &= keep[nt][j];
-              const uint32_t hi = hmul2(ph[nt][j], d);
-              const uint32_t lo = hfma2(pl[nt][j], d, hfma2(ph[nt][j], d, hi ^ 0x80008000u));
-              bb[j] = g < 4 ? hi : lo;
+            for (int k = 0; k < 2; k++) {
+              uint32_t d = dv[b][k];
+              if (!full[nt]) d &= keep[nt][k];
+              const uint32_t hi = hmul2(ph[nt][k], d);
+              const uint32_t lo = hfma2(pl[nt][k], d, hfms2(ph[nt][k], d, hi));
+              bb[k] = g < 4 ? hi : lo;
             }
-            mma16816(O[nt][2 * b], x & kLowCodes, xs & kLowCodes, y & kLowCodes, ys & kLowCodes, bb[0], bb[1]);
-            mma16816(O[nt][2 * b + 1], x & kHighCodes, xs & kHighCodes, y & kHighCodes, ys & kHighCodes, bb[0], bb[1]);
-            mma16816(O[nt][2 * b], kMinus8Low, kMinus8Low, kMinus8Low, kMinus8Low, bb[0], bb[1]);
-            mma16816(O[nt][2 * b + 1], kMinus8High, kMinus8High, kMinus8High, kMinus8High, bb[0], bb[1]);
+            mma16816(O[nt][2 * b], al[0], al[1], al[2], al[3], bb[0], bb[1]);
+            mma16816(O[nt][2 * b + 1], ah[0], ah[1], ah[2], ah[3], bb[0], bb[1]);
           }
         }
       } else {
 #pragma unroll
-        for (int j = 0; j < HD / 64; j++) {
+        for (int q = 0; q < HD / 64; q++) {
           uint32_t vw[4][4];
 #pragma unroll
-          for (int i = 0; i < 4; i++) lds_words<4>(vw[i], vp + ((j * 4 + i) * 32 + lane) * 16);
+          for (int k = 0; k < 4; k++) lds_words<4>(vw[k], vp + ((q * 4 + k) * 32 + lane) * 16);
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const uint32_t a0 = __byte_perm(vw[0][i], vw[1][i], 0x5410), a1 = __byte_perm(vw[0][i], vw[1][i], 0x7632);
-            const uint32_t a2 = __byte_perm(vw[2][i], vw[3][i], 0x5410), a3 = __byte_perm(vw[2][i], vw[3][i], 0x7632);
+          for (int k = 0; k < 4; k++) {
+            const uint32_t a0 = __byte_perm(vw[0][k], vw[1][k], 0x5410), a1 = __byte_perm(vw[0][k], vw[1][k], 0x7632);
+            const uint32_t a2 = __byte_perm(vw[2][k], vw[3][k], 0x5410), a3 = __byte_perm(vw[2][k], vw[3][k], 0x7632);
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
               if (NT > 1 && !live[nt]) continue;
-              if (full[nt]) mma16816(O[nt][4 * j + i], a0, a1, a2, a3, ph[nt][0], ph[nt][1]);
+              if (full[nt]) mma16816(O[nt][4 * q + k], a0, a1, a2, a3, ph[nt][0], ph[nt][1]);
               else
-                mma16816(O[nt][4 * j + i], a0 & keep[nt][0], a1 & keep[nt][0], a2 & keep[nt][1], a3 & keep[nt][1],
+                mma16816(O[nt][4 * q + k], a0 & keep[nt][0], a1 & keep[nt][0], a2 & keep[nt][1], a3 & keep[nt][1],
                          ph[nt][0], ph[nt][1]);
             }
           }
         }
       }
       __syncwarp();
-      if (alive) issue();
+      if (lane == 0 && alive) mbar_arrive_n(&freed[st], WS);
     }
+    j0 += u.span.count;
 
-    // ---- the warps' states, merged
+    // ---- the warps' states
+    consumers();                     // the q fragments have been read
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
-      for (int j = 0; j < 2; j++) {
-        float l = lsum[nt][j];
+      for (int k = 0; k < 2; k++) {
+        float l = lsum[nt][k];
         l += __shfl_xor_sync(0xffffffffu, l, 4);
         l += __shfl_xor_sync(0xffffffffu, l, 8);
         l += __shfl_xor_sync(0xffffffffu, l, 16);
         if (lane < 2) {
-          ml[(warp * COLS + nt * 4 + 2 * t + j) * 2] = m[nt][j];
-          ml[(warp * COLS + nt * 4 + 2 * t + j) * 2 + 1] = l;
+          ml[(warp * LC + nt * 4 + 2 * t + k) * 2] = top[nt][k] - lift;
+          ml[(warp * LC + nt * 4 + 2 * t + k) * 2 + 1] = l;
         }
       }
 #pragma unroll
-      for (int i = 0; i < TILES; i++)
+      for (int o = 0; o < OT; o++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          float o = O[nt][i][j];
-          o += __shfl_xor_sync(0xffffffffu, o, 2);
-          int dim;
-          if constexpr (BITS == 4) {
-            o *= i & 1 ? kTwo20 : kTwo24;
-            dim = (i / 2) * 32 + 4 * g + (i & 1) + 2 * (j >> 1);
-          } else {
-            dim = (i / 4) * 64 + 8 * g + 2 * (i & 3) + (j >> 1);
-          }
-          if (t < 2) merge[(size_t)(warp * COLS + nt * 4 + 2 * t + (j & 1)) * HD + dim] = o;
+        for (int k = 0; k < 4; k++) {
+          const float x = O[nt][o][k] + __shfl_xor_sync(0xffffffffu, O[nt][o][k], 2);
+          const int dim = BITS == 4 ? (o / 2) * 32 + 4 * g + (o & 1) + 2 * (k >> 1)
+                                    : (o / 4) * 64 + 8 * g + 2 * (o & 3) + (k >> 1);
+          if (t < 2) merge[(size_t)(warp * LC + nt * 4 + 2 * t + (k & 1)) * HD + dim] = x;
         }
     }
-    __syncthreads();
-    const bool whole = seg.k0 == 0 && seg.k1 == w.np;
-    const uint64_t unit_end = seg.unit0 + w.np;
-    const uint32_t c0 = (uint32_t)(((seg.unit0 + 1) * C - 1) / T), c1 = (uint32_t)((unit_end * C - 1) / T);
-    const uint32_t row0 = (p.d.rows ? p.d.rows[seg.s] : (uint32_t)seg.s) + (seg.pmin - w.p0);
-    const auto finish = [&](int c, int dim, float o, float M, float L) {
-      const int head = seg.kvh * p.G + (p.G > 4 ? c : c & 3);
-      const size_t row = row0 + (p.G > 4 ? 0 : c >> 2);
-      const float val = L != 0.f ? o / L : 0.f;          // a NaN sum stays one
-      if (p.out_f) p.out_f[(row * p.QH + head) * HD + dim] = val;
-      if (p.out_h)
-        p.out_h[row * p.QH * HD + (p.xfo ? xfo_pos(head * HD + dim) : head * HD + dim)] = f2h(val);
+    consumers();
+    const uint32_t c0 = (uint32_t)(((u.unit0 + 1) * C - 1) / T), c1 = (uint32_t)((u.unit1 * C - 1) / T);
+    const bool whole = c0 == c1;
+    const auto finish = [&](int c, int dim, const float4& o, float M, float L) {
+      const int head = u.kvh * p.G + col_head(c);
+      const size_t row = row0 + col_row(c);
+      const float r = L != 0.f ? 1.f / L : 0.f;          // a NaN sum stays one
+      const float4 x = make_float4(o.x * r, o.y * r, o.z * r, o.w * r);
+      if (p.out_f) *reinterpret_cast<float4*>(p.out_f + (row * p.QH + head) * HD + dim) = x;
+      if (p.out_h) {
+        uint16_t* out = p.out_h + row * p.QH * HD;
+        const int at = head * HD + dim;
+        if (p.xfo) {
+          out[xfo_pos(at)] = f2h(x.x), out[xfo_pos(at + 1)] = f2h(x.y);
+          out[xfo_pos(at + 2)] = f2h(x.z), out[xfo_pos(at + 3)] = f2h(x.w);
+        } else {
+          *reinterpret_cast<uint2*>(out + at) = make_uint2(pack2(x.x, x.y), pack2(x.z, x.w));
+        }
+      }
       if (p.lse && dim == 0) p.lse[row * p.QH + head] = L != 0.f ? (M + log2f(L)) * 0.6931471805599453f : -INFINITY;
     };
-    const auto col_live = [&](int c) {
-      return p.G > 4 ? c < p.G : (c & 3) < p.G && seg.pmin + (c >> 2) <= seg.pmax;
-    };
-    for (int e = tid; e < COLS * HD; e += THREADS) {
-      const int c = e / HD, dim = e % HD;
+    float* part = p.parts + (2 * (size_t)cta + (first ? 0 : 1)) * kPartFloats;
+    for (int e = tid; e < cols * (HD / 4); e += CT) {
+      const int c = e / (HD / 4), dim = e % (HD / 4) * 4;
       if (!col_live(c)) continue;
-      float M = -INFINITY, o = 0.f, L = 0.f;
-#pragma unroll
-      for (int i = 0; i < W; i++) M = fmaxf(M, ml[(i * COLS + c) * 2]);
-#pragma unroll
-      for (int i = 0; i < W; i++) {
-        const float mi = ml[(i * COLS + c) * 2], a = mi == M ? 1.f : ex2(mi - M);
-        L = fmaf(a, ml[(i * COLS + c) * 2 + 1], L);
-        o = fmaf(a, merge[(size_t)(i * COLS + c) * HD + dim], o);
+      const int w0 = (c >> 2) / NT, lc = ((c >> 2) % NT) * 4 + (c & 3);
+      float M = -INFINITY, L = 0.f;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (uint32_t i = 0; i < WS; i++) M = fmaxf(M, ml[((i * WC + w0) * LC + lc) * 2]);
+      for (uint32_t i = 0; i < WS; i++) {
+        const int at = (i * WC + w0) * LC + lc;
+        const float mi = ml[at * 2], a = mi == M ? 1.f : ex2(mi - M);
+        const float4 x = *reinterpret_cast<const float4*>(merge + (size_t)at * HD + dim);
+        L = fmaf(a, ml[at * 2 + 1], L);
+        o.x = fmaf(a, x.x, o.x), o.y = fmaf(a, x.y, o.y), o.z = fmaf(a, x.z, o.z), o.w = fmaf(a, x.w, o.w);
       }
       if (whole) {
         finish(c, dim, o, M, L);
       } else {
-        float* part = p.parts + (2 * (size_t)cta + (first ? 0 : 1)) * kPartFloats;
-        part[c * HD + dim] = o;
-        if (dim == 0) part[kCols * 256 + 2 * c] = M, part[kCols * 256 + 2 * c + 1] = L;
+        *reinterpret_cast<float4*>(part + c * HD + dim) = o;
+        if (dim == 0) part[kMaxCols * 256 + 2 * c] = M, part[kMaxCols * 256 + 2 * c + 1] = L;
       }
     }
     if (!whole) {
-      // a unit cut between CTAs c0..c1: only c0 may hold it behind other segments
+      // a unit cut between CTAs c0..c1: only c0 may hold it behind other units
+      const uint32_t n = c1 - c0 + 1;
       __threadfence();
-      __syncthreads();
+      consumers();
       if (tid == 0) {
-        const uint32_t n = c1 - c0;
-        last_one = atomicInc(&p.arrived[c0], n) == n;    // wraps to zero with the last arrival
+        last_one = atomicInc(&p.arrived[c0], n - 1) == n - 1;        // wraps to zero with the last arrival
         __threadfence();
       }
-      __syncthreads();
+      consumers();
       if (last_one) {
-        const uint32_t n = c1 - c0 + 1;
-        const uint64_t c0_begin = T * c0 / C;
+        const bool behind = udiv(T * c0, C) != u.unit0;
         const auto part_of = [&](uint32_t i) {
-          return p.parts + (2 * (size_t)(c0 + i) + (i == 0 && c0_begin != seg.unit0 ? 1 : 0)) * kPartFloats;
+          return p.parts + (2 * (size_t)(c0 + i) + (i == 0 && behind ? 1 : 0)) * kPartFloats;
         };
-        for (int c = 0; c < COLS; c++) {
+        // a warp takes 128 dims of a column, a lane four of them
+        constexpr int kSplit = HD > 128 ? HD / 128 : 1;
+        float* wt = weight[warp];
+        for (int task = warp; task < cols * kSplit; task += W) {
+          const int c = task / kSplit, dim = (task % kSplit) * 128 + lane * 4;
           if (!col_live(c)) continue;
-          if (warp == 0) {
-            float M = -INFINITY, L = 0.f;
-            for (uint32_t i = lane; i < n; i += 32) M = fmaxf(M, __ldcg(&part_of(i)[kCols * 256 + 2 * c]));
-            M = warp_max(M);
-            for (uint32_t i = 0; i < n; i++) {
-              const float mi = __ldcg(&part_of(i)[kCols * 256 + 2 * c]), li = __ldcg(&part_of(i)[kCols * 256 + 2 * c + 1]);
-              const float a = mi == M ? 1.f : ex2(mi - M);
-              if (lane == 0) weight[i] = a;
-              L = fmaf(a, li, L);
+          float M = -INFINITY, L = 0.f;
+          for (uint32_t i = lane; i < n; i += 32) {
+            wt[i] = __ldcg(part_of(i) + kMaxCols * 256 + 2 * c);
+            M = fmaxf(M, wt[i]);
+          }
+          M = warp_max(M);
+          for (uint32_t i = lane; i < n; i += 32) {
+            wt[i] = wt[i] == M ? 1.f : ex2(wt[i] - M);
+            L = fmaf(wt[i], __ldcg(part_of(i) + kMaxCols * 256 + 2 * c + 1), L);
+          }
+          L = warp_sum(L);
+          __syncwarp();
+          float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (dim < HD) {
+#pragma unroll 1
+            for (uint32_t i0 = 0; i0 < n; i0 += 8) {      // eight parts' loads in flight
+              float4 x[8];
+#pragma unroll
+              for (int i = 0; i < 8; i++)
+                x[i] = __ldcg(reinterpret_cast<const float4*>(part_of(min(i0 + i, n - 1)) + c * HD + dim));
+#pragma unroll
+              for (int i = 0; i < 8; i++) {
+                const float a = i0 + i < n ? wt[i0 + i] : 0.f;
+                o.x = fmaf(a, x[i].x, o.x), o.y = fmaf(a, x[i].y, o.y);
+                o.z = fmaf(a, x[i].z, o.z), o.w = fmaf(a, x[i].w, o.w);
+              }
             }
-            if (lane == 0) fin[0] = M, fin[1] = L;
           }
-          __syncthreads();
-          for (int dim = tid; dim < HD; dim += THREADS) {
-            float o = 0.f;
-            for (uint32_t i = 0; i < n; i++) o = fmaf(weight[i], __ldcg(&part_of(i)[c * HD + dim]), o);
-            finish(c, dim, o, fin[0], fin[1]);
-          }
-          __syncthreads();
+          __syncwarp();
+          if (dim < HD) finish(c, dim, o, M, L);
         }
       }
     }
     first = false;
-    __syncthreads();                 // q fragments, merge buffer and states are free again
+    consumers();                     // the merge buffer and the states are free again
   }
-  // after a time-out: copies still in flight land (bounded) before the CTA exits
-  for (; used < issued; used++) mbar_wait(&bars[warp * ST + used % ST], (used / ST) & 1u, p.d.status);
 }
 
 template <int BITS, int HD, int NT>
 int launch(e4b_ctx* c, const AttnP& p) {
   using Sh = Shape<BITS, HD, NT>;
-  static_assert(Sh::SMEM < 226 * 1024, "shared memory");
+  static_assert(Sh::SMEM + 14 * 1024 < 227 * 1024, "shared memory");
   E4B_CUDA(c, cudaFuncSetAttribute(k_attn_paged<BITS, HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Sh::SMEM));
   const int ctas = c->sm_count < kMaxCtas ? c->sm_count : kMaxCtas;
   return e4b_launch(c, "attn_paged", k_attn_paged<BITS, HD, NT>, dim3(ctas), dim3(Sh::THREADS), Sh::SMEM, p);
@@ -692,12 +825,14 @@ int launch_hd(e4b_ctx* c, const AttnP& p, int HD) {
 
 extern "C" {
 
-E4B_API size_t e4b_paged_scratch_bytes(void) { return kMaxCtas * sizeof(uint32_t) + 2 * kMaxCtas * kPartFloats * sizeof(float); }
+E4B_API size_t e4b_paged_scratch_bytes(void) {
+  return kMaxCtas * sizeof(uint32_t) + 2 * kMaxCtas * kPartFloats * sizeof(float);
+}
 
 E4B_API int e4b_attn_paged(e4b_ctx* c, const e4b_paged_kv* kv, const float* q, uint16_t* out_h, float* out_f,
                            float* lse, void* scratch, int QH, int window, int sinks, float scale, int xfo, int n_rows) {
   E4B_CHECK_CTX(c);
-  const char* fault = attn_paged_fault(kv, q, out_h, out_f, scratch, QH, window, sinks, scale, xfo, n_rows);
+  const char* fault = attn_paged_fault(kv, q, out_h, out_f, lse, scratch, QH, window, sinks, scale, xfo, n_rows);
   E4B_REQUIRE(c, !fault, "attn_paged: %s", fault);
   if (n_rows == 0) return E4B_OK;
   AttnP p;
@@ -714,10 +849,9 @@ E4B_API int e4b_attn_paged(e4b_ctx* c, const e4b_paged_kv* kv, const float* q, u
   p.window = (uint32_t)window;
   p.sinks = (uint32_t)sinks;
   p.scale = scale;
-  // n-tiles of 4 heads: one row per unit, or two rows that share the decoded keys
-  // and values when a sequence may have several; more than 4 heads take both tiles
+  // a warp's n-tiles of 4 heads: one, or two where a sequence may have several rows
+  // (they share the decoded keys and values) and for more than 4 heads
   const int NT = p.G > 4 || kv->rows ? 2 : 1;
-  p.per_unit = p.G > 4 ? 1 : NT;
   if (kv->bits == 16) return NT == 1 ? launch_hd<16, 1>(c, p, kv->head_dim) : launch_hd<16, 2>(c, p, kv->head_dim);
   return NT == 1 ? launch_hd<4, 1>(c, p, kv->head_dim) : launch_hd<4, 2>(c, p, kv->head_dim);
 }

@@ -70,6 +70,32 @@ E4B_HD PieceRange piece_range(uint32_t p0, uint32_t p1, uint32_t window, uint32_
   return r;
 }
 
+// Of the pieces r.at(k0) .. r.at(k1 - 1), those that the queries at positions p0..p1
+// need, p0 and p1 among the positions that r was made for: `count` of them, the
+// i-th at at(i).
+struct PieceSpan {
+  uint32_t head, tail, first, count;
+  E4B_HD uint32_t at(uint32_t i) const {
+    const uint32_t n = first + i;
+    return n < head ? n : tail + (n - head);
+  }
+};
+E4B_HD PieceSpan piece_span(const PieceRange& r, uint32_t k0, uint32_t k1, uint32_t p0, uint32_t p1, uint32_t window,
+                            uint32_t sinks) {
+  const PieceRange u = piece_range(p0, p1, window, sinks);
+  PieceSpan s;
+  s.head = u.head;
+  s.tail = u.tail;
+  s.first = s.count = 0;
+  if (k0 >= k1) return s;
+  const uint32_t lo = r.at(k0), hi = r.at(k1 - 1) + 1;   // pieces lo <= p < hi
+  const uint32_t a = lo < u.head ? lo : (lo <= u.tail ? u.head : u.head + (lo - u.tail));
+  const uint32_t b = hi < u.head ? hi : (hi <= u.tail ? u.head : u.head + (hi - u.tail));
+  s.first = a;
+  s.count = (b < u.count ? b : u.count) > a ? (b < u.count ? b : u.count) - a : 0;
+  return s;
+}
+
 // ---- checks of the descriptor; a message, or NULL when it is usable.
 inline const char* paged_fault(const e4b_paged_kv* kv) {
   if (!kv) return "null cache descriptor";
@@ -118,7 +144,7 @@ inline const char* kvread_paged_fault(const e4b_paged_kv* kv, const void* k_out,
   return nullptr;
 }
 inline const char* attn_paged_fault(const e4b_paged_kv* kv, const float* q, const uint16_t* out_h, const float* out_f,
-                                    const void* scratch, int QH, int window, int sinks, float scale, int xfo,
+                                    const float* lse, const void* scratch, int QH, int window, int sinks, float scale, int xfo,
                                     int n_rows) {
   if (const char* m = paged_fault(kv)) return m;
   if (const char* m = paged_rows_fault(kv, n_rows)) return m;
@@ -127,8 +153,9 @@ inline const char* attn_paged_fault(const e4b_paged_kv* kv, const float* q, cons
   if (window < 0 || sinks < 0) return "negative window or sinks";
   if (!(scale == scale) || scale > 3e38f || scale < -3e38f) return "scale must be finite";
   if (xfo && !out_h) return "fragment order is an order of out_h";
-  if (((uintptr_t)q | (uintptr_t)scratch) % 16 != 0 || (uintptr_t)out_h % 2 != 0 || (uintptr_t)out_f % 4 != 0)
-    return "q and scratch must be 16-byte aligned";
+  if (((uintptr_t)q | (uintptr_t)scratch) % 16 != 0 || ((uintptr_t)out_h | (uintptr_t)out_f) % 16 != 0 ||
+      (uintptr_t)lse % 4 != 0)
+    return "q, outputs and scratch must be 16-byte aligned (lse: 4)";
   return nullptr;
 }
 

@@ -560,8 +560,9 @@ E4B_API int e4b_kvread_paged(e4b_ctx* ctx, const e4b_paged_kv* kv, void* k_out, 
  * that sees nothing gives zeros and lse = -inf.  Products carry f32 precision
  * (q and p as f16 hi + lo), sums are f32.  Pages wholly between the sinks and
  * the window are not read and need no valid id.  scratch: e4b_paged_scratch_bytes(),
- * 16-byte aligned, zeroed once before its first use (each call leaves it ready
- * for the next) and not shared by calls that may overlap.  QH/KVH <= 8. */
+ * zeroed once before its first use (each call leaves it ready for the next) and
+ * not shared by calls that may overlap.  q, outputs and scratch 16-byte aligned;
+ * QH/KVH <= 8; |q * scale| below 2^100. */
 E4B_API size_t e4b_paged_scratch_bytes(void);
 E4B_API int e4b_attn_paged(e4b_ctx* ctx, const e4b_paged_kv* kv, const float* q, uint16_t* out_h, float* out_f,
                            float* lse, void* scratch, int QH, int window, int sinks, float scale, int xfo, int n_rows);

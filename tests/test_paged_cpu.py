@@ -29,14 +29,19 @@ uint32_t range(uint32_t p0, uint32_t p1, uint32_t w, uint32_t n, uint32_t* out) 
   for (uint32_t k = 0; k < r.count; k++) out[k] = r.at(k);
   return r.count;
 }
+uint32_t span(uint32_t q0, uint32_t q1, uint32_t k0, uint32_t k1, uint32_t p0, uint32_t p1, uint32_t w, uint32_t n, uint32_t* out) {
+  PieceSpan s = piece_span(piece_range(q0, q1, w, n), k0, k1, p0, p1, w, n);
+  for (uint32_t i = 0; i < s.count; i++) out[i] = s.at(i);
+  return s.count;
+}
 const char* f_prep(const e4b_paged_kv* kv, const void* qkv, const float* qw, const float* kw, const float* q_out, int QH,
                    int angles, float theta, float eps, int norm, int keqv, int h, int stride, int parts, int n) {
   return headprep_paged_fault(kv, qkv, qw, kw, q_out, QH, angles, theta, eps, norm, keqv, h, stride, parts, n);
 }
 const char* f_read(const e4b_paged_kv* kv, const void* k, const void* v, int n) { return kvread_paged_fault(kv, k, v, n); }
-const char* f_attn(const e4b_paged_kv* kv, const float* q, const uint16_t* oh, const float* of, const void* sc, int QH,
-                   int w, int s, float scale, int xfo, int n) {
-  return attn_paged_fault(kv, q, oh, of, sc, QH, w, s, scale, xfo, n);
+const char* f_attn(const e4b_paged_kv* kv, const float* q, const uint16_t* oh, const float* of, const float* lse, const void* sc,
+                   int QH, int w, int s, float scale, int xfo, int n) {
+  return attn_paged_fault(kv, q, oh, of, lse, sc, QH, w, s, scale, xfo, n);
 }
 }
 """
@@ -109,6 +114,28 @@ def test_piece_range_covers_exactly_the_visible_slots(shim, window, sinks):
             assert bool(shim.seen(t, p, window, sinks)) == bool(op.visible(64, p, window, sinks)[t])
 
 
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1, 0), (1, 1), (16, 4), (17, 33), (40, 16), (40, 100), (5, 1000)])
+def test_piece_span_cuts_a_group_of_rows_out_of_a_run(shim, window, sinks):
+    """Cut anywhere, the parts of a group's pieces are each needed piece once, in order."""
+    out, whole = (ctypes.c_uint32 * 64)(), (ctypes.c_uint32 * 64)()
+    rng = np.random.default_rng(window + sinks)
+    for q0 in (0, 3, 15, 16, 100, 331):
+        for rows in (1, 7, 60):
+            q1 = q0 + rows - 1
+            n = shim.range(q0, q1, window, sinks, whole)
+            for p0 in range(q0, q1 + 1, 11):
+                p1 = min(q1, p0 + int(rng.integers(0, 20)))
+                m = shim.range(p0, p1, window, sinks, out)
+                want = list(out[:m])
+                cuts = [0] + sorted(int(x) for x in rng.integers(0, n + 1, 3)) + [n]
+                got = []
+                for a, b in zip(cuts, cuts[1:]):
+                    c = shim.span(q0, q1, a, b, p0, p1, window, sinks, out)
+                    assert all(x in list(whole[a:b]) for x in out[:c])
+                    got += list(out[:c])
+                assert got == want
+
+
 def test_visibility_at_the_far_end(shim):
     top = (1 << 31) - 2
     assert shim.seen(top, top, 1, 0) and not shim.seen(top - 1, top, 1, 0) and shim.seen(0, top, 1, 1)
@@ -138,10 +165,10 @@ def _prep(shim, kv, **o):
 
 
 def _attn(shim, kv, **o):
-    a = dict(q=4096, oh=4096, of=None, sc=4096, QH=8, w=0, s=0, scale=1.0, xfo=0, n=2)
+    a = dict(q=4096, oh=4096, of=None, lse=None, sc=4096, QH=8, w=0, s=0, scale=1.0, xfo=0, n=2)
     a.update(o)
     V = ctypes.c_void_p
-    return shim.f_attn(kv and ctypes.byref(kv), V(a["q"]), V(a["oh"]), V(a["of"]), V(a["sc"]), a["QH"], a["w"], a["s"],
+    return shim.f_attn(kv and ctypes.byref(kv), V(a["q"]), V(a["oh"]), V(a["of"]), V(a["lse"]), V(a["sc"]), a["QH"], a["w"], a["s"],
                        ctypes.c_float(a["scale"]), a["xfo"], a["n"])
 
 
@@ -178,7 +205,7 @@ def test_bad_arguments_are_refused(e4b, shim):
     assert _prep(shim, kv, keqv=1, stride=6 * 128) is None
     for bad in (dict(q=None), dict(q=4100), dict(oh=None), dict(sc=None), dict(sc=4104), dict(QH=0), dict(QH=3), dict(QH=18),
                 dict(w=-1), dict(s=-1), dict(scale=float("nan")), dict(scale=float("inf")), dict(n=1), dict(n=-2),
-                dict(oh=None, of=4096, xfo=1), dict(oh=4097), dict(of=4098)):
+                dict(oh=None, of=4096, xfo=1), dict(oh=4104), dict(of=4100), dict(lse=4098)):
         assert _attn(shim, kv, **bad), bad
     assert _attn(shim, ragged, n=-1) and _attn(shim, ragged, n=0) is None
     assert shim.f_read(ctypes.byref(kv), None, None, 2) and shim.f_read(ctypes.byref(kv), ctypes.c_void_p(8), None, 2)
@@ -206,7 +233,7 @@ def test_calls_reject_a_null_context_and_size_queries(e4b):
     assert L.e4b_paged_pool_bytes(16, 4096, 1 << 20, 8, 256) == (1 << 20) * 8 * 4096 * 512
     for bad in ((8, 64, 1, 1, 64), (4, 24, 1, 1, 64), (4, 64, 0, 1, 64), (4, 64, 1, 1, 96)):
         assert L.e4b_paged_pool_bytes(*bad) == 0
-    assert 0 < L.e4b_paged_scratch_bytes() <= 8 << 20
+    assert 0 < L.e4b_paged_scratch_bytes() <= 64 << 20
 
 
 def test_host_class_checks_its_tables(e4b):
