@@ -71,6 +71,8 @@ struct Shape {
   // warps (a warp then never waits for a phase before the stage's last one is done)
   static constexpr int S = NT == 1 ? W * (BITS == 16 ? (HD == 256 ? 1 : (HD == 128 ? 2 : 4)) : (HD == 256 ? 2 : (HD == 128 ? 4 : 6)))
                                    : W * (BITS == 16 ? (HD == 256 ? 1 : (HD == 128 ? 2 : 4)) : (HD == 64 ? 8 : 4));
+  // what a unit costs beside its pieces (q, the merge, the outputs), in pieces
+  static constexpr int U = BITS == 16 ? (HD == 256 ? 6 : (HD == 128 ? 8 : 12)) : (HD == 256 ? 12 : 16);
   static constexpr int LN = S <= 32 ? S : (NT == 1 ? 22 : 32);          // producer lanes; S is a multiple
   static constexpr int THREADS = 384, CT = 32 * W;
   static constexpr int TILES = W * NT;                                  // n-tiles of a unit at most
@@ -101,9 +103,9 @@ struct SeqWork {
   uint32_t p0, nq;                   // first row's position, rows
   PieceRange range;
   uint32_t full, tail_wc;            // units of W sharing warps, sharing warps of the last unit (0: none)
-  uint64_t cost;                     // sum over units and KV heads of pieces * sharing warps
+  uint64_t cost;                     // sum over units and KV heads of U + pieces * sharing warps
 };
-template <int W, int NT>
+template <int W, int NT, int U>
 E4B_DEV SeqWork seq_work(const AttnP& p, int s) {
   const Rows<W, NT> rows(p.G);
   SeqWork w;
@@ -122,17 +124,18 @@ E4B_DEV SeqWork seq_work(const AttnP& p, int s) {
     w.full = w.nq / rows.per_unit();
     const uint32_t rest = w.nq % rows.per_unit();
     w.tail_wc = rest ? rows.sharing(rest) : 0u;
-    w.cost = (uint64_t)w.range.count * p.d.KVH * ((uint64_t)w.full * W + w.tail_wc);
+    const uint64_t np = w.range.count;
+    w.cost = p.d.KVH * (w.full * (U + np * W) + (rest ? U + np * w.tail_wc : 0));
   }
   return w;
 }
 
-E4B_DEV uint64_t udiv(uint64_t a, uint32_t b) {
-  return (a >> 32) == 0 ? (uint64_t)((uint32_t)a / b) : a / b;
+E4B_DEV uint64_t udiv(uint64_t a, uint64_t b) {
+  return ((a | b) >> 32) == 0 ? (uint64_t)((uint32_t)a / (uint32_t)b) : a / b;
 }
 
 // Walks a CTA's run [g, end) of the work, unit by unit.
-template <int W, int NT>
+template <int W, int NT, int U>
 struct Walk {
   uint64_t g, end, base;             // base: where the current sequence's work begins
   int s;
@@ -149,31 +152,32 @@ struct Walk {
         g = end;
         return false;
       }
-      w = seq_work<W, NT>(p, s);
+      w = seq_work<W, NT, U>(p, s);
     }
     const Rows<W, NT> rows(p.G);
     const uint32_t KVH = p.d.KVH, np = w.range.count;
-    const uint64_t off = g - base, full_cost = (uint64_t)np * W * w.full * KVH;
+    const uint64_t off = g - base, full_cost = ((uint64_t)np * W + U) * w.full * KVH;
     uint32_t group, unit;
     if (off < full_cost) {
       wc = W;
-      unit = (uint32_t)udiv(off, np * W);
-      unit0 = base + (uint64_t)unit * np * W;
+      unit = (uint32_t)udiv(off, np * W + U);
+      unit0 = base + (uint64_t)unit * (np * W + U);
       group = unit / KVH;
       kvh = unit % KVH;
       nrows = rows.per_unit();
     } else {
       wc = w.tail_wc;
-      kvh = (uint32_t)udiv(off - full_cost, np * wc);
-      unit0 = base + full_cost + (uint64_t)kvh * np * wc;
+      kvh = (uint32_t)udiv(off - full_cost, np * wc + U);
+      unit0 = base + full_cost + (uint64_t)kvh * (np * wc + U);
       group = w.full;
       nrows = w.nq - group * rows.per_unit();
     }
-    unit1 = unit0 + (uint64_t)np * wc;
+    unit1 = unit0 + np * wc + U;
     pmin = w.p0 + group * rows.per_unit();
     pmax = pmin + nrows - 1;
     const uint64_t stop = min(unit1, end);
-    const uint32_t k0 = ((uint32_t)(g - unit0) + wc - 1) / wc, k1 = ((uint32_t)(stop - unit0) + wc - 1) / wc;
+    const uint32_t o0 = (uint32_t)(g - unit0), o1 = (uint32_t)(stop - unit0);
+    const uint32_t k0 = o0 <= U ? 0u : (o0 - U + wc - 1) / wc, k1 = o1 <= U ? 0u : (o1 - U + wc - 1) / wc;
     const uint32_t p1 = min(pmax, p.d.cap - 1);
     span = piece_span(w.range, k0, k1, min(pmin, p1), p1, p.window, p.sinks);
     g = stop;
@@ -217,9 +221,19 @@ E4B_DEV void mma16816_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
 // The pair of codes in bits 0..3 (4..7) of each half, as f16 n - 8: OR-ed under the
 // exponent of 1024 they read 1024 + n (1024 + 16 n), from which one instruction
 // takes 1032 (and divides by 16).
-E4B_DEV uint32_t low_codes(uint32_t x) { return hsub2((x & kLowCodes) | 0x64006400u, 0x64086408u); }
+E4B_DEV uint32_t and_or(uint32_t x, uint32_t mask, uint32_t bits) {    // one instruction: (x & mask) | bits
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(x), "r"(mask), "r"(bits));
+  return r;
+}
+E4B_DEV uint32_t low_codes(uint32_t x) { return hsub2(and_or(x, kLowCodes, 0x64006400u), 0x64086408u); }
 E4B_DEV uint32_t high_codes(uint32_t x) {
-  return hfma2((x & kHighCodes) | 0x64006400u, 0x2C002C00u, 0xD480D480u);   // / 16, - 72
+  return hfma2(and_or(x, kHighCodes, 0x64006400u), 0x2C002C00u, 0xD480D480u);   // / 16, - 72
+}
+E4B_DEV bool finite2(uint32_t x) { return (x & 0x7C00u) != 0x7C00u && (x & 0x7C000000u) != 0x7C000000u; }
+E4B_DEV float half_of(uint32_t x, int upper) {
+  const __half2 h = *reinterpret_cast<const __half2*>(&x);
+  return upper ? __high2float(h) : __low2float(h);
 }
 E4B_DEV uint4 lds128(const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); }
 template <int WORDS>
@@ -238,13 +252,18 @@ E4B_DEV void mbar_arrive_n(uint64_t* b, uint32_t n) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(b)), "r"(n) : "memory");
 }
 
+__device__ __noinline__ bool wait_slow(uint64_t* b, uint32_t parity, uint32_t* status) {
+  return mbar_wait(b, parity, status);
+}
+
 template <int BITS, int HD, int NT>
 __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, 1) k_attn_paged(const AttnP p) {
   using Sh = Shape<BITS, HD, NT>;
   constexpr int NB = Sh::NB, PB = Sh::PB, W = Sh::W, S = Sh::S, LN = Sh::LN, CT = Sh::CT, LC = NT * 4;
   static_assert(S % W == 0 && S % LN == 0 && LN <= 32 && S <= Sh::THREADS, "ring");
   constexpr int OT = HD / 16;        // m16 tiles of O
-  using Unit = Walk<W, NT>;
+  constexpr int U = Sh::U;
+  using Unit = Walk<W, NT, U>;
   extern __shared__ __align__(128) uint8_t smem[];
   uint8_t* ring = smem;
   float* merge = reinterpret_cast<float*>(smem + Sh::RING);            // [W][LC][HD]
@@ -270,7 +289,7 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, 1) k_attn_paged(
   // ---- the run of this CTA: the work of all units, cut evenly
   uint64_t mine = 0;
   const int per = (p.d.nseq + Sh::THREADS - 1) / Sh::THREADS;
-  for (int s = tid * per; s < min(p.d.nseq, (tid + 1) * per); s++) mine += seq_work<W, NT>(p, s).cost;
+  for (int s = tid * per; s < min(p.d.nseq, (tid + 1) * per); s++) mine += seq_work<W, NT, U>(p, s).cost;
   if (blockIdx.x == 0) live_rows(p.d);                   // records a row count past n_rows
   uint64_t upto = mine;                                  // inclusive sum over the threads
 #pragma unroll
@@ -287,21 +306,41 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, 1) k_attn_paged(
     T += warp_sum_[i];
   }
   upto += before;
-  const uint64_t want = udiv(T + W - 1, W);              // at least a piece per warp
-  const uint32_t C = want < gridDim.x ? (uint32_t)want : gridDim.x;
+  // runs of 2 U at least; an end that falls within U of a unit's start or end moves
+  // there, so short units stay whole and no fragment is shorter than U
+  const uint64_t want = udiv(T, 2 * U);
+  const uint32_t C = T == 0 ? 0u : (want < 1 ? 1u : (want < gridDim.x ? (uint32_t)want : gridDim.x));
   const uint32_t cta = blockIdx.x;
   if (cta >= C) return;
-  Unit u;
-  u.g = udiv(T * cta, C);
-  u.end = udiv(T * (cta + 1), C);
-  // the thread whose sequences hold the run's start tells the others
-  __shared__ uint64_t start_base;
-  __shared__ int start_seq;
-  if (upto - mine <= u.g && u.g < upto) start_base = upto - mine, start_seq = tid * per;
+  __shared__ uint64_t run_end[2], run_base[2];
+  __shared__ int run_seq[2];
+#pragma unroll
+  for (int i = 0; i < 2; i++) {      // the thread whose sequences hold the end
+    const uint64_t raw = udiv(T * (cta + i), C);
+    if (upto - mine <= raw && raw < upto) run_base[i] = upto - mine, run_seq[i] = tid * per;
+  }
   __syncthreads();
-  u.base = start_base;
-  u.s = start_seq;
-  u.w = seq_work<W, NT>(p, u.s);
+  Unit u;
+  if (warp < 2) {
+    const uint64_t raw = udiv(T * (cta + warp), C);
+    uint64_t at = raw;
+    if (raw > 0 && raw < T) {
+      u.base = run_base[warp];
+      u.s = run_seq[warp];
+      u.w = seq_work<W, NT, U>(p, u.s);
+      u.g = raw;
+      u.end = raw + 1;
+      u.next(p);
+      at = raw - u.unit0 < U ? u.unit0 : (u.unit1 - raw < U ? u.unit1 : raw);
+    }
+    if (lane == 0) run_end[warp] = at;
+  }
+  __syncthreads();
+  u.g = run_end[0];
+  u.end = run_end[1];
+  u.base = run_base[0];
+  u.s = run_seq[0];
+  u.w = seq_work<W, NT, U>(p, u.s);
 
   if (warp >= W) {
     // ---- producer: lane i brings the CTA's pieces i, i + LN, .., piece j into stage j % S
@@ -369,7 +408,6 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, 1) k_attn_paged(
   const auto consumers = []() { asm volatile("bar.sync 1, %0;" ::"n"(CT) : "memory"); };
   uint32_t j0 = 0;                   // the CTA's pieces before the unit's
   bool alive = true;                 // no wait has run out
-  bool first = true;                 // the CTA's first segment
   float O[NT][OT][4];
 
   while (u.next(p)) {
@@ -468,7 +506,8 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, 1) k_attn_paged(
     const uint32_t turn = j0 % WS;   // group (j % WS) takes the CTA's piece j
     for (uint32_t i = (uint32_t)ws >= turn ? ws - turn : ws + WS - turn; i < u.span.count; i += WS) {
       const uint32_t j = j0 + i, st = j % S, t0 = u.span.at(i) * kPieceSlots;
-      if (alive) alive = __all_sync(0xffffffffu, mbar_wait(&landed[st], (j / S) & 1u, p.d.status));
+      if (!__all_sync(0xffffffffu, mbar_try_wait(&landed[st], (j / S) & 1u)) && alive)
+        alive = __all_sync(0xffffffffu, wait_slow(&landed[st], (j / S) & 1u, p.d.status));
       const bool here = alive && usable[st] != 0;
       const uint8_t* kp = ring + (size_t)st * Sh::STAGE;
       const uint8_t* vp = kp + PB;
@@ -499,7 +538,7 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, 1) k_attn_paged(
           for (int q = 0; q < RUN; q++) {
             const int b = r * RUN + q;
             const uint32_t sa = wa[q] >> 8, sb = wb[q] >> 8;
-            const float d0 = h2f((uint16_t)(da[b / 2] >> (16 * (b & 1)))), d1 = h2f((uint16_t)(db[b / 2] >> (16 * (b & 1))));
+            const float d0 = half_of(da[b / 2], b & 1), d1 = half_of(db[b / 2], b & 1);
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
               if (NT > 1 && !live[nt]) continue;
@@ -620,10 +659,42 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, 1) k_attn_paged(
           const float2 hf = __half22float2(*reinterpret_cast<const __half2*>(&h));
           const uint32_t l = pack2(e[2 * k] - hf.x, e[2 * k + 1] - hf.y);
           if constexpr (BITS == 4) {
-            ph[nt][k] = transpose8x8(h);
-            pl[nt][k] = transpose8x8(l);
+            // columns 0-3: (0, hi), columns 4-7: (hi, lo); see the product with the scales
+            ph[nt][k] = transpose8x8(t < 2 ? 0u : h);
+            pl[nt][k] = transpose8x8(t < 2 ? h : l);
           } else {
             ph[nt][k] = transpose8x8(t < 2 ? h : l);      // columns 0-3 hi, 4-7 lo
+          }
+        }
+      }
+
+      // ---- slots that no row of the warp sees may hold anything: their scales (values)
+      // become zero.  strict: a row does not see a slot that another row sees and that
+      // holds an infinity or NaN, so its own mask goes on every operand.
+      bool strict[NT];
+      uint32_t seen[2] = {0u, 0u};
+      bool masked = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++) {
+        strict[nt] = false;
+        if (NT > 1 && !live[nt]) continue;
+        if (full[nt]) keep[nt][0] = keep[nt][1] = 0xffffffffu;
+        else masked = true;
+        seen[0] |= keep[nt][0], seen[1] |= keep[nt][1];
+      }
+      if constexpr (BITS == 4) {
+        if (masked) {
+          bool odd = false;
+#pragma unroll
+          for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+              dv[b][k] &= seen[k];
+              odd |= !finite2(dv[b][k]);
+            }
+          if (NT > 1 && __any_sync(0xffffffffu, odd)) {
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) strict[nt] = true;
           }
         }
       }
@@ -646,11 +717,9 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, 1) k_attn_paged(
             uint32_t bb[2];
 #pragma unroll
             for (int k = 0; k < 2; k++) {
-              uint32_t d = dv[b][k];
-              if (!full[nt]) d &= keep[nt][k];
-              const uint32_t hi = hmul2(ph[nt][k], d);
-              const uint32_t lo = hfma2(pl[nt][k], d, hfms2(ph[nt][k], d, hi));
-              bb[k] = g < 4 ? hi : lo;
+              // hi columns: f16(hi d); lo columns: lo d + (hi d - f16(hi d))
+              const uint32_t d = strict[nt] ? dv[b][k] & keep[nt][k] : dv[b][k];
+              bb[k] = hfma2(pl[nt][k], d, hfms2(ph[nt][k], d, hmul2(ph[nt][k], d)));
             }
             mma16816(O[nt][2 * b], al[0], al[1], al[2], al[3], bb[0], bb[1]);
             mma16816(O[nt][2 * b + 1], ah[0], ah[1], ah[2], ah[3], bb[0], bb[1]);
@@ -664,14 +733,21 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, 1) k_attn_paged(
           for (int k = 0; k < 4; k++) lds_words<4>(vw[k], vp + ((q * 4 + k) * 32 + lane) * 16);
 #pragma unroll
           for (int k = 0; k < 4; k++) {
-            const uint32_t a0 = __byte_perm(vw[0][k], vw[1][k], 0x5410), a1 = __byte_perm(vw[0][k], vw[1][k], 0x7632);
-            const uint32_t a2 = __byte_perm(vw[2][k], vw[3][k], 0x5410), a3 = __byte_perm(vw[2][k], vw[3][k], 0x7632);
+            uint32_t a[4] = {__byte_perm(vw[0][k], vw[1][k], 0x5410), __byte_perm(vw[0][k], vw[1][k], 0x7632),
+                             __byte_perm(vw[2][k], vw[3][k], 0x5410), __byte_perm(vw[2][k], vw[3][k], 0x7632)};
+            bool each = false;                           // every row with its own mask
+            if (masked) {
+#pragma unroll
+              for (int i2 = 0; i2 < 4; i2++) a[i2] &= seen[i2 >> 1];
+              if (NT > 1)
+                each = __any_sync(0xffffffffu, !finite2(a[0]) || !finite2(a[1]) || !finite2(a[2]) || !finite2(a[3]));
+            }
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
               if (NT > 1 && !live[nt]) continue;
-              if (full[nt]) mma16816(O[nt][4 * q + k], a0, a1, a2, a3, ph[nt][0], ph[nt][1]);
+              if (!each) mma16816(O[nt][4 * q + k], a[0], a[1], a[2], a[3], ph[nt][0], ph[nt][1]);
               else
-                mma16816(O[nt][4 * q + k], a0 & keep[nt][0], a1 & keep[nt][0], a2 & keep[nt][1], a3 & keep[nt][1],
+                mma16816(O[nt][4 * q + k], a[0] & keep[nt][0], a[1] & keep[nt][0], a[2] & keep[nt][1], a[3] & keep[nt][1],
                          ph[nt][0], ph[nt][1]);
             }
           }
@@ -708,7 +784,14 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, 1) k_attn_paged(
         }
     }
     consumers();
-    const uint32_t c0 = (uint32_t)(((u.unit0 + 1) * C - 1) / T), c1 = (uint32_t)((u.unit1 * C - 1) / T);
+    // the CTAs whose runs hold the unit, c0..c1
+    const auto run_of = [&](uint64_t x) { return (uint32_t)udiv(((x + 1) * C - 1), T); };
+    uint32_t c0 = run_of(u.unit0), c1 = run_of(u.unit1 - 1);
+    {
+      const uint64_t after = udiv(T * (c0 + 1), C), inside = udiv(T * c1, C);
+      if (c1 > c0 && inside - u.unit0 >= U && u.unit1 - inside < U) c1--;
+      if (after > u.unit0 && after < u.unit1 && after - u.unit0 < U) c0++;
+    }
     const bool whole = c0 == c1;
     const auto finish = [&](int c, int dim, const float4& o, float M, float L) {
       const int head = u.kvh * p.G + col_head(c);
@@ -728,7 +811,7 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, 1) k_attn_paged(
       }
       if (p.lse && dim == 0) p.lse[row * p.QH + head] = L != 0.f ? (M + log2f(L)) * 0.6931471805599453f : -INFINITY;
     };
-    float* part = p.parts + (2 * (size_t)cta + (first ? 0 : 1)) * kPartFloats;
+    float* part = p.parts + (2 * (size_t)cta + (cta == c0 ? 1 : 0)) * kPartFloats;  // a run ends with at most one cut unit, and begins with one
     for (int e = tid; e < cols * (HD / 4); e += CT) {
       const int c = e / (HD / 4), dim = e % (HD / 4) * 4;
       if (!col_live(c)) continue;
@@ -751,7 +834,6 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, 1) k_attn_paged(
       }
     }
     if (!whole) {
-      // a unit cut between CTAs c0..c1: only c0 may hold it behind other units
       const uint32_t n = c1 - c0 + 1;
       __threadfence();
       consumers();
@@ -761,9 +843,8 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, 1) k_attn_paged(
       }
       consumers();
       if (last_one) {
-        const bool behind = udiv(T * c0, C) != u.unit0;
         const auto part_of = [&](uint32_t i) {
-          return p.parts + (2 * (size_t)(c0 + i) + (i == 0 && behind ? 1 : 0)) * kPartFloats;
+          return p.parts + (2 * (size_t)(c0 + i) + (i == 0 ? 1 : 0)) * kPartFloats;
         };
         // a warp takes 128 dims of a column, a lane four of them
         constexpr int kSplit = HD > 128 ? HD / 128 : 1;
@@ -804,7 +885,6 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, 1) k_attn_paged(
         }
       }
     }
-    first = false;
     consumers();                     // the merge buffer and the states are free again
   }
 }
