@@ -26,9 +26,9 @@
 // The MMA aligns a subnormal by its exponent field, which costs it up to 7 of the
 // sum's 24 bits: no loss for 15-bit products of one magnitude (q's), but 6e-6 of
 // the result where p spreads over many, so 4-bit values are decoded to normal f16
-// n - 8.  A value block's scale multiplies p, again as hi + lo; p is kept as
-// p * 2^14 unless a scale of the piece is 2 or more, so that the lo parts stay
-// clear of f16's subnormals.
+// n - 8.  A value block's scale multiplies p, again as hi + lo; p is lifted by 2^8
+// unless a scale of the piece is 2 or more, so that the lo parts stay clear of
+// f16's subnormals.
 #include "paged.cuh"
 #include "stream.cuh"
 
@@ -38,7 +38,9 @@ using namespace e4b;
 constexpr int kMaxCtas = 160;
 constexpr uint32_t kLowCodes = 0x000F000Fu, kHighCodes = 0x00F000F0u;
 constexpr float kTwo24 = 16777216.f;
-constexpr float kLift = 14.f;        // p is held as p * 2^14 (see above)
+// p is held as p * 2^8 relative to a maximum that may lag behind the largest score by
+// 2^6, so a rescaling of O is rare and p * d stays below 2^15 for scales d below 2
+constexpr float kLift = 8.f, kSlack = 6.f;
 
 struct AttnP {
   PagedDev d;
@@ -69,11 +71,11 @@ struct Shape {
   static constexpr int W = NT == 1 ? (BITS == 16 && HD == 256 ? 10 : 11) : 8;
   // ring depth: a multiple of W, so a stage's uses within a unit belong to the same
   // warps (a warp then never waits for a phase before the stage's last one is done)
-  static constexpr int S = NT == 1 ? W * (BITS == 16 ? (HD == 256 ? 1 : (HD == 128 ? 2 : 4)) : (HD == 256 ? 2 : (HD == 128 ? 4 : 6)))
+  static constexpr int S = NT == 1 ? W * (BITS == 16 ? (HD == 256 ? 1 : (HD == 128 ? 2 : 4)) : (HD == 256 ? 3 : (HD == 128 ? 5 : 8)))
                                    : W * (BITS == 16 ? (HD == 256 ? 1 : (HD == 128 ? 2 : 4)) : (HD == 64 ? 8 : 4));
   // what a unit costs beside its pieces (q, the merge, the outputs), in pieces
   static constexpr int U = BITS == 16 ? (HD == 256 ? 6 : (HD == 128 ? 8 : 12)) : (HD == 256 ? 12 : 16);
-  static constexpr int LN = S <= 32 ? S : (NT == 1 ? 22 : 32);          // producer lanes; S is a multiple
+  static constexpr int LN = S <= 32 ? S : (NT == 1 ? 11 : 32);          // producer lanes; S is a multiple
   static constexpr int THREADS = 384, CT = 32 * W;
   static constexpr int TILES = W * NT;                                  // n-tiles of a unit at most
   static constexpr size_t RING = (size_t)S * STAGE;
@@ -236,6 +238,11 @@ E4B_DEV float half_of(uint32_t x, int upper) {
   return upper ? __high2float(h) : __low2float(h);
 }
 E4B_DEV uint4 lds128(const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); }
+E4B_DEV uint4 lds128_once(const uint8_t* p) {            // a load that is not kept for later uses of the address
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(smem_u32(p)));
+  return v;
+}
 template <int WORDS>
 E4B_DEV void lds_words(uint32_t (&w)[WORDS], const uint8_t* p) {
   if constexpr (WORDS == 4) {
@@ -274,7 +281,8 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, 1) k_attn_paged(
   __shared__ uint2 qzero[BITS == 4 ? Sh::TILES * 32 : 1];               // B of the -8 term: -8 sum q per block, hi and lo
   __shared__ float qfac[Sh::TILES * 4];
   __shared__ float ml[W * LC * 2], weight[W][kMaxCtas];
-  __shared__ int last_one;
+  __shared__ int last_one, more_units;
+  __shared__ Unit unit;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
 
   if (tid < S) {
@@ -388,7 +396,7 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, 1) k_attn_paged(
       if (__any_sync(kLanes, ready)) {
         idle = 0;
       } else {
-        __nanosleep(40);
+        __nanosleep(200);
         if (idle == 0) since = globaltimer_ns();
         if ((++idle & 255u) == 0 && __any_sync(kLanes, globaltimer_ns() - since > 2000000000ull)) {
           set_status(p.d.status, E4B_ST_TIMEOUT);        // the consumers gave up
@@ -410,14 +418,20 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, 1) k_attn_paged(
   bool alive = true;                 // no wait has run out
   float O[NT][OT][4];
 
-  while (u.next(p)) {
-    const uint32_t WC = u.wc, WS = W / WC;
+  // the unit in hand lives in shared memory: the loop over its pieces needs the registers
+  if (tid == 0) {
+    more_units = u.next(p);
+    unit = u;
+  }
+  consumers();
+  while (more_units) {
+    const uint32_t WC = unit.wc, WS = W / WC;
     const int wc = warp % WC, ws = warp / WC;
-    const uint32_t row0 = (p.d.rows ? p.d.rows[u.s] : (uint32_t)u.s) + (u.pmin - u.w.p0);
+    const uint32_t row0 = (p.d.rows ? p.d.rows[unit.s] : (uint32_t)unit.s) + (unit.pmin - unit.w.p0);
     // column c of the unit: tile c / 4 -> row of the unit, head
     const auto col_row = [&](int c) { return p.G > 4 ? c >> 3 : c >> 2; };
     const auto col_head = [&](int c) { return p.G > 4 ? c & 7 : c & 3; };
-    const auto col_live = [&](int c) { return col_head(c) < p.G && (uint32_t)col_row(c) < u.nrows; };
+    const auto col_live = [&](int c) { return col_head(c) < p.G && (uint32_t)col_row(c) < unit.nrows; };
     const int cols = WC * LC;
 
     // ---- q as B fragments: HD/8 lanes take a column, a lane the 8 dims of one (block, t)
@@ -431,7 +445,7 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, 1) k_attn_paged(
         for (int i = 0; i < 8; i++) x[i] = 0.f;
         if (c < cols && col_live(c)) {
           const float4* src = reinterpret_cast<const float4*>(
-              p.q + ((size_t)(row0 + col_row(c)) * p.QH + u.kvh * p.G + col_head(c)) * HD + 8 * l);
+              p.q + ((size_t)(row0 + col_row(c)) * p.QH + unit.kvh * p.G + col_head(c)) * HD + 8 * l);
           const float4 a = src[0], b = src[1];
           x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
         }
@@ -482,14 +496,14 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, 1) k_attn_paged(
       }
     }
     consumers();
-    float top[NT][2], lsum[NT][2], fac[NT][2], lift = kLift;  // largest score so far; sum of p; score factor
+    float top[NT][2], lsum[NT][2], fac[NT][2], lift = kLift, slack = kSlack;  // reference score; sum of p; score factor
     bool live[NT];
     uint32_t pos[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
       const int tile = wc * NT + nt;
-      pos[nt] = u.pmin + col_row(tile * 4);
-      live[nt] = (uint32_t)col_row(tile * 4) < u.nrows && col_head(tile * 4) < p.G;
+      pos[nt] = unit.pmin + col_row(tile * 4);
+      live[nt] = (uint32_t)col_row(tile * 4) < unit.nrows && col_head(tile * 4) < p.G;
 #pragma unroll
       for (int i = 0; i < 2; i++) {
         top[nt][i] = -INFINITY;
@@ -503,11 +517,15 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, 1) k_attn_paged(
     }
     const uint4* qf = qfrag + (size_t)wc * NT * NB * 32 + lane;
 
+    const PieceSpan span = unit.span;
     const uint32_t turn = j0 % WS;   // group (j % WS) takes the CTA's piece j
-    for (uint32_t i = (uint32_t)ws >= turn ? ws - turn : ws + WS - turn; i < u.span.count; i += WS) {
-      const uint32_t j = j0 + i, st = j % S, t0 = u.span.at(i) * kPieceSlots;
-      if (!__all_sync(0xffffffffu, mbar_try_wait(&landed[st], (j / S) & 1u)) && alive)
-        alive = __all_sync(0xffffffffu, wait_slow(&landed[st], (j / S) & 1u, p.d.status));
+    bool fresh = true;               // O is zero
+    const uint32_t i0 = (uint32_t)ws >= turn ? ws - turn : ws + WS - turn;
+    uint32_t st = (j0 + i0) % S, phase = (j0 + i0) / S & 1u;
+    for (uint32_t i = i0; i < span.count; i += WS) {
+      const uint32_t t0 = span.at(i) * kPieceSlots;
+      if (!__all_sync(0xffffffffu, mbar_try_wait(&landed[st], phase)) && alive)
+        alive = __all_sync(0xffffffffu, wait_slow(&landed[st], phase, p.d.status));
       const bool here = alive && usable[st] != 0;
       const uint8_t* kp = ring + (size_t)st * Sh::STAGE;
       const uint8_t* vp = kp + PB;
@@ -579,24 +597,22 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, 1) k_attn_paged(
       }
 
       // ---- value scales of slots (2t, 2t+1) and (2t+8, 2t+9); one of 2 or more ends the lift of p
-      uint32_t dv[BITS == 4 ? NB : 1][2];
       if constexpr (BITS == 4) {
         uint32_t any = 0;
 #pragma unroll
         for (int b = 0; b < NB; b += 2) {
-          const uint4 d4 = lds128(vp + (t * NB + b) * 8);
-          dv[b][0] = d4.x, dv[b][1] = d4.y, dv[b + 1][0] = d4.z, dv[b + 1][1] = d4.w;
+          const uint4 d4 = lds128_once(vp + (t * NB + b) * 8);
           any |= d4.x | d4.y | d4.z | d4.w;
         }
         if (__any_sync(0xffffffffu, (any & 0x40004000u) != 0) && lift != 0.f) {
-          lift = 0.f;
+          lift = slack = 0.f;
 #pragma unroll
           for (int nt = 0; nt < NT; nt++) {
-            lsum[nt][0] *= 1.f / 16384.f, lsum[nt][1] *= 1.f / 16384.f;
+            lsum[nt][0] *= 1.f / 256.f, lsum[nt][1] *= 1.f / 256.f;
 #pragma unroll
             for (int o = 0; o < OT; o++)
 #pragma unroll
-              for (int k = 0; k < 4; k++) O[nt][o][k] *= 1.f / 16384.f;
+              for (int k = 0; k < 4; k++) O[nt][o][k] *= 1.f / 256.f;
           }
         }
       }
@@ -627,7 +643,7 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, 1) k_attn_paged(
             if (here && slot_visible(t0 + 2 * t + (k & 1) + 8 * (k >> 1), pos[nt], p.window, p.sinks))
               keep[nt][k >> 1] |= 0xffffu << (16 * (k & 1));
         }
-        const bool grow = v[0] > top[nt][0] || v[2] > top[nt][0] || v[1] > top[nt][1] || v[3] > top[nt][1];
+        const bool grow = fmaxf(v[0], v[2]) > top[nt][0] + slack || fmaxf(v[1], v[3]) > top[nt][1] + slack;
         if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
           for (int k = 0; k < 2; k++) {
@@ -639,8 +655,10 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, 1) k_attn_paged(
             const float a = n == top[nt][k] ? 1.f : ex2(top[nt][k] - n);
             top[nt][k] = n;
             lsum[nt][k] *= a;
+            if (!fresh) {
 #pragma unroll
-            for (int o = 0; o < OT; o++) O[nt][o][k] *= a, O[nt][o][k + 2] *= a;
+              for (int o = 0; o < OT; o++) O[nt][o][k] *= a, O[nt][o][k + 2] *= a;
+            }
           }
         }
         float e[4];
@@ -682,7 +700,13 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, 1) k_attn_paged(
         else masked = true;
         seen[0] |= keep[nt][0], seen[1] |= keep[nt][1];
       }
+      uint32_t dv[BITS == 4 ? NB : 1][2];
       if constexpr (BITS == 4) {
+#pragma unroll
+        for (int b = 0; b < NB; b += 2) {
+          const uint4 d4 = lds128(vp + (t * NB + b) * 8);
+          dv[b][0] = d4.x, dv[b][1] = d4.y, dv[b + 1][0] = d4.z, dv[b + 1][1] = d4.w;
+        }
         if (masked) {
           bool odd = false;
 #pragma unroll
@@ -755,8 +779,11 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, 1) k_attn_paged(
       }
       __syncwarp();
       if (lane == 0 && alive) mbar_arrive_n(&freed[st], WS);
+      fresh = false;
+      st += WS;
+      if (st >= (uint32_t)S) st -= S, phase ^= 1u;
     }
-    j0 += u.span.count;
+    j0 += unit.span.count;
 
     // ---- the warps' states
     consumers();                     // the q fragments have been read
@@ -786,15 +813,15 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, 1) k_attn_paged(
     consumers();
     // the CTAs whose runs hold the unit, c0..c1
     const auto run_of = [&](uint64_t x) { return (uint32_t)udiv(((x + 1) * C - 1), T); };
-    uint32_t c0 = run_of(u.unit0), c1 = run_of(u.unit1 - 1);
+    uint32_t c0 = run_of(unit.unit0), c1 = run_of(unit.unit1 - 1);
     {
       const uint64_t after = udiv(T * (c0 + 1), C), inside = udiv(T * c1, C);
-      if (c1 > c0 && inside - u.unit0 >= U && u.unit1 - inside < U) c1--;
-      if (after > u.unit0 && after < u.unit1 && after - u.unit0 < U) c0++;
+      if (c1 > c0 && inside - unit.unit0 >= U && unit.unit1 - inside < U) c1--;
+      if (after > unit.unit0 && after < unit.unit1 && after - unit.unit0 < U) c0++;
     }
     const bool whole = c0 == c1;
     const auto finish = [&](int c, int dim, const float4& o, float M, float L) {
-      const int head = u.kvh * p.G + col_head(c);
+      const int head = unit.kvh * p.G + col_head(c);
       const size_t row = row0 + col_row(c);
       const float r = L != 0.f ? 1.f / L : 0.f;          // a NaN sum stays one
       const float4 x = make_float4(o.x * r, o.y * r, o.z * r, o.w * r);
@@ -886,6 +913,12 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, 1) k_attn_paged(
       }
     }
     consumers();                     // the merge buffer and the states are free again
+    if (tid == 0) {
+      Unit v = unit;
+      more_units = v.next(p);
+      unit = v;
+    }
+    consumers();
   }
 }
 
