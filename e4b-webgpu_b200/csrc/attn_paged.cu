@@ -35,7 +35,9 @@
 namespace {
 using namespace e4b;
 
-constexpr int kMaxCtas = 160;
+constexpr int kMaxCtas = 320;
+constexpr int kGroup = 12, kGroupMax = (kMaxCtas + kGroup - 1) / kGroup;   // CTAs whose parts are merged first; groups
+static_assert(kGroupMax >= kGroup, "weights");
 constexpr uint32_t kLowCodes = 0x000F000Fu, kHighCodes = 0x00F000F0u;
 constexpr float kTwo24 = 16777216.f;
 // p is held as p * 2^8 relative to a maximum that may lag behind the largest score by
@@ -48,15 +50,12 @@ struct AttnP {
   uint16_t* out_h;
   float* out_f;
   float* lse;
-  uint32_t* arrived;                 // [kMaxCtas], zero at rest
-  float* parts;                      // [2 * CTAs][columns][HD], then (max, sum) per column
+  uint32_t* arrived;                 // [3][kMaxCtas], zero at rest: by a unit's first CTA, a later group's first, for the groups
+  float* parts;                      // [2 * CTAs]: [columns][HD] of O, then (max, sum) per column
   int QH, G, xfo;
   uint32_t window, sinks;
   float scale;
 };
-
-constexpr int kMaxCols = 64;         // columns (row, head) of a unit at most
-constexpr size_t kPartFloats = (size_t)kMaxCols * (256 + 2);
 
 constexpr int kConsumerRegs = 224, kProducerRegs = 56;
 
@@ -65,18 +64,21 @@ struct Shape {
   static constexpr int NB = HD / 32;
   static constexpr int PB = BITS == 16 ? 32 * HD : 9 * HD;
   static constexpr int STAGE = 2 * PB;
-  // consumer warps: with one n-tile a warp needs 168 registers, so 12 warps fit an SM;
-  // with two it needs more, which the producer's warpgroup gives up (setmaxnreg):
+  // consumer warps: with one n-tile a warp needs 168 registers, so 12 warps fit an SM,
+  // two CTAs of 5 + 1, so that one's set-up and merges pass beside the other's pieces;
+  // with two a warp needs more, which the producer's warpgroup gives up (setmaxnreg):
   // 8 * 32 * 224 + 4 * 32 * 56 = 384 * 168, what the block was launched with
-  static constexpr int W = NT == 1 ? (BITS == 16 && HD == 256 ? 10 : 11) : 8;
+  static constexpr int W = NT == 1 ? 5 : 8, PER_SM = NT == 1 ? 2 : 1, MAX_CTAS = NT == 1 ? kMaxCtas : kMaxCtas / 2;
   // ring depth: a multiple of W, so a stage's uses within a unit belong to the same
   // warps (a warp then never waits for a phase before the stage's last one is done)
-  static constexpr int S = NT == 1 ? W * (BITS == 16 ? (HD == 256 ? 1 : (HD == 128 ? 2 : 4)) : (HD == 256 ? 3 : (HD == 128 ? 5 : 8)))
+  static constexpr int S = NT == 1 ? W * (BITS == 16 ? (HD == 256 ? 1 : (HD == 128 ? 2 : 4)) : (HD == 256 ? 3 : (HD == 128 ? 6 : 8)))
                                    : W * (BITS == 16 ? (HD == 256 ? 1 : (HD == 128 ? 2 : 4)) : (HD == 64 ? 8 : 4));
   // what a unit costs beside its pieces (q, the merge, the outputs), in pieces
   static constexpr int U = BITS == 16 ? (HD == 256 ? 6 : (HD == 128 ? 8 : 12)) : (HD == 256 ? 12 : 16);
-  static constexpr int LN = S <= 32 ? S : (NT == 1 ? 11 : 32);          // producer lanes; S is a multiple
-  static constexpr int THREADS = 384, CT = 32 * W;
+  static constexpr int LN = S <= 32 ? S : (NT == 1 ? 20 : 32);          // producer lanes; S is a multiple
+  static constexpr int THREADS = NT == 1 ? 32 * (W + 1) : 384, CT = 32 * W;
+  static constexpr int COLS = NT == 1 ? 4 : 64;                         // columns (row, head) of a unit at most
+  static constexpr size_t PART = (size_t)COLS * (HD + 2);               // floats of a partial
   static constexpr int TILES = W * NT;                                  // n-tiles of a unit at most
   static constexpr size_t RING = (size_t)S * STAGE;
   // q fragments [TILES][NB][32] while a unit's pieces pass, then the warps' O [W][NT*4][HD]
@@ -264,7 +266,7 @@ __device__ __noinline__ bool wait_slow(uint64_t* b, uint32_t parity, uint32_t* s
 }
 
 template <int BITS, int HD, int NT>
-__global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, 1) k_attn_paged(const AttnP p) {
+__global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, Shape<BITS, HD, NT>::PER_SM) k_attn_paged(const AttnP p) {
   using Sh = Shape<BITS, HD, NT>;
   constexpr int NB = Sh::NB, PB = Sh::PB, W = Sh::W, S = Sh::S, LN = Sh::LN, CT = Sh::CT, LC = NT * 4;
   static_assert(S % W == 0 && S % LN == 0 && LN <= 32 && S <= Sh::THREADS, "ring");
@@ -280,7 +282,7 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, 1) k_attn_paged(
   __shared__ uint64_t warp_sum_[Sh::THREADS / 32];
   __shared__ uint2 qzero[BITS == 4 ? Sh::TILES * 32 : 1];               // B of the -8 term: -8 sum q per block, hi and lo
   __shared__ float qfac[Sh::TILES * 4];
-  __shared__ float ml[W * LC * 2], weight[W][kMaxCtas];
+  __shared__ float ml[W * LC * 2], weight[W][2 * kGroupMax];
   __shared__ int last_one, more_units;
   __shared__ Unit unit;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -838,7 +840,7 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, 1) k_attn_paged(
       }
       if (p.lse && dim == 0) p.lse[row * p.QH + head] = L != 0.f ? (M + log2f(L)) * 0.6931471805599453f : -INFINITY;
     };
-    float* part = p.parts + (2 * (size_t)cta + (cta == c0 ? 1 : 0)) * kPartFloats;  // a run ends with at most one cut unit, and begins with one
+    float* part = p.parts + (2 * (size_t)cta + (cta == c0 ? 1 : 0)) * Sh::PART;  // a run ends with at most one cut unit, and begins with one
     for (int e = tid; e < cols * (HD / 4); e += CT) {
       const int c = e / (HD / 4), dim = e % (HD / 4) * 4;
       if (!col_live(c)) continue;
@@ -857,37 +859,41 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, 1) k_attn_paged(
         finish(c, dim, o, M, L);
       } else {
         *reinterpret_cast<float4*>(part + c * HD + dim) = o;
-        if (dim == 0) part[kMaxCols * 256 + 2 * c] = M, part[kMaxCols * 256 + 2 * c + 1] = L;
+        if (dim == 0) part[Sh::COLS * HD + 2 * c] = M, part[Sh::COLS * HD + 2 * c + 1] = L;
       }
     }
     if (!whole) {
-      const uint32_t n = c1 - c0 + 1;
-      __threadfence();
-      consumers();
-      if (tid == 0) {
-        last_one = atomicInc(&p.arrived[c0], n - 1) == n - 1;        // wraps to zero with the last arrival
+      // The last CTA to arrive merges the parts; of many parts, the last of each group of
+      // kGroup merges the group's into its first CTA's, and the last of those the rest.
+      const auto part_of = [&](uint32_t c) { return p.parts + (2 * (size_t)c + (c == c0 ? 1 : 0)) * Sh::PART; };
+      const auto arrive = [&](uint32_t* counter, uint32_t n) {
         __threadfence();
-      }
-      consumers();
-      if (last_one) {
-        const auto part_of = [&](uint32_t i) {
-          return p.parts + (2 * (size_t)(c0 + i) + (i == 0 ? 1 : 0)) * kPartFloats;
-        };
-        // a warp takes 128 dims of a column, a lane four of them
-        constexpr int kSplit = HD > 128 ? HD / 128 : 1;
+        consumers();
+        if (tid == 0) {
+          last_one = atomicInc(counter, n - 1) == n - 1;               // wraps to zero with the last arrival
+          __threadfence();
+        }
+        consumers();
+        return last_one != 0;
+      };
+      // parts of CTAs a, a + step, .. (n of them): into the outputs, or into a's part
+      const auto combine = [&](uint32_t a, uint32_t step, uint32_t n, bool final) {
+        constexpr int kSplit = HD > 128 ? HD / 128 : 1;                // a warp takes 128 dims of a column, a lane four
         float* wt = weight[warp];
         for (int task = warp; task < cols * kSplit; task += W) {
           const int c = task / kSplit, dim = (task % kSplit) * 128 + lane * 4;
           if (!col_live(c)) continue;
           float M = -INFINITY, L = 0.f;
           for (uint32_t i = lane; i < n; i += 32) {
-            wt[i] = __ldcg(part_of(i) + kMaxCols * 256 + 2 * c);
-            M = fmaxf(M, wt[i]);
+            const float2 x = __ldcg(reinterpret_cast<const float2*>(part_of(a + i * step) + Sh::COLS * HD + 2 * c));
+            wt[i] = x.x;
+            wt[kGroupMax + i] = x.y;
+            M = fmaxf(M, x.x);
           }
           M = warp_max(M);
           for (uint32_t i = lane; i < n; i += 32) {
             wt[i] = wt[i] == M ? 1.f : ex2(wt[i] - M);
-            L = fmaf(wt[i], __ldcg(part_of(i) + kMaxCols * 256 + 2 * c + 1), L);
+            L = fmaf(wt[i], wt[kGroupMax + i], L);
           }
           L = warp_sum(L);
           __syncwarp();
@@ -898,17 +904,35 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, 1) k_attn_paged(
               float4 x[8];
 #pragma unroll
               for (int i = 0; i < 8; i++)
-                x[i] = __ldcg(reinterpret_cast<const float4*>(part_of(min(i0 + i, n - 1)) + c * HD + dim));
+                x[i] = __ldcg(reinterpret_cast<const float4*>(part_of(a + min(i0 + i, n - 1) * step) + c * HD + dim));
 #pragma unroll
               for (int i = 0; i < 8; i++) {
-                const float a = i0 + i < n ? wt[i0 + i] : 0.f;
-                o.x = fmaf(a, x[i].x, o.x), o.y = fmaf(a, x[i].y, o.y);
-                o.z = fmaf(a, x[i].z, o.z), o.w = fmaf(a, x[i].w, o.w);
+                const float f = i0 + i < n ? wt[i0 + i] : 0.f;
+                o.x = fmaf(f, x[i].x, o.x), o.y = fmaf(f, x[i].y, o.y);
+                o.z = fmaf(f, x[i].z, o.z), o.w = fmaf(f, x[i].w, o.w);
               }
             }
+            if (final) finish(c, dim, o, M, L);
+            else *reinterpret_cast<float4*>(part_of(a) + c * HD + dim) = o;
           }
+          if (!final && task % kSplit == 0 && lane == 0) ml[2 * c] = M, ml[2 * c + 1] = L;
           __syncwarp();
-          if (dim < HD) finish(c, dim, o, M, L);
+        }
+        if (!final) {                // every warp has read a's (max, sum)
+          consumers();
+          for (int c = tid; c < cols; c += CT)
+            if (col_live(c)) part_of(a)[Sh::COLS * HD + 2 * c] = ml[2 * c], part_of(a)[Sh::COLS * HD + 2 * c + 1] = ml[2 * c + 1];
+        }
+      };
+      const uint32_t n = c1 - c0 + 1, groups = (n + kGroup - 1) / kGroup;
+      if (groups == 1) {
+        if (arrive(p.arrived + c0, n)) combine(c0, 1, n, true);
+      } else {
+        const uint32_t gi = (cta - c0) / kGroup, from = c0 + gi * kGroup;
+        const uint32_t size = min((uint32_t)kGroup, n - gi * kGroup);
+        if (arrive(p.arrived + (gi ? kMaxCtas : 0) + from, size)) {
+          combine(from, 1, size, false);
+          if (arrive(p.arrived + 2 * kMaxCtas + c0, groups)) combine(c0, kGroup, groups, true);
         }
       }
     }
@@ -925,9 +949,9 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, 1) k_attn_paged(
 template <int BITS, int HD, int NT>
 int launch(e4b_ctx* c, const AttnP& p) {
   using Sh = Shape<BITS, HD, NT>;
-  static_assert(Sh::SMEM + 14 * 1024 < 227 * 1024, "shared memory");
+  static_assert(Sh::PER_SM * (Sh::SMEM + 13 * 1024) < 228 * 1024, "shared memory");
   E4B_CUDA(c, cudaFuncSetAttribute(k_attn_paged<BITS, HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Sh::SMEM));
-  const int ctas = c->sm_count < kMaxCtas ? c->sm_count : kMaxCtas;
+  const int ctas = Sh::PER_SM * c->sm_count < Sh::MAX_CTAS ? Sh::PER_SM * c->sm_count : Sh::MAX_CTAS;
   return e4b_launch(c, "attn_paged", k_attn_paged<BITS, HD, NT>, dim3(ctas), dim3(Sh::THREADS), Sh::SMEM, p);
 }
 template <int BITS, int NT>
@@ -939,7 +963,8 @@ int launch_hd(e4b_ctx* c, const AttnP& p, int HD) {
 extern "C" {
 
 E4B_API size_t e4b_paged_scratch_bytes(void) {
-  return kMaxCtas * sizeof(uint32_t) + 2 * kMaxCtas * kPartFloats * sizeof(float);
+  // two partials for each of kMaxCtas / 2 CTAs of the shape with the largest ones
+  return kMaxCtas * (3 * sizeof(uint32_t) + Shape<4, 256, 2>::PART * sizeof(float));
 }
 
 E4B_API int e4b_attn_paged(e4b_ctx* c, const e4b_paged_kv* kv, const float* q, uint16_t* out_h, float* out_f,
@@ -955,7 +980,7 @@ E4B_API int e4b_attn_paged(e4b_ctx* c, const e4b_paged_kv* kv, const float* q, u
   p.out_f = out_f;
   p.lse = lse;
   p.arrived = static_cast<uint32_t*>(scratch);
-  p.parts = reinterpret_cast<float*>(p.arrived + kMaxCtas);
+  p.parts = reinterpret_cast<float*>(p.arrived + 3 * kMaxCtas);
   p.QH = QH;
   p.G = QH / kv->kv_heads;
   p.xfo = xfo ? 1 : 0;
