@@ -36,8 +36,7 @@ namespace {
 using namespace e4b;
 
 constexpr int kMaxCtas = 320;
-constexpr int kGroup = 12, kGroupMax = (kMaxCtas + kGroup - 1) / kGroup;   // CTAs whose parts are merged first; groups
-static_assert(kGroupMax >= kGroup, "weights");
+constexpr int kGroup = 12;           // CTAs whose parts are merged first
 constexpr uint32_t kLowCodes = 0x000F000Fu, kHighCodes = 0x00F000F0u;
 constexpr float kTwo24 = 16777216.f;
 // p is held as p * 2^8 relative to a maximum that may lag behind the largest score by
@@ -59,23 +58,25 @@ struct AttnP {
 
 constexpr int kConsumerRegs = 224, kProducerRegs = 56;
 
-template <int BITS, int HD, int NT>
+template <int BITS, int HD, int NT, bool WIDE>
 struct Shape {
   static constexpr int NB = HD / 32;
   static constexpr int PB = BITS == 16 ? 32 * HD : 9 * HD;
   static constexpr int STAGE = 2 * PB;
-  // consumer warps: with one n-tile a warp needs 168 registers, so 12 warps fit an SM,
-  // two CTAs of 5 + 1, so that one's set-up and merges pass beside the other's pieces;
-  // with two a warp needs more, which the producer's warpgroup gives up (setmaxnreg):
-  // 8 * 32 * 224 + 4 * 32 * 56 = 384 * 168, what the block was launched with
-  static constexpr int W = NT == 1 ? 5 : 8, PER_SM = NT == 1 ? 2 : 1, MAX_CTAS = NT == 1 ? kMaxCtas : kMaxCtas / 2;
+  // consumer warps: with one n-tile a warp needs 168 registers, so 12 warps fit an SM:
+  // one CTA of 11 + 1 (WIDE), or two of 5 + 1, where one's set-up and merges pass
+  // beside the other's pieces; with two tiles a warp needs more, which the producer's
+  // warpgroup gives up (setmaxnreg): 8 * 32 * 224 + 4 * 32 * 56 = 384 * 168, what the
+  // block was launched with
+  static constexpr int PER_SM = NT == 1 && !WIDE ? 2 : 1, MAX_CTAS = PER_SM * kMaxCtas / 2;
+  static constexpr int W = NT == 2 ? 8 : (!WIDE ? 5 : (BITS == 16 && HD == 256 ? 10 : 11));
   // ring depth: a multiple of W, so a stage's uses within a unit belong to the same
   // warps (a warp then never waits for a phase before the stage's last one is done)
-  static constexpr int S = NT == 1 ? W * (BITS == 16 ? (HD == 256 ? 1 : (HD == 128 ? 2 : 4)) : (HD == 256 ? 3 : (HD == 128 ? 6 : 8)))
-                                   : W * (BITS == 16 ? (HD == 256 ? 1 : (HD == 128 ? 2 : 4)) : (HD == 64 ? 8 : 4));
+  static constexpr int S = W * (BITS == 16 ? (HD == 256 ? 1 : (HD == 128 ? 2 : 4)) :
+                                NT == 2 ? (HD == 64 ? 8 : 4) : (HD == 256 ? 3 : (HD == 128 ? 5 : 8)));
   // what a unit costs beside its pieces (q, the merge, the outputs), in pieces
   static constexpr int U = BITS == 16 ? (HD == 256 ? 6 : (HD == 128 ? 8 : 12)) : (HD == 256 ? 12 : 16);
-  static constexpr int LN = S <= 32 ? S : (NT == 1 ? 20 : 32);          // producer lanes; S is a multiple
+  static constexpr int LN = S <= 32 ? S : (W == 11 ? 11 : (W == 5 ? (S == 40 ? 20 : 25) : 32));   // producer lanes; S is a multiple
   static constexpr int THREADS = NT == 1 ? 32 * (W + 1) : 384, CT = 32 * W;
   static constexpr int COLS = NT == 1 ? 4 : 64;                         // columns (row, head) of a unit at most
   static constexpr size_t PART = (size_t)COLS * (HD + 2);               // floats of a partial
@@ -162,7 +163,7 @@ struct Walk {
     const uint32_t KVH = p.d.KVH, np = w.range.count;
     const uint64_t off = g - base, full_cost = ((uint64_t)np * W + U) * w.full * KVH;
     uint32_t group, unit;
-    if (off < full_cost) {
+    if (NT > 1 && off < full_cost) {
       wc = W;
       unit = (uint32_t)udiv(off, np * W + U);
       unit0 = base + (uint64_t)unit * (np * W + U);
@@ -181,7 +182,8 @@ struct Walk {
     pmax = pmin + nrows - 1;
     const uint64_t stop = min(unit1, end);
     const uint32_t o0 = (uint32_t)(g - unit0), o1 = (uint32_t)(stop - unit0);
-    const uint32_t k0 = o0 <= U ? 0u : (o0 - U + wc - 1) / wc, k1 = o1 <= U ? 0u : (o1 - U + wc - 1) / wc;
+    const int sh = 31 - __clz((int)wc);                  // wc is a power of two
+    const uint32_t k0 = o0 <= U ? 0u : (o0 - U + wc - 1) >> sh, k1 = o1 <= U ? 0u : (o1 - U + wc - 1) >> sh;
     const uint32_t p1 = min(pmax, p.d.cap - 1);
     span = piece_span(w.range, k0, k1, min(pmin, p1), p1, p.window, p.sinks);
     g = stop;
@@ -265,9 +267,9 @@ __device__ __noinline__ bool wait_slow(uint64_t* b, uint32_t parity, uint32_t* s
   return mbar_wait(b, parity, status);
 }
 
-template <int BITS, int HD, int NT>
-__global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, Shape<BITS, HD, NT>::PER_SM) k_attn_paged(const AttnP p) {
-  using Sh = Shape<BITS, HD, NT>;
+template <int BITS, int HD, int NT, bool WIDE>
+__global__ void __launch_bounds__(Shape<BITS, HD, NT, WIDE>::THREADS, Shape<BITS, HD, NT, WIDE>::PER_SM) k_attn_paged(const AttnP p) {
+  using Sh = Shape<BITS, HD, NT, WIDE>;
   constexpr int NB = Sh::NB, PB = Sh::PB, W = Sh::W, S = Sh::S, LN = Sh::LN, CT = Sh::CT, LC = NT * 4;
   static_assert(S % W == 0 && S % LN == 0 && LN <= 32 && S <= Sh::THREADS, "ring");
   constexpr int OT = HD / 16;        // m16 tiles of O
@@ -282,9 +284,10 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, Shape<BITS, HD, 
   __shared__ uint64_t warp_sum_[Sh::THREADS / 32];
   __shared__ uint2 qzero[BITS == 4 ? Sh::TILES * 32 : 1];               // B of the -8 term: -8 sum q per block, hi and lo
   __shared__ float qfac[Sh::TILES * 4];
-  __shared__ float ml[W * LC * 2], weight[W][2 * kGroupMax];
+  __shared__ float ml[W * LC * 2];
   __shared__ int last_one, more_units;
-  __shared__ Unit unit;
+  __shared__ Unit start, unit;
+  __shared__ uint32_t unit_c0, unit_c1;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
 
   if (tid < S) {
@@ -298,8 +301,13 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, Shape<BITS, HD, 
 
   // ---- the run of this CTA: the work of all units, cut evenly
   uint64_t mine = 0;
+  SeqWork own;                       // of the thread's first sequence
   const int per = (p.d.nseq + Sh::THREADS - 1) / Sh::THREADS;
-  for (int s = tid * per; s < min(p.d.nseq, (tid + 1) * per); s++) mine += seq_work<W, NT, U>(p, s).cost;
+  for (int s = tid * per; s < min(p.d.nseq, (tid + 1) * per); s++) {
+    const SeqWork w = seq_work<W, NT, U>(p, s);
+    if (s == tid * per) own = w;
+    mine += w.cost;
+  }
   if (blockIdx.x == 0) live_rows(p.d);                   // records a row count past n_rows
   uint64_t upto = mine;                                  // inclusive sum over the threads
 #pragma unroll
@@ -322,35 +330,36 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, Shape<BITS, HD, 
   const uint32_t C = T == 0 ? 0u : (want < 1 ? 1u : (want < gridDim.x ? (uint32_t)want : gridDim.x));
   const uint32_t cta = blockIdx.x;
   if (cta >= C) return;
-  __shared__ uint64_t run_end[2], run_base[2];
-  __shared__ int run_seq[2];
+  __shared__ uint64_t run_end[2];
+  {
+    Unit v;                          // at an end of the run, formed by the thread whose sequences hold it
+    v.unit0 = v.unit1 = 0;
 #pragma unroll
-  for (int i = 0; i < 2; i++) {      // the thread whose sequences hold the end
-    const uint64_t raw = udiv(T * (cta + i), C);
-    if (upto - mine <= raw && raw < upto) run_base[i] = upto - mine, run_seq[i] = tid * per;
-  }
-  __syncthreads();
-  Unit u;
-  if (warp < 2) {
-    const uint64_t raw = udiv(T * (cta + warp), C);
-    uint64_t at = raw;
-    if (raw > 0 && raw < T) {
-      u.base = run_base[warp];
-      u.s = run_seq[warp];
-      u.w = seq_work<W, NT, U>(p, u.s);
-      u.g = raw;
-      u.end = raw + 1;
-      u.next(p);
-      at = raw - u.unit0 < U ? u.unit0 : (u.unit1 - raw < U ? u.unit1 : raw);
+    for (int i = 0; i < 2; i++) {
+      const uint64_t raw = udiv(T * (cta + i), C);
+      if (upto - mine <= raw && raw < upto) {
+        if (raw < v.unit0 || raw >= v.unit1) {
+          v.base = upto - mine;
+          v.s = tid * per;
+          v.w = own;
+          v.g = raw;
+          v.end = raw + 1;
+          v.next(p);
+        }
+        const uint64_t at = raw - v.unit0 < U ? v.unit0 : (v.unit1 - raw < U ? v.unit1 : raw);
+        run_end[i] = at;
+        if (i == 0) {
+          v.g = at;
+          start = v;
+        }
+      } else if (i == 1 && raw == T && tid == 0) {
+        run_end[1] = T;
+      }
     }
-    if (lane == 0) run_end[warp] = at;
   }
   __syncthreads();
-  u.g = run_end[0];
+  Unit u = start;
   u.end = run_end[1];
-  u.base = run_base[0];
-  u.s = run_seq[0];
-  u.w = seq_work<W, NT, U>(p, u.s);
 
   if (warp >= W) {
     // ---- producer: lane i brings the CTA's pieces i, i + LN, .., piece j into stage j % S
@@ -421,10 +430,20 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, Shape<BITS, HD, 
   float O[NT][OT][4];
 
   // the unit in hand lives in shared memory: the loop over its pieces needs the registers
-  if (tid == 0) {
-    more_units = u.next(p);
-    unit = u;
-  }
+  const auto next_unit = [&](Unit& v) {                  // thread 0; with the CTAs whose runs hold the unit, c0..c1
+    more_units = v.next(p);
+    unit = v;
+    const auto run_of = [&](uint64_t x) { return (uint32_t)udiv((x + 1) * C - 1, T); };
+    uint32_t c0 = run_of(v.unit0), c1 = run_of(v.unit1 - 1);
+    if (c1 > c0) {
+      const uint64_t after = udiv(T * (c0 + 1), C), inside = udiv(T * c1, C);
+      if (inside - v.unit0 >= U && v.unit1 - inside < U) c1--;
+      if (after > v.unit0 && after < v.unit1 && after - v.unit0 < U) c0++;
+    }
+    unit_c0 = c0;
+    unit_c1 = c1;
+  };
+  if (tid == 0) next_unit(u);
   consumers();
   while (more_units) {
     const uint32_t WC = unit.wc, WS = W / WC;
@@ -802,25 +821,21 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, Shape<BITS, HD, 
           ml[(warp * LC + nt * 4 + 2 * t + k) * 2 + 1] = l;
         }
       }
+      // hi + lo: lanes t < 2 (the hi columns) take the even tiles, their partners the odd ones
 #pragma unroll
-      for (int o = 0; o < OT; o++)
+      for (int o = 0; o < OT; o += 2)
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-          const float x = O[nt][o][k] + __shfl_xor_sync(0xffffffffu, O[nt][o][k], 2);
-          const int dim = BITS == 4 ? (o / 2) * 32 + 4 * g + (o & 1) + 2 * (k >> 1)
-                                    : (o / 4) * 64 + 8 * g + 2 * (o & 3) + (k >> 1);
-          if (t < 2) merge[(size_t)(warp * LC + nt * 4 + 2 * t + (k & 1)) * HD + dim] = x;
+          const float give = t < 2 ? O[nt][o + 1][k] : O[nt][o][k], keep_ = t < 2 ? O[nt][o][k] : O[nt][o + 1][k];
+          const float x = keep_ + __shfl_xor_sync(0xffffffffu, give, 2);
+          const int tile = o + (t >> 1);
+          const int dim = BITS == 4 ? (o / 2) * 32 + 4 * g + (t >> 1) + 2 * (k >> 1)
+                                    : (o / 4) * 64 + 8 * g + 2 * (tile & 3) + (k >> 1);
+          merge[(size_t)(warp * LC + nt * 4 + 2 * (t & 1) + (k & 1)) * HD + dim] = x;
         }
     }
     consumers();
-    // the CTAs whose runs hold the unit, c0..c1
-    const auto run_of = [&](uint64_t x) { return (uint32_t)udiv(((x + 1) * C - 1), T); };
-    uint32_t c0 = run_of(unit.unit0), c1 = run_of(unit.unit1 - 1);
-    {
-      const uint64_t after = udiv(T * (c0 + 1), C), inside = udiv(T * c1, C);
-      if (c1 > c0 && inside - unit.unit0 >= U && unit.unit1 - inside < U) c1--;
-      if (after > unit.unit0 && after < unit.unit1 && after - unit.unit0 < U) c0++;
-    }
+    const uint32_t c0 = unit_c0, c1 = unit_c1;
     const bool whole = c0 == c1;
     const auto finish = [&](int c, int dim, const float4& o, float M, float L) {
       const int head = unit.kvh * p.G + col_head(c);
@@ -847,8 +862,12 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, Shape<BITS, HD, 
       const int w0 = (c >> 2) / NT, lc = ((c >> 2) % NT) * 4 + (c & 3);
       float M = -INFINITY, L = 0.f;
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (uint32_t i = 0; i < WS; i++) M = fmaxf(M, ml[((i * WC + w0) * LC + lc) * 2]);
-      for (uint32_t i = 0; i < WS; i++) {
+#pragma unroll
+      for (uint32_t i = 0; i < W; i++)
+        if (i < WS) M = fmaxf(M, ml[((i * WC + w0) * LC + lc) * 2]);
+#pragma unroll
+      for (uint32_t i = 0; i < W; i++) {
+        if (i >= WS) continue;
         const int at = (i * WC + w0) * LC + lc;
         const float mi = ml[at * 2], a = mi == M ? 1.f : ex2(mi - M);
         const float4 x = *reinterpret_cast<const float4*>(merge + (size_t)at * HD + dim);
@@ -878,50 +897,38 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, Shape<BITS, HD, 
       };
       // parts of CTAs a, a + step, .. (n of them): into the outputs, or into a's part
       const auto combine = [&](uint32_t a, uint32_t step, uint32_t n, bool final) {
-        constexpr int kSplit = HD > 128 ? HD / 128 : 1;                // a warp takes 128 dims of a column, a lane four
-        float* wt = weight[warp];
-        for (int task = warp; task < cols * kSplit; task += W) {
-          const int c = task / kSplit, dim = (task % kSplit) * 128 + lane * 4;
+        float2* part_ml = reinterpret_cast<float2*>(merge);            // [n][cols]
+        for (uint32_t e = tid; e < n * cols; e += CT)
+          part_ml[e] = __ldcg(reinterpret_cast<const float2*>(part_of(a + e / cols * step) + Sh::COLS * HD + 2 * (e % cols)));
+        consumers();
+        for (int e = tid; e < cols * (HD / 4); e += CT) {
+          const int c = e / (HD / 4), dim = e % (HD / 4) * 4;
           if (!col_live(c)) continue;
           float M = -INFINITY, L = 0.f;
-          for (uint32_t i = lane; i < n; i += 32) {
-            const float2 x = __ldcg(reinterpret_cast<const float2*>(part_of(a + i * step) + Sh::COLS * HD + 2 * c));
-            wt[i] = x.x;
-            wt[kGroupMax + i] = x.y;
-            M = fmaxf(M, x.x);
-          }
-          M = warp_max(M);
-          for (uint32_t i = lane; i < n; i += 32) {
-            wt[i] = wt[i] == M ? 1.f : ex2(wt[i] - M);
-            L = fmaf(wt[i], wt[kGroupMax + i], L);
-          }
-          L = warp_sum(L);
-          __syncwarp();
+          for (uint32_t i = 0; i < n; i++) M = fmaxf(M, part_ml[i * cols + c].x);
           float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (dim < HD) {
 #pragma unroll 1
-            for (uint32_t i0 = 0; i0 < n; i0 += 8) {      // eight parts' loads in flight
-              float4 x[8];
+          for (uint32_t i0 = 0; i0 < n; i0 += 8) {        // eight parts' loads in flight
+            float4 x[8];
 #pragma unroll
-              for (int i = 0; i < 8; i++)
-                x[i] = __ldcg(reinterpret_cast<const float4*>(part_of(a + min(i0 + i, n - 1) * step) + c * HD + dim));
+            for (int i = 0; i < 8; i++)
+              x[i] = __ldcg(reinterpret_cast<const float4*>(part_of(a + min(i0 + i, n - 1) * step) + c * HD + dim));
 #pragma unroll
-              for (int i = 0; i < 8; i++) {
-                const float f = i0 + i < n ? wt[i0 + i] : 0.f;
-                o.x = fmaf(f, x[i].x, o.x), o.y = fmaf(f, x[i].y, o.y);
-                o.z = fmaf(f, x[i].z, o.z), o.w = fmaf(f, x[i].w, o.w);
-              }
+            for (int i = 0; i < 8; i++) {
+              if (i0 + i >= n) continue;
+              const float2 y = part_ml[(i0 + i) * cols + c];
+              const float f = y.x == M ? 1.f : ex2(y.x - M);
+              L = fmaf(f, y.y, L);
+              o.x = fmaf(f, x[i].x, o.x), o.y = fmaf(f, x[i].y, o.y);
+              o.z = fmaf(f, x[i].z, o.z), o.w = fmaf(f, x[i].w, o.w);
             }
-            if (final) finish(c, dim, o, M, L);
-            else *reinterpret_cast<float4*>(part_of(a) + c * HD + dim) = o;
           }
-          if (!final && task % kSplit == 0 && lane == 0) ml[2 * c] = M, ml[2 * c + 1] = L;
-          __syncwarp();
-        }
-        if (!final) {                // every warp has read a's (max, sum)
-          consumers();
-          for (int c = tid; c < cols; c += CT)
-            if (col_live(c)) part_of(a)[Sh::COLS * HD + 2 * c] = ml[2 * c], part_of(a)[Sh::COLS * HD + 2 * c + 1] = ml[2 * c + 1];
+          if (final) {
+            finish(c, dim, o, M, L);
+          } else {
+            *reinterpret_cast<float4*>(part_of(a) + c * HD + dim) = o;
+            if (dim == 0) *reinterpret_cast<float2*>(part_of(a) + Sh::COLS * HD + 2 * c) = make_float2(M, L);
+          }
         }
       };
       const uint32_t n = c1 - c0 + 1, groups = (n + kGroup - 1) / kGroup;
@@ -939,24 +946,34 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT>::THREADS, Shape<BITS, HD, 
     consumers();                     // the merge buffer and the states are free again
     if (tid == 0) {
       Unit v = unit;
-      more_units = v.next(p);
-      unit = v;
+      next_unit(v);
     }
     consumers();
   }
 }
 
-template <int BITS, int HD, int NT>
+template <int BITS, int HD, int NT, bool WIDE>
 int launch(e4b_ctx* c, const AttnP& p) {
-  using Sh = Shape<BITS, HD, NT>;
-  static_assert(Sh::PER_SM * (Sh::SMEM + 13 * 1024) < 228 * 1024, "shared memory");
-  E4B_CUDA(c, cudaFuncSetAttribute(k_attn_paged<BITS, HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Sh::SMEM));
+  using Sh = Shape<BITS, HD, NT, WIDE>;
+  static_assert(Sh::PER_SM * (Sh::SMEM + 8 * 1024) < 228 * 1024, "shared memory");
+  E4B_CUDA(c, cudaFuncSetAttribute(k_attn_paged<BITS, HD, NT, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Sh::SMEM));
   const int ctas = Sh::PER_SM * c->sm_count < Sh::MAX_CTAS ? Sh::PER_SM * c->sm_count : Sh::MAX_CTAS;
-  return e4b_launch(c, "attn_paged", k_attn_paged<BITS, HD, NT>, dim3(ctas), dim3(Sh::THREADS), Sh::SMEM, p);
+  return e4b_launch(c, "attn_paged", k_attn_paged<BITS, HD, NT, WIDE>, dim3(ctas), dim3(Sh::THREADS), Sh::SMEM, p);
 }
-template <int BITS, int NT>
+template <int BITS, int HD>
+int launch_nt(e4b_ctx* c, const AttnP& p) {
+  // a warp's n-tiles of 4 heads: one, or two where a sequence may have several rows
+  // (they share the decoded keys and values) and for more than 4 heads
+  if (p.G > 4 || p.d.rows) return launch<BITS, HD, 2, false>(c, p);
+  // few units: all of an SM's warps on one (a 131K-token sequence of 2 KV heads 32 us
+  // against 40 us); more units than SMs: two CTAs per SM (64 x 1..8000 tokens of 4 KV
+  // heads, f16: 33 us against 60 us; 64 x 1035 tokens, 4 bits: 37 us against 41 us)
+  if (p.d.nseq * p.d.KVH <= c->sm_count) return launch<BITS, HD, 1, true>(c, p);
+  return launch<BITS, HD, 1, false>(c, p);
+}
+template <int BITS>
 int launch_hd(e4b_ctx* c, const AttnP& p, int HD) {
-  return HD == 256 ? launch<BITS, 256, NT>(c, p) : (HD == 128 ? launch<BITS, 128, NT>(c, p) : launch<BITS, 64, NT>(c, p));
+  return HD == 256 ? launch_nt<BITS, 256>(c, p) : (HD == 128 ? launch_nt<BITS, 128>(c, p) : launch_nt<BITS, 64>(c, p));
 }
 }  // namespace
 
@@ -964,7 +981,7 @@ extern "C" {
 
 E4B_API size_t e4b_paged_scratch_bytes(void) {
   // two partials for each of kMaxCtas / 2 CTAs of the shape with the largest ones
-  return kMaxCtas * (3 * sizeof(uint32_t) + Shape<4, 256, 2>::PART * sizeof(float));
+  return kMaxCtas * (3 * sizeof(uint32_t) + Shape<4, 256, 2, false>::PART * sizeof(float));
 }
 
 E4B_API int e4b_attn_paged(e4b_ctx* c, const e4b_paged_kv* kv, const float* q, uint16_t* out_h, float* out_f,
@@ -987,11 +1004,7 @@ E4B_API int e4b_attn_paged(e4b_ctx* c, const e4b_paged_kv* kv, const float* q, u
   p.window = (uint32_t)window;
   p.sinks = (uint32_t)sinks;
   p.scale = scale;
-  // a warp's n-tiles of 4 heads: one, or two where a sequence may have several rows
-  // (they share the decoded keys and values) and for more than 4 heads
-  const int NT = p.G > 4 || kv->rows ? 2 : 1;
-  if (kv->bits == 16) return NT == 1 ? launch_hd<16, 1>(c, p, kv->head_dim) : launch_hd<16, 2>(c, p, kv->head_dim);
-  return NT == 1 ? launch_hd<4, 1>(c, p, kv->head_dim) : launch_hd<4, 2>(c, p, kv->head_dim);
+  return kv->bits == 16 ? launch_hd<16>(c, p, kv->head_dim) : launch_hd<4>(c, p, kv->head_dim);
 }
 
 }  // extern "C"
