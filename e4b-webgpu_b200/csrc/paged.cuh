@@ -46,13 +46,14 @@ E4B_DEV uint32_t live_rows(const PagedDev& p) {
   return n;
 }
 
-// Sequence of a live row, looked up by the whole CTA (every thread calls it).
+// Sequence of a live row, looked up by a warp (all 32 lanes call it): the number of
+// sequences after the first that begin at or before the row.
 E4B_DEV int seq_of_row(const PagedDev& p, uint32_t row) {
   if (!p.rows) return (int)row;
   int n = 0;
-  for (int s0 = 1; s0 < p.nseq; s0 += blockDim.x) {
-    const int s = s0 + threadIdx.x;
-    n += __syncthreads_count(s < p.nseq && p.rows[s] <= row);
+  for (int s0 = 1; s0 < p.nseq; s0 += 32) {
+    const int s = s0 + (threadIdx.x & 31);
+    n += __popc(__ballot_sync(0xffffffffu, s < p.nseq && p.rows[s] <= row));
   }
   return n;
 }
