@@ -1,11 +1,10 @@
 // Paged KV cache: head prep (per-head RMSNorm, RoPE) with the append of keys and
 // values in f16 or 4 bits, reading rows back, and advancing the lengths.
 #include "paged.cuh"
+#include "stream.cuh"
 
 namespace {
 using namespace e4b;
-
-constexpr int kThreads = 256;
 
 struct PrepP {
   PagedDev d;
@@ -14,111 +13,182 @@ struct PrepP {
   const float* kw;
   float* q_out;
   int QH, angles, norm, keqv, nparts;
+  int rows_per_turn;                 // rows of a CTA's turn
   int64_t stride;                    // elements between rows
-  uint64_t per_q, per_kv;            // ceil(2^32 / QH), ceil(2^32 / (2 KVH))
+  uint64_t per_q, per_kv;            // ceil(2^32 / QH), ceil(2^32 / (2 KVH)): quotients of small numerators
   float eps;
   double log2_theta;
 };
+
+// How the rows reach the lanes: straight from global memory, a few rows, each spread
+// over CTAs (kFew); through shared memory, whole rows by bulk copies into two stages,
+// so some 150 KB per SM are in flight whatever the lanes do (kStaged); or from global
+// memory, four rows a turn, for what the copies cannot take (kDirect: partial sums,
+// rows that are too long or not 16-byte aligned).
+enum { kFew, kStaged, kDirect };
+constexpr int kTurnRows = 4;         // rows of a turn at most
+constexpr int kStageBytes = 48 * 1024;
+template <int MODE>
+constexpr int threads_of() { return MODE == kStaged ? 512 : 256; }
 
 struct Quad {
   float x[4];
 };
 
-E4B_DEV uint32_t pack2(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
+E4B_DEV __half2 as_h2(uint32_t x) { return *reinterpret_cast<const __half2*>(&x); }
+E4B_DEV uint32_t as_u32(__half2 x) { return *reinterpret_cast<const uint32_t*>(&x); }
+E4B_DEV uint32_t pack2(float lo, float hi) { return as_u32(__floats2half2_rn(lo, hi)); }
 
-// Dims 4q..4q+3 of a head that begins at element `at` of the input rows.
+// Four consecutive elements of an input row.
 template <bool XF16>
-E4B_DEV Quad load_quad(const PrepP& p, int64_t at) {
+E4B_DEV Quad load_quad(const uint8_t* row, int at) {
   Quad r;
   if constexpr (XF16) {
-    const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.qkv) + at);
-    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
+    const uint2 w = *reinterpret_cast<const uint2*>(row + 2 * at);
+    const float2 a = __half22float2(as_h2(w.x)), b = __half22float2(as_h2(w.y));
     r.x[0] = a.x, r.x[1] = a.y, r.x[2] = b.x, r.x[3] = b.y;
   } else {
-    const float* x = static_cast<const float*>(p.qkv) + at;
-    float4 v = *reinterpret_cast<const float4*>(x);
-    for (int k = 1; k < p.nparts; k++) {
-      const float4 w = *reinterpret_cast<const float4*>(x + (int64_t)k * p.d.n_rows * p.stride);
-      v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
-    }
+    const float4 v = *reinterpret_cast<const float4*>(row + 4 * at);
     r.x[0] = v.x, r.x[1] = v.y, r.x[2] = v.z, r.x[3] = v.w;
   }
   return r;
 }
 
-// Four consecutive f16 values of a 32-dim block held by 8 neighbouring lanes ->
-// their q4_0 codes trunc(x / d + 8.5); `d16` is the block's stored scale (the same in
-// all 8 lanes).  x and 8 d are f16, so a quotient that is not exactly between two
-// codes is at least 2^-13 away from there: with 2^-15 added, the product with 1 / d
-// (off by less than 2^-18) gives the exact quotient's code, ties upwards.
-E4B_DEV uint32_t quantise_quad(const uint32_t (&h2)[2], int lane8, uint16_t& d16) {
-  // order by magnitude, then by first index; the sign rides along
-  uint32_t key = 0;
+// With f32 partial sums (never staged), their sum in order.
+template <bool XF16, int MODE>
+E4B_DEV Quad load_parts(const PrepP& p, const uint8_t* row, int at) {
+  Quad v = load_quad<XF16>(row, at);
+  if (MODE != kStaged && !XF16)
+    for (int k = 1; k < p.nparts; k++) {
+      const Quad w = load_quad<XF16>(row + (uint64_t)k * p.d.n_rows * p.stride * 4, at);
 #pragma unroll
-  for (int j = 0; j < 4; j++) {
-    const uint32_t h = j & 1 ? h2[j >> 1] >> 16 : h2[j >> 1] & 0xffffu;
-    key = max(key, ((h & 0x7fffu) << 6) | ((31u - (lane8 * 4 + j)) << 1) | (h >> 15));
-  }
-#pragma unroll
-  for (int o = 1; o < 8; o <<= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
-  const uint32_t mag = key >> 6;
-  const float d = h2f((uint16_t)(mag | (key & 1u) << 15)) * -0.125f;
-  d16 = f2h(d);
-  if (mag >= 0x7c00u) d16 = 0x7fffu;                     // an infinity or NaN in the block
-  if (mag >= 0x7c00u || mag == 0) return 0x8888u;
-  const float inv = 1.f / d;
-  uint32_t w = 0;
-#pragma unroll
-  for (int j = 0; j < 4; j++) {
-    const __half2 h = *reinterpret_cast<const __half2*>(&h2[j >> 1]);
-    const float x = j & 1 ? __high2float(h) : __low2float(h);
-    const float c = fminf(fmaxf(fmaf(x, inv, 8.5f + 1.f / 32768.f), 0.f), 15.f);
-    // adding 2^23 towards minus infinity leaves the integer part in the low bits
-    w |= (__float_as_uint(__fadd_rd(c, 8388608.f)) & 15u) << (4 * j);
-  }
-  return w;
+      for (int j = 0; j < 4; j++) v.x[j] += w.x[j];
+    }
+  return v;
 }
 
-// Where a row goes: its sequence's position, and the page that holds it.
+E4B_DEV float rsqrt_fast(float x) {
+  float y;
+  asm("rsqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+E4B_DEV float rcp_fast(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// x^-1/2 to 64-bit precision: two Newton steps from the f32 estimate.
+E4B_DEV double rsqrt64(double x) {
+  if (!(x > 1e-30 && x < 1e30)) return rsqrt(x);         // the estimate's range
+  double y = (double)rsqrt_fast((float)x);
+#pragma unroll
+  for (int i = 0; i < 2; i++) y = y * fma(-0.5 * x * y, y, 1.5);
+  return y;
+}
+
+// The q4_0 codes of two quads (four consecutive f16 values each, their blocks in 8
+// neighbouring lanes): d = m / -8 for the first element m of the largest magnitude,
+// codes trunc(x / d + 8.5).  x and 8 d are f16, so a quotient that is not exactly
+// between two codes is at least 2^-13 away from there: with 2^-15 added, the product
+// with 1 / d (off by less than 2^-19) gives the exact quotient's code, ties upwards.
+// d16: the blocks' stored scales.
+E4B_DEV void quantise(const uint32_t (&h)[2][2], int lane8, uint32_t (&codes)[2], uint32_t (&d16)[2]) {
+  __half2 hi[2], lo[2];
+#pragma unroll
+  for (int q = 0; q < 2; q++) {
+    hi[q] = __hmax2_nan(as_h2(h[q][0]), as_h2(h[q][1]));
+    lo[q] = __hmin2_nan(as_h2(h[q][0]), as_h2(h[q][1]));
+  }
+  // both quads' largest and smallest values, then over the blocks' lanes
+  __half2 top = __hmax2_nan(__lows2half2(hi[0], hi[1]), __highs2half2(hi[0], hi[1]));
+  __half2 bot = __hmin2_nan(__lows2half2(lo[0], lo[1]), __highs2half2(lo[0], lo[1]));
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) {
+    top = __hmax2_nan(top, as_h2(__shfl_xor_sync(0xffffffffu, as_u32(top), o)));
+    bot = __hmin2_nan(bot, as_h2(__shfl_xor_sync(0xffffffffu, as_u32(bot), o)));
+  }
+#pragma unroll
+  for (int q = 0; q < 2; q++) {
+    const float t = q ? __high2float(top) : __low2float(top), b = q ? __high2float(bot) : __low2float(bot);
+    float m = t > -b ? t : b;
+    if (__any_sync(0xffffffffu, t == -b && t != 0.f)) {  // of both signs: the first one
+      uint32_t first = 64;
+#pragma unroll
+      for (int j = 3; j >= 0; j--) {
+        const float x = j & 1 ? __high2float(as_h2(h[q][j >> 1])) : __low2float(as_h2(h[q][j >> 1]));
+        if (fabsf(x) == t) first = (uint32_t)(lane8 * 4 + j) * 2 + (x < 0.f);
+      }
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
+      if (t == -b && t != 0.f) m = first & 1u ? b : t;
+    }
+    const float d = m * -0.125f;
+    d16[q] = f2h(d);
+    if (!(fabsf(d) < INFINITY)) d16[q] = 0x7fffu;        // an infinity or NaN in the block
+    const float inv = rcp_fast(d);
+    uint32_t w = 0;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const float x = j & 1 ? __high2float(as_h2(h[q][j >> 1])) : __low2float(as_h2(h[q][j >> 1]));
+      const float c = fminf(fmaxf(fmaf(x, inv, 8.5f + 1.f / 32768.f), 0.f), 15.f);
+      // adding 2^23 towards minus infinity leaves the integer part in the low bits
+      w |= (__float_as_uint(__fadd_rd(c, 8388608.f)) & 15u) << (4 * j);
+    }
+    codes[q] = d == 0.f || d16[q] == 0x7fffu ? 0x8888u : w;
+  }
+}
+
+// Where a row goes: its sequence's position, and in the pools the byte of its piece of
+// KV head 0 (head h is h * (page / 16) pieces further) and its slot there.
 struct RowPlace {
-  uint64_t pos;
-  uint32_t page;
-  int in_page, ok;                   // ok: the cache has a slot for it
+  uint64_t pos, offset;
+  int slot, ok;                      // ok: the cache has a slot for it
 };
+template <int PB>
 E4B_DEV RowPlace place_row(const PagedDev& d, uint32_t row) {          // a warp
   const int seq = seq_of_row(d, row);
   RowPlace r;
   r.pos = (uint64_t)d.lens[seq] + (d.rows ? row - d.rows[seq] : 0u);
-  r.in_page = (int)((uint32_t)r.pos % (uint32_t)d.page);
-  r.ok = page_of(d, seq, r.pos, r.page);
+  uint32_t page;
+  r.ok = page_of(d, seq, r.pos, page);
+  const int in_page = (int)((uint32_t)r.pos % (uint32_t)d.page);
+  r.slot = in_page % kPieceSlots;
+  r.offset = piece_offset(page, 0, in_page, d.KVH, d.page, PB);
   return r;
 }
 
-// A CTA takes RB rows at a time; HD/8 lanes take a head, each lane dims 4l..4l+3 and
-// HD/2 + 4l..4l+3, so a rotation pair (p, p + HD/2) and a group of four codes sit in
-// one lane and a 32-dim block in 8 neighbouring lanes.  The rotation's angles are
-// formed once per row for all its heads, in 64 bits (a position of 10^6 times a
-// frequency leaves f32 no fraction).  q is computed in f32.  Keys and values are
-// formed in 64 bits: what is stored is then the rounding of the exact value whatever
-// the order of the sums, so the 4-bit codes do not depend on it.
-// Bound by memory: per row of 16 q + 2 x 4 heads of 256, 24.6 KB read, 16.4 KB of q and
-// 2.3 KB (4 bits) of cache written.
-template <int HD, int RB, int BITS, bool XF16>
-__global__ void __launch_bounds__(kThreads) k_headprep_paged(const PrepP p) {
-  constexpr int LPH = HD / 8, HALF = HD / 2, NS = kThreads / LPH;
-  __shared__ double2 turn[RB][HALF];                     // (cos, sin) of the rows' angles
-  __shared__ float2 turn32[RB][HALF];
+// HD/8 lanes take a head, each lane dims 4l..4l+3 and HD/2 + 4l..4l+3, so a rotation
+// pair (p, p + HD/2) and a group of four codes sit in one lane and a 32-dim block in 8
+// neighbouring lanes.  The rotation's angles are formed once per row for all its heads,
+// in 64 bits (a position of 10^6 times a frequency leaves f32 no fraction).  q is
+// computed in f32.  Keys and values are formed in 64 bits: what is stored is then the
+// rounding of the exact value whatever the order of the sums, so the 4-bit codes do not
+// depend on it.  Bound by memory for many rows (per row of 16 q + 2 x 4 heads of 256:
+// 24.6 KB read, 16.4 KB of q and 2.3 KB of 4-bit cache written), by latency for few.
+template <int HD, int BITS, bool XF16, int MODE>
+__global__ void __launch_bounds__(threads_of<MODE>(), MODE == kFew ? 1 : 2) k_headprep_paged(const PrepP p) {
+  constexpr int LPH = HD / 8, HALF = HD / 2, PB = BITS == 16 ? 32 * HD : 9 * HD, ES = XF16 ? 2 : 4;
+  constexpr int THREADS = threads_of<MODE>(), NS = THREADS / LPH, ROWS = MODE == kFew ? 1 : kTurnRows;
+  extern __shared__ __align__(128) uint8_t stages[];     // kStaged: 2 x kStageBytes
+  __shared__ __align__(16) double2 turn[ROWS][HALF];     // (cos, sin) of the rows' angles
+  __shared__ __align__(16) float2 turn32[ROWS][HALF];
   __shared__ double kw64[HD];
-  __shared__ RowPlace place[RB];
+  __shared__ RowPlace place[ROWS];
+  __shared__ uint64_t landed[2];
   const int tid = threadIdx.x, warp = tid >> 5, l = tid % LPH, sub = tid / LPH, lane8 = l & 7;
-  const int KVH = p.d.KVH;
-  constexpr int pb = BITS == 16 ? 32 * HD : 9 * HD;
+  const int KVH = p.d.KVH, RT = MODE == kFew ? 1 : p.rows_per_turn;
+  const uint32_t head_bytes = (uint32_t)(p.d.page / kPieceSlots) * PB;
+  const uint32_t row_bytes = (uint32_t)(p.QH + KVH * (p.keqv ? 1 : 2)) * HD * ES;
+  const uint8_t* const qkv = static_cast<const uint8_t*>(p.qkv);
   // pair tid % HALF of the angles; 1/pi: sincospi reduces its argument exactly
   const int pair = tid % HALF;
   const double freq = pair < p.angles ? exp2((-2.0 * pair / HD) * p.log2_theta) * 0.3183098861837906715 : 0.0;
+  const int turned = min(max(p.angles - 4 * l, 0), 4);   // of the lane's four pairs
+  if (MODE == kStaged && tid == 0) {
+    mbar_init(&landed[0], 1);
+    mbar_init(&landed[1], 1);
+    fence_barrier_init();
+  }
   float qw[8];
 #pragma unroll
   for (int j = 0; j < 8; j++) qw[j] = 1.f;
@@ -127,166 +197,204 @@ __global__ void __launch_bounds__(kThreads) k_headprep_paged(const PrepP p) {
       const float4 a = *reinterpret_cast<const float4*>(p.qw + 4 * l), b = *reinterpret_cast<const float4*>(p.qw + HALF + 4 * l);
       qw[0] = a.x, qw[1] = a.y, qw[2] = a.z, qw[3] = a.w, qw[4] = b.x, qw[5] = b.y, qw[6] = b.z, qw[7] = b.w;
     }
-    for (int i = tid; i < HD; i += kThreads) kw64[i] = (double)p.kw[i];
+    for (int i = tid; i < HD; i += THREADS) kw64[i] = (double)p.kw[i];
   }
   pdl_wait();
-  const uint32_t live = live_rows(p.d);
-  for (uint32_t row0 = blockIdx.x * RB; row0 < live; row0 += gridDim.x * RB) {
-    const int rows = (int)min((uint32_t)RB, live - row0);
-    __syncthreads();                 // the previous rows' angles and places have been used
+  const uint32_t live = live_rows(p.d), first_row = blockIdx.x * RT, stride_rows = gridDim.x * RT;
+  const auto bring = [&](uint32_t turn_no) {             // thread 0: the rows of a turn into its stage
+    const uint64_t row = (uint64_t)first_row + (uint64_t)turn_no * stride_rows;
+    if (row >= live) return;
+    const int n = (int)min((uint64_t)RT, live - row);
+    uint64_t* bar = &landed[turn_no & 1];
+    mbar_expect_tx(bar, n * row_bytes);
+    for (int i = 0; i < n; i++)
+      bulk_g2s(stages + (turn_no & 1) * kStageBytes + i * row_bytes, qkv + (row + i) * (uint64_t)p.stride * ES, row_bytes, bar);
+  };
+  if (MODE == kStaged && tid == 0) {
+    bring(0);
+    bring(1);
+  }
+  __syncthreads();
+  uint32_t turn_no = 0;
+  bool alive = true;
+  for (uint32_t row0 = first_row; row0 < live; row0 += stride_rows, turn_no++) {
+    const int rows = (int)min((uint32_t)RT, live - row0);
     if (warp < rows) {
-      const RowPlace r = place_row(p.d, row0 + warp);
-      if ((tid & 31) == 0) place[warp] = r;
+      const RowPlace pl = place_row<PB>(p.d, row0 + warp);
+      if ((tid & 31) == 0) place[warp] = pl;
     }
     __syncthreads();
-    for (int r = tid / HALF; r < rows; r += kThreads / HALF)
+    for (int i = tid / HALF; i < rows; i += THREADS / HALF)
       if (pair < p.angles) {
         double s, c;
-        sincospi((double)place[r].pos * freq, &s, &c);
-        turn[r][pair] = make_double2(c, s);
-        turn32[r][pair] = make_float2((float)c, (float)s);
+        sincospi((double)place[i].pos * freq, &s, &c);
+        turn[i][pair] = make_double2(c, s);
+        turn32[i][pair] = make_float2((float)c, (float)s);
       }
     __syncthreads();
-    // every lane of a warp makes the same number of turns (the shuffles below)
-    const int nq = rows * p.QH, nkv = rows * 2 * KVH, qpasses = (nq + NS - 1) / NS;
+    if constexpr (MODE == kStaged)
+      alive = __all_sync(0xffffffffu, mbar_wait(&landed[turn_no & 1], (turn_no >> 1) & 1u, p.d.status));
+    const uint8_t* const rows_at = MODE == kStaged ? stages + (turn_no & 1) * kStageBytes : qkv + (uint64_t)row0 * p.stride * ES;
+    const uint64_t rows_by = MODE == kStaged ? row_bytes : (uint64_t)p.stride * ES;
+    // Head i of the rows' query heads (then of their key and value heads) goes to lane
+    // group i % NS of pass i / NS; the passes are dealt to blockIdx.y.  Every lane of a
+    // warp makes the same turns (shuffles): a group without a head repeats the last one.
+    const int nq = alive ? rows * p.QH : 0, nkv = alive ? rows * 2 * KVH : 0, qpasses = (nq + NS - 1) / NS;
 #pragma unroll 2
     for (int ps = blockIdx.y; ps < qpasses; ps += gridDim.y) {
-      const int i0 = ps * NS;
-      const int i = min(i0 + sub, nq - 1), r = RB == 1 ? 0 : (int)((i * p.per_q) >> 32), h = i - r * p.QH;
-      const uint32_t row = row0 + r;
-      const int64_t at = (int64_t)row * p.stride + (int64_t)h * HD + 4 * l;
-      Quad a = load_quad<XF16>(p, at), b = load_quad<XF16>(p, at + HALF);
+      const int at = ps * NS + sub, i = min(at, nq - 1), r = ROWS == 1 ? 0 : (int)((i * p.per_q) >> 32), h = i - r * p.QH;
+      Quad a = load_parts<XF16, MODE>(p, rows_at + r * rows_by, h * HD + 4 * l);
+      Quad b = load_parts<XF16, MODE>(p, rows_at + r * rows_by, h * HD + HALF + 4 * l);
+      float(&xa)[4] = a.x;
+      float(&xb)[4] = b.x;
       if (p.norm) {
         float s = 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; j++) s = fmaf(a.x[j], a.x[j], fmaf(b.x[j], b.x[j], s));
+        for (int j = 0; j < 4; j++) s = fmaf(xa[j], xa[j], fmaf(xb[j], xb[j], s));
 #pragma unroll
         for (int o = 1; o < LPH; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        const float inv = rms_scale(s, HD, p.eps);
+        const float inv = rsqrt_fast(s * (1.f / HD) + p.eps);
 #pragma unroll
-        for (int j = 0; j < 4; j++) a.x[j] *= inv * qw[j], b.x[j] *= inv * qw[4 + j];
+        for (int j = 0; j < 4; j++) xa[j] *= inv * qw[j], xb[j] *= inv * qw[4 + j];
       }
+      if (turned) {
+        const float4 c0 = *reinterpret_cast<const float4*>(&turn32[r][4 * l]);
+        const float4 c1 = *reinterpret_cast<const float4*>(&turn32[r][4 * l + 2]);
+        const float cs[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
 #pragma unroll
-      for (int j = 0; j < 4; j++)
-        if (4 * l + j < p.angles) {
-          const float2 cs = turn32[r][4 * l + j];
-          const float y = a.x[j] * cs.x - b.x[j] * cs.y;
-          b.x[j] = a.x[j] * cs.y + b.x[j] * cs.x;
-          a.x[j] = y;
+        for (int j = 0; j < 4; j++) {
+          const float y = xa[j] * cs[2 * j] - xb[j] * cs[2 * j + 1], z = xa[j] * cs[2 * j + 1] + xb[j] * cs[2 * j];
+          if (j < turned) xa[j] = y, xb[j] = z;
         }
-      if (i0 + sub < nq) {
-        float* qo = p.q_out + ((size_t)row * p.QH + h) * HD + 4 * l;
-        *reinterpret_cast<float4*>(qo) = make_float4(a.x[0], a.x[1], a.x[2], a.x[3]);
-        *reinterpret_cast<float4*>(qo + HALF) = make_float4(b.x[0], b.x[1], b.x[2], b.x[3]);
+      }
+      if (at < nq) {
+        float* qo = p.q_out + ((size_t)row0 * p.QH + at) * HD + 4 * l;
+        *reinterpret_cast<float4*>(qo) = make_float4(xa[0], xa[1], xa[2], xa[3]);
+        *reinterpret_cast<float4*>(qo + HALF) = make_float4(xb[0], xb[1], xb[2], xb[3]);
       }
     }
-    for (int i0 = (int)((blockIdx.y + gridDim.y - qpasses % gridDim.y) % gridDim.y) * NS; i0 < nkv; i0 += gridDim.y * NS) {
-      const int i = min(i0 + sub, nkv - 1), r = RB == 1 ? 0 : (int)((i * p.per_kv) >> 32), h = i - r * 2 * KVH;
+    const int first = (int)((blockIdx.y + gridDim.y - (uint32_t)qpasses % gridDim.y) % gridDim.y);
+    for (int i0 = first * NS; i0 < nkv; i0 += gridDim.y * NS) {
+      const int i = min(i0 + sub, nkv - 1), r = ROWS == 1 ? 0 : (int)((i * p.per_kv) >> 32), h = i - r * 2 * KVH;
       const bool is_v = h >= KVH;
-      const int kvh = is_v ? h - KVH : h;
-      const uint32_t row = row0 + r;
-      const int64_t at = (int64_t)row * p.stride + (int64_t)(p.QH + (p.keqv ? kvh : h)) * HD + 4 * l;
-      const Quad a = load_quad<XF16>(p, at), b = load_quad<XF16>(p, at + HALF);
+      const int kvh = is_v ? h - KVH : h, at = (p.QH + (p.keqv ? kvh : h)) * HD + 4 * l;
+      const Quad a = load_parts<XF16, MODE>(p, rows_at + r * rows_by, at), b = load_parts<XF16, MODE>(p, rows_at + r * rows_by, at + HALF);
       double inv = 1.0;
       if (p.norm) {
         double s = 0.0;
 #pragma unroll
-        for (int j = 0; j < 4; j++) s += (double)a.x[j] * a.x[j] + (double)b.x[j] * b.x[j];
+        for (int j = 0; j < 4; j++) s = fma((double)a.x[j], (double)a.x[j], fma((double)b.x[j], (double)b.x[j], s));
 #pragma unroll
         for (int o = 1; o < LPH; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        inv = rsqrt(s / HD + (double)p.eps);
+        inv = rsqrt64(s * (1.0 / HD) + (double)p.eps);
       }
       float fa[4], fb[4];
+      if (is_v || (!p.norm && !turned)) {
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        double xa = (double)a.x[j] * inv, xb = (double)b.x[j] * inv;
-        if (!is_v) {
+        for (int j = 0; j < 4; j++) fa[j] = (float)((double)a.x[j] * inv), fb[j] = (float)((double)b.x[j] * inv);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          double xa = (double)a.x[j] * inv, xb = (double)b.x[j] * inv;
           if (p.norm) xa *= kw64[4 * l + j], xb *= kw64[HALF + 4 * l + j];
-          if (4 * l + j < p.angles) {
+          if (j < turned) {
             const double2 cs = turn[r][4 * l + j];
             const double y = xa * cs.x - xb * cs.y;
             xb = xa * cs.y + xb * cs.x;
             xa = y;
           }
+          fa[j] = (float)xa;
+          fb[j] = (float)xb;
         }
-        fa[j] = (float)xa;
-        fb[j] = (float)xb;
       }
-      const uint32_t ha[2] = {pack2(fa[0], fa[1]), pack2(fa[2], fa[3])}, hb[2] = {pack2(fb[0], fb[1]), pack2(fb[2], fb[3])};
-      uint16_t da = 0, db = 0;
-      uint32_t ca = 0, cb = 0;
-      if constexpr (BITS == 4) {
-        ca = quantise_quad(ha, lane8, da);
-        cb = quantise_quad(hb, lane8, db);
-      }
-      const RowPlace pl = place[r];
-      if (i0 + sub >= nkv || !pl.ok) continue;
-      const int s = pl.in_page % kPieceSlots;
-      uint8_t* piece = (is_v ? p.d.v : p.d.k) + piece_offset(pl.page, kvh, pl.in_page, KVH, p.d.page, pb);
-      const int qa = l, qb = l + LPH;
-      if constexpr (BITS == 16) {
-        *reinterpret_cast<uint2*>(piece + (is_v ? v16_quad(s, qa) : k16_quad(s, qa))) = make_uint2(ha[0], ha[1]);
-        *reinterpret_cast<uint2*>(piece + (is_v ? v16_quad(s, qb) : k16_quad(s, qb))) = make_uint2(hb[0], hb[1]);
-      } else {
-        *reinterpret_cast<uint16_t*>(piece + (is_v ? v4_quad(s, qa, HD) : k4_quad(s, qa, HD))) = (uint16_t)ca;
-        *reinterpret_cast<uint16_t*>(piece + (is_v ? v4_quad(s, qb, HD) : k4_quad(s, qb, HD))) = (uint16_t)cb;
-        if (lane8 == 0) {
-          *reinterpret_cast<uint16_t*>(piece + (is_v ? v4_scale(s, qa / 8, HD) : k4_scale(s, qa / 8, HD))) = da;
-          *reinterpret_cast<uint16_t*>(piece + (is_v ? v4_scale(s, qb / 8, HD) : k4_scale(s, qb / 8, HD))) = db;
+      const uint32_t w[2][2] = {{pack2(fa[0], fa[1]), pack2(fa[2], fa[3])}, {pack2(fb[0], fb[1]), pack2(fb[2], fb[3])}};
+      uint32_t codes[2] = {0u, 0u}, d16[2] = {0u, 0u};
+      if constexpr (BITS == 4) quantise(w, lane8, codes, d16);
+      if (i0 + sub >= nkv || !place[r].ok) continue;
+      const int s = place[r].slot;
+      uint8_t* piece = (is_v ? p.d.v : p.d.k) + place[r].offset + (uint64_t)head_bytes * kvh;
+#pragma unroll
+      for (int k = 0; k < 2; k++) {
+        const int q = l + k * LPH;
+        if constexpr (BITS == 16) {
+          *reinterpret_cast<uint2*>(piece + (is_v ? v16_quad(s, q) : k16_quad(s, q))) = make_uint2(w[k][0], w[k][1]);
+        } else {
+          *reinterpret_cast<uint16_t*>(piece + (is_v ? v4_quad(s, q, HD) : k4_quad(s, q, HD))) = (uint16_t)codes[k];
+          if (lane8 == 0)
+            *reinterpret_cast<uint16_t*>(piece + (is_v ? v4_scale(s, q / 8, HD) : k4_scale(s, q / 8, HD))) = (uint16_t)d16[k];
         }
       }
     }
+    // the turn's rows, angles and places have been used
+    if constexpr (MODE == kStaged) {
+      if (!__syncthreads_and(alive)) break;
+      if (tid == 0) bring(turn_no + 2);
+    } else {
+      __syncthreads();
+    }
   }
+  if (MODE == kStaged && !alive)     // after a time-out: copies still in flight land (bounded)
+    for (uint32_t i = 0; i < 2; i++)
+      if ((uint64_t)first_row + (uint64_t)(turn_no + i) * stride_rows < live)
+        mbar_wait(&landed[(turn_no + i) & 1], ((turn_no + i) >> 1) & 1u, p.d.status);
 }
 
 // Rows back out of the pages: a warp per row (several where rows are few), a lane per
 // 8 elements (two quads that the layouts keep in one 16-byte or 4-byte word).
 template <int HD, int BITS>
 __global__ void __launch_bounds__(128) k_kvread_paged(const PagedDev d, void* k_out, void* v_out, int out_f32) {
+  constexpr int PB = BITS == 16 ? 32 * HD : 9 * HD;
   pdl_wait();
   const uint32_t live = live_rows(d);
   const int per = d.KVH * HD / 8;
-  constexpr int pb = BITS == 16 ? 32 * HD : 9 * HD;
+  const uint32_t head_bytes = (uint32_t)(d.page / kPieceSlots) * PB;
   for (uint32_t row = blockIdx.x * 4 + (threadIdx.x >> 5); row < live; row += gridDim.x * 4) {
-    const RowPlace pl = place_row(d, row);
-    const int s = pl.in_page % kPieceSlots;
-#pragma unroll 4
-    for (int e = blockIdx.y * 32 + (threadIdx.x & 31); e < 2 * per; e += gridDim.y * 32) {
-      const bool is_v = e >= per;
+    const RowPlace pl = place_row<PB>(d, row);
+    const int s = pl.slot;
+#pragma unroll
+    for (int is_v = 0; is_v < 2; is_v++) {
       void* out = is_v ? v_out : k_out;
       if (!out) continue;
-      const int r = is_v ? e - per : e, h = r / (HD / 8), w = r % (HD / 8);
-      // the word's two quads: dims 8w.. (f16, and 4-bit keys); the same quad of two blocks (4-bit values)
-      const bool split = BITS == 4 && is_v;
-      const int q0 = split ? (w >> 3) * 16 + (w & 7) : 2 * w, q1 = split ? q0 + 8 : 2 * w + 1;
-      float x[8];
-#pragma unroll
-      for (int j = 0; j < 8; j++) x[j] = 0.f;
-      if (pl.ok) {
-        const uint8_t* piece = (is_v ? d.v : d.k) + piece_offset(pl.page, h, pl.in_page, d.KVH, d.page, pb);
-        if constexpr (BITS == 16) {
-          const uint4 v = *reinterpret_cast<const uint4*>(piece + (is_v ? v16_quad(s, q0) : k16_quad(s, q0)));
-          const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-          for (int j = 0; j < 8; j++) x[j] = h2f((uint16_t)(u[j >> 1] >> (16 * (j & 1))));
-        } else {
-          const uint32_t v = *reinterpret_cast<const uint32_t*>(piece + (is_v ? v4_quad(s, q0, HD) : k4_quad(s, q0, HD)));
-          const uint16_t* d0 = reinterpret_cast<const uint16_t*>(piece + (is_v ? v4_scale(s, q0 / 8, HD) : k4_scale(s, q0 / 8, HD)));
-          const uint16_t* d1 = reinterpret_cast<const uint16_t*>(piece + (is_v ? v4_scale(s, q1 / 8, HD) : k4_scale(s, q1 / 8, HD)));
-          const float s0 = h2f(*d0), s1 = h2f(*d1);
-#pragma unroll
-          for (int j = 0; j < 8; j++) x[j] = (j < 4 ? s0 : s1) * (float)((int)((v >> (4 * j)) & 15u) - 8);
+      const uint8_t* pool = (is_v ? d.v : d.k) + pl.offset;
+      const size_t at = (size_t)row * d.KVH * HD;
+#pragma unroll 4
+      for (int e = blockIdx.y * 32 + (threadIdx.x & 31); e < per; e += gridDim.y * 32) {
+        const int h = e / (HD / 8), w = e % (HD / 8);
+        // the word's two quads: dims 8w.. (f16, and 4-bit keys); the same quad of two blocks (4-bit values)
+        const int q0 = BITS == 4 && is_v ? (w >> 3) * 16 + (w & 7) : 2 * w, q1 = BITS == 4 && is_v ? q0 + 8 : 2 * w + 1;
+        const uint8_t* piece = pool + (uint64_t)head_bytes * h;
+        uint32_t y[4] = {0u, 0u, 0u, 0u};                // the two quads as f16 pairs
+        float sc[2] = {0.f, 0.f};
+        uint32_t codes = 0x88888888u;
+        if (pl.ok) {
+          if constexpr (BITS == 16) {
+            const uint4 v = *reinterpret_cast<const uint4*>(piece + (is_v ? v16_quad(s, q0) : k16_quad(s, q0)));
+            y[0] = v.x, y[1] = v.y, y[2] = v.z, y[3] = v.w;
+          } else {
+            codes = *reinterpret_cast<const uint32_t*>(piece + (is_v ? v4_quad(s, q0, HD) : k4_quad(s, q0, HD)));
+            sc[0] = h2f(*reinterpret_cast<const uint16_t*>(piece + (is_v ? v4_scale(s, q0 / 8, HD) : k4_scale(s, q0 / 8, HD))));
+            sc[1] = is_v ? h2f(*reinterpret_cast<const uint16_t*>(piece + v4_scale(s, q1 / 8, HD))) : sc[0];
+          }
         }
-      }
-      const size_t at = (size_t)row * d.KVH * HD + (size_t)h * HD;
+        const size_t o0 = at + (size_t)h * HD + 4 * q0, o1 = at + (size_t)h * HD + 4 * q1;
+        if (BITS == 16 && !out_f32) {
+          *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + o0) = make_uint4(y[0], y[1], y[2], y[3]);
+          continue;
+        }
+        float x[8];
 #pragma unroll
-      for (int k = 0; k < 2; k++) {
-        const size_t o = at + 4 * (k ? q1 : q0);
-        const float* y = x + 4 * k;
-        if (out_f32) *reinterpret_cast<float4*>(static_cast<float*>(out) + o) = make_float4(y[0], y[1], y[2], y[3]);
-        else
-          *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + o) =
-              make_uint2(f2h(y[0]) | (uint32_t)f2h(y[1]) << 16, f2h(y[2]) | (uint32_t)f2h(y[3]) << 16);
+        for (int j = 0; j < 8; j++) {
+          if constexpr (BITS == 16) x[j] = h2f((uint16_t)(y[j >> 1] >> (16 * (j & 1))));
+          else x[j] = sc[j >> 2] * (float)((int)((codes >> (4 * j)) & 15u) - 8);
+        }
+        if (out_f32) {
+          *reinterpret_cast<float4*>(static_cast<float*>(out) + o0) = make_float4(x[0], x[1], x[2], x[3]);
+          *reinterpret_cast<float4*>(static_cast<float*>(out) + o1) = make_float4(x[4], x[5], x[6], x[7]);
+        } else {
+          const uint2 a = make_uint2(pack2(x[0], x[1]), pack2(x[2], x[3])), b = make_uint2(pack2(x[4], x[5]), pack2(x[6], x[7]));
+          *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + o0) = a;
+          *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + o1) = b;
+        }
       }
     }
   }
@@ -297,13 +405,32 @@ __global__ void k_paged_advance(uint32_t* lens, const uint32_t* __restrict__ row
   const int s = blockIdx.x * blockDim.x + threadIdx.x;
   if (s < nseq) lens[s] += rows ? rows[s + 1] - rows[s] : 1u;
 }
+
+template <int HD, int MODE>
+int launch_prep(e4b_ctx* c, const PrepP& p, int bits, int x_f16, dim3 grid) {
+  auto kern = bits == 16 ? (x_f16 ? k_headprep_paged<HD, 16, true, MODE> : k_headprep_paged<HD, 16, false, MODE>)
+                         : (x_f16 ? k_headprep_paged<HD, 4, true, MODE> : k_headprep_paged<HD, 4, false, MODE>);
+  const size_t smem = MODE == kStaged ? 2 * kStageBytes : 0;
+  if (smem) E4B_CUDA(c, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  return e4b_launch(c, "headprep_paged", kern, grid, dim3(threads_of<MODE>()), smem, p);
+}
+
 template <int HD>
-int launch_prep(e4b_ctx* c, const PrepP& p, int bits, int x_f16, bool few, dim3 grid) {
-  auto kern = few ? (bits == 16 ? (x_f16 ? k_headprep_paged<HD, 1, 16, true> : k_headprep_paged<HD, 1, 16, false>)
-                                : (x_f16 ? k_headprep_paged<HD, 1, 4, true> : k_headprep_paged<HD, 1, 4, false>))
-                  : (bits == 16 ? (x_f16 ? k_headprep_paged<HD, 4, 16, true> : k_headprep_paged<HD, 4, 16, false>)
-                                : (x_f16 ? k_headprep_paged<HD, 4, 4, true> : k_headprep_paged<HD, 4, 4, false>));
-  return e4b_launch(c, "headprep_paged", kern, grid, dim3(kThreads), 0, p);
+int launch_prep(e4b_ctx* c, PrepP& p, int bits, int x_f16) {
+  // few rows: a row per CTA, and a CTA per pass over its heads (latency); the rest in
+  // turns of up to four rows, which share the barriers and the lookups
+  const int ns = threads_of<kFew>() / (HD / 8);
+  const int passes = (p.QH + ns - 1) / ns + (2 * p.d.KVH + ns - 1) / ns;
+  if ((int64_t)p.d.n_rows * passes <= 8 * c->sm_count)
+    return launch_prep<HD, kFew>(c, p, bits, x_f16, dim3(p.d.n_rows, passes));
+  const int es = x_f16 ? 2 : 4;
+  const int64_t row_bytes = (int64_t)(p.QH + p.d.KVH * (p.keqv ? 1 : 2)) * HD * es;
+  const bool staged = p.nparts == 1 && row_bytes <= kStageBytes && reinterpret_cast<uintptr_t>(p.qkv) % 16 == 0 &&
+                      p.stride * es % 16 == 0;
+  p.rows_per_turn = staged && kStageBytes / row_bytes < kTurnRows ? (int)(kStageBytes / row_bytes) : kTurnRows;
+  const int turns = (p.d.n_rows + p.rows_per_turn - 1) / p.rows_per_turn, resident = 2 * c->sm_count;
+  const dim3 grid(turns < resident ? turns : resident);
+  return staged ? launch_prep<HD, kStaged>(c, p, bits, x_f16, grid) : launch_prep<HD, kDirect>(c, p, bits, x_f16, grid);
 }
 }  // namespace
 
@@ -336,21 +463,14 @@ E4B_API int e4b_headprep_paged(e4b_ctx* c, const e4b_paged_kv* kv, const void* q
   p.norm = norm ? 1 : 0;
   p.keqv = keqv ? 1 : 0;
   p.nparts = nparts;
+  p.rows_per_turn = 1;
   p.stride = row_stride ? row_stride : (int64_t)(QH + kv->kv_heads * (keqv ? 1 : 2)) * HD;
   p.per_q = QH > 0 ? (((uint64_t)1 << 32) + QH - 1) / QH : 0;
   p.per_kv = (((uint64_t)1 << 32) + 2 * kv->kv_heads - 1) / (2 * kv->kv_heads);
   p.eps = eps;
   p.log2_theta = log2((double)theta);
-  // few rows: a row per CTA, and a CTA per pass over its heads, so that a row spreads
-  // over several SMs (latency); many: four rows share the barriers and the lookups
-  const int ns = kThreads / (HD / 8), passes = (QH + ns - 1) / ns + (2 * kv->kv_heads + ns - 1) / ns;
-  const int most = 8 * c->sm_count;
-  const bool few = (int64_t)n_rows * passes <= most;
-  const int groups = (n_rows + 3) / 4;
-  const dim3 grid = few ? dim3(n_rows, passes) : dim3(groups < most ? groups : most);
-  return HD == 256 ? launch_prep<256>(c, p, kv->bits, x_f16, few, grid)
-                   : (HD == 128 ? launch_prep<128>(c, p, kv->bits, x_f16, few, grid)
-                                : launch_prep<64>(c, p, kv->bits, x_f16, few, grid));
+  return HD == 256 ? launch_prep<256>(c, p, kv->bits, x_f16)
+                   : (HD == 128 ? launch_prep<128>(c, p, kv->bits, x_f16) : launch_prep<64>(c, p, kv->bits, x_f16));
 }
 
 E4B_API int e4b_kvread_paged(e4b_ctx* c, const e4b_paged_kv* kv, void* k_out, void* v_out, int out_f32, int n_rows) {
@@ -358,10 +478,9 @@ E4B_API int e4b_kvread_paged(e4b_ctx* c, const e4b_paged_kv* kv, void* k_out, vo
   const char* fault = kvread_paged_fault(kv, k_out, v_out, n_rows);
   E4B_REQUIRE(c, !fault, "kvread_paged: %s", fault);
   if (n_rows == 0) return E4B_OK;
-  const int groups = (n_rows + 3) / 4, most = 16 * c->sm_count;
-  const int slices = (2 * kv->kv_heads * kv->head_dim / 8 + 63) / 64;   // of two turns a warp
-  const dim3 grid = groups * slices <= most ? dim3(groups, slices) : dim3(groups < most ? groups : most);
-  const int HD = kv->head_dim;
+  const int HD = kv->head_dim, groups = (n_rows + 3) / 4, most = 16 * c->sm_count;
+  const int slices = (kv->kv_heads * HD / 8 + 31) / 32;  // of one turn a warp
+  const dim3 grid = (int64_t)groups * slices <= most ? dim3(groups, slices) : dim3(groups < most ? groups : most);
   auto kern = kv->bits == 16 ? (HD == 256 ? k_kvread_paged<256, 16> : (HD == 128 ? k_kvread_paged<128, 16> : k_kvread_paged<64, 16>))
                              : (HD == 256 ? k_kvread_paged<256, 4> : (HD == 128 ? k_kvread_paged<128, 4> : k_kvread_paged<64, 4>));
   return e4b_launch(c, "kvread_paged", kern, grid, dim3(128), 0, paged_dev(c, kv, n_rows), k_out, v_out, out_f32 ? 1 : 0);
