@@ -23,11 +23,12 @@ struct PrepP {
 // How the rows reach the lanes: straight from global memory, a few rows, each spread
 // over CTAs (kFew); through shared memory, whole rows by bulk copies into two stages,
 // so some 150 KB per SM are in flight whatever the lanes do (kStaged); or from global
-// memory, four rows a turn, for what the copies cannot take (kDirect: partial sums,
+// memory, some rows a turn, for what the copies cannot take (kDirect: partial sums,
 // rows that are too long or not 16-byte aligned).
 enum { kFew, kStaged, kDirect };
-constexpr int kTurnRows = 4;         // rows of a turn at most
 constexpr int kStageBytes = 48 * 1024;
+constexpr int kBatch = 64;           // rows whose places are looked up at once
+constexpr int turn_rows(int HD) { return 512 / HD; }     // rows of a turn at most
 template <int MODE>
 constexpr int threads_of() { return MODE == kStaged ? 512 : 256; }
 
@@ -145,8 +146,7 @@ struct RowPlace {
   int slot, ok;                      // ok: the cache has a slot for it
 };
 template <int PB>
-E4B_DEV RowPlace place_row(const PagedDev& d, uint32_t row) {          // a warp
-  const int seq = seq_of_row(d, row);
+E4B_DEV RowPlace place_in(const PagedDev& d, uint32_t row, int seq) {
   RowPlace r;
   r.pos = (uint64_t)d.lens[seq] + (d.rows ? row - d.rows[seq] : 0u);
   uint32_t page;
@@ -155,6 +155,20 @@ E4B_DEV RowPlace place_row(const PagedDev& d, uint32_t row) {          // a warp
   r.slot = in_page % kPieceSlots;
   r.offset = piece_offset(page, 0, in_page, d.KVH, d.page, PB);
   return r;
+}
+template <int PB>
+E4B_DEV RowPlace place_row(const PagedDev& d, uint32_t row) {          // a warp
+  return place_in<PB>(d, row, seq_of_row(d, row));
+}
+template <int PB>
+E4B_DEV RowPlace place_one(const PagedDev& d, uint32_t row) {          // a thread: the last sequence that begins by the row
+  int lo = 0, hi = d.rows ? d.nseq - 1 : 0;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) / 2;
+    if (d.rows[mid] <= row) lo = mid;
+    else hi = mid - 1;
+  }
+  return place_in<PB>(d, row, d.rows ? lo : (int)row);
 }
 
 // HD/8 lanes take a head, each lane dims 4l..4l+3 and HD/2 + 4l..4l+3, so a rotation
@@ -168,12 +182,13 @@ E4B_DEV RowPlace place_row(const PagedDev& d, uint32_t row) {          // a warp
 template <int HD, int BITS, bool XF16, int MODE>
 __global__ void __launch_bounds__(threads_of<MODE>(), MODE == kFew ? 1 : 2) k_headprep_paged(const PrepP p) {
   constexpr int LPH = HD / 8, HALF = HD / 2, PB = BITS == 16 ? 32 * HD : 9 * HD, ES = XF16 ? 2 : 4;
-  constexpr int THREADS = threads_of<MODE>(), NS = THREADS / LPH, ROWS = MODE == kFew ? 1 : kTurnRows;
+  constexpr int THREADS = threads_of<MODE>(), NS = THREADS / LPH, ROWS = MODE == kFew ? 1 : turn_rows(HD);
   extern __shared__ __align__(128) uint8_t stages[];     // kStaged: 2 x kStageBytes
-  __shared__ __align__(16) double2 turn[ROWS][HALF];     // (cos, sin) of the rows' angles
-  __shared__ __align__(16) float2 turn32[ROWS][HALF];
+  constexpr int BUFS = MODE == kFew ? 1 : 2, BATCH = MODE == kFew ? 1 : kBatch;
+  __shared__ __align__(16) double2 turns[BUFS][ROWS][HALF];            // (cos, sin) of a turn's angles
+  __shared__ __align__(16) float2 turns32[BUFS][ROWS][HALF];
   __shared__ double kw64[HD];
-  __shared__ RowPlace place[ROWS];
+  __shared__ RowPlace places[BATCH];
   __shared__ uint64_t landed[2];
   const int tid = threadIdx.x, warp = tid >> 5, l = tid % LPH, sub = tid / LPH, lane8 = l & 7;
   const int KVH = p.d.KVH, RT = MODE == kFew ? 1 : p.rows_per_turn;
@@ -214,24 +229,43 @@ __global__ void __launch_bounds__(threads_of<MODE>(), MODE == kFew ? 1 : 2) k_he
     bring(0);
     bring(1);
   }
+  // rows of turn n, and the places of the batch that begins with it
+  const auto rows_of = [&](uint32_t n) -> int {
+    const uint64_t row = (uint64_t)first_row + (uint64_t)n * stride_rows;
+    return row >= live ? 0 : (int)min((uint64_t)RT, live - row);
+  };
+  const int batch_turns = BATCH / RT;
+  const auto look_up = [&](uint32_t n) {
+    if constexpr (MODE == kFew) {
+      if (warp == 0 && rows_of(n)) {
+        const RowPlace pl = place_row<PB>(p.d, first_row + n * stride_rows);
+        if (tid == 0) places[0] = pl;
+      }
+    } else if (tid < batch_turns * RT && tid % RT < rows_of(n + tid / RT)) {
+      places[tid] = place_one<PB>(p.d, first_row + (n + tid / RT) * stride_rows + tid % RT);
+    }
+    __syncthreads();
+  };
+  const auto form_angles = [&](uint32_t n) {
+    const int base = (int)(n % batch_turns) * RT;
+    for (int i = tid / HALF; i < rows_of(n); i += THREADS / HALF)
+      if (pair < p.angles) {
+        double s, c;
+        sincospi((double)places[base + i].pos * freq, &s, &c);
+        turns[n % BUFS][i][pair] = make_double2(c, s);
+        turns32[n % BUFS][i][pair] = make_float2((float)c, (float)s);
+      }
+  };
+  look_up(0);
+  form_angles(0);
   __syncthreads();
   uint32_t turn_no = 0;
   bool alive = true;
   for (uint32_t row0 = first_row; row0 < live; row0 += stride_rows, turn_no++) {
-    const int rows = (int)min((uint32_t)RT, live - row0);
-    if (warp < rows) {
-      const RowPlace pl = place_row<PB>(p.d, row0 + warp);
-      if ((tid & 31) == 0) place[warp] = pl;
-    }
-    __syncthreads();
-    for (int i = tid / HALF; i < rows; i += THREADS / HALF)
-      if (pair < p.angles) {
-        double s, c;
-        sincospi((double)place[i].pos * freq, &s, &c);
-        turn[i][pair] = make_double2(c, s);
-        turn32[i][pair] = make_float2((float)c, (float)s);
-      }
-    __syncthreads();
+    const int rows = rows_of(turn_no);
+    const auto& turn = turns[turn_no % BUFS];
+    const auto& turn32 = turns32[turn_no % BUFS];
+    const RowPlace* place = places + (turn_no % batch_turns) * RT;
     if constexpr (MODE == kStaged)
       alive = __all_sync(0xffffffffu, mbar_wait(&landed[turn_no & 1], (turn_no >> 1) & 1u, p.d.status));
     const uint8_t* const rows_at = MODE == kStaged ? stages + (turn_no & 1) * kStageBytes : qkv + (uint64_t)row0 * p.stride * ES;
@@ -325,7 +359,15 @@ __global__ void __launch_bounds__(threads_of<MODE>(), MODE == kFew ? 1 : 2) k_he
         }
       }
     }
-    // the turn's rows, angles and places have been used
+    // the next turn's angles, beside the others' heads; then this turn's rows, angles and
+    // places have been used
+    if (row0 + stride_rows >= live) break;
+    const bool new_batch = MODE == kFew || (turn_no + 1) % batch_turns == 0;
+    if (new_batch) {
+      __syncthreads();
+      look_up(turn_no + 1);
+    }
+    form_angles(turn_no + 1);
     if constexpr (MODE == kStaged) {
       if (!__syncthreads_and(alive)) break;
       if (tid == 0) bring(turn_no + 2);
@@ -418,7 +460,7 @@ int launch_prep(e4b_ctx* c, const PrepP& p, int bits, int x_f16, dim3 grid) {
 template <int HD>
 int launch_prep(e4b_ctx* c, PrepP& p, int bits, int x_f16) {
   // few rows: a row per CTA, and a CTA per pass over its heads (latency); the rest in
-  // turns of up to four rows, which share the barriers and the lookups
+  // turns of several rows, which share the barriers
   const int ns = threads_of<kFew>() / (HD / 8);
   const int passes = (p.QH + ns - 1) / ns + (2 * p.d.KVH + ns - 1) / ns;
   if ((int64_t)p.d.n_rows * passes <= 8 * c->sm_count)
@@ -427,7 +469,7 @@ int launch_prep(e4b_ctx* c, PrepP& p, int bits, int x_f16) {
   const int64_t row_bytes = (int64_t)(p.QH + p.d.KVH * (p.keqv ? 1 : 2)) * HD * es;
   const bool staged = p.nparts == 1 && row_bytes <= kStageBytes && reinterpret_cast<uintptr_t>(p.qkv) % 16 == 0 &&
                       p.stride * es % 16 == 0;
-  p.rows_per_turn = staged && kStageBytes / row_bytes < kTurnRows ? (int)(kStageBytes / row_bytes) : kTurnRows;
+  p.rows_per_turn = staged && kStageBytes / row_bytes < turn_rows(HD) ? (int)(kStageBytes / row_bytes) : turn_rows(HD);
   const int turns = (p.d.n_rows + p.rows_per_turn - 1) / p.rows_per_turn, resident = 2 * c->sm_count;
   const dim3 grid(turns < resident ? turns : resident);
   return staged ? launch_prep<HD, kStaged>(c, p, bits, x_f16, grid) : launch_prep<HD, kDirect>(c, p, bits, x_f16, grid);
