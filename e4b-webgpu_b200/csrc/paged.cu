@@ -13,9 +13,8 @@ struct PrepP {
   const float* kw;
   float* q_out;
   int QH, angles, norm, keqv, nparts;
-  int rows_per_turn;                 // rows of a CTA's turn
+  int rows_per_turn, rows_per_cta;
   int64_t stride;                    // elements between rows
-  uint64_t per_q, per_kv;            // ceil(2^32 / QH), ceil(2^32 / (2 KVH)): quotients of small numerators
   float eps;
   double log2_theta;
 };
@@ -179,12 +178,21 @@ E4B_DEV RowPlace place_one(const PagedDev& d, uint32_t row) {          // a thre
 // rounding of the exact value whatever the order of the sums, so the 4-bit codes do not
 // depend on it.  Bound by memory for many rows (per row of 16 q + 2 x 4 heads of 256:
 // 24.6 KB read, 16.4 KB of q and 2.3 KB of 4-bit cache written), by latency for few.
+// A head of a turn: where its elements are, and where it goes.
+struct Item {
+  uint32_t src;                      // bytes from the turn's first row (rows row_bytes apart: kStaged), or of its row
+  uint16_t row, head;                // row of the turn (kNoRow: none); query head, or KV head with kKey / kValue
+};
+enum : uint16_t { kNoRow = 0xffff, kKey = 0x4000, kValue = 0x8000, kHeadMask = 0x3fff };
+
 template <int HD, int BITS, bool XF16, int MODE>
 __global__ void __launch_bounds__(threads_of<MODE>(), MODE == kFew ? 1 : 2) k_headprep_paged(const PrepP p) {
   constexpr int LPH = HD / 8, HALF = HD / 2, PB = BITS == 16 ? 32 * HD : 9 * HD, ES = XF16 ? 2 : 4;
   constexpr int THREADS = threads_of<MODE>(), NS = THREADS / LPH, ROWS = MODE == kFew ? 1 : turn_rows(HD);
-  extern __shared__ __align__(128) uint8_t stages[];     // kStaged: 2 x kStageBytes
-  constexpr int BUFS = MODE == kFew ? 1 : 2, BATCH = MODE == kFew ? 1 : kBatch;
+  constexpr int BUFS = MODE == kFew ? 1 : 2, BATCH = MODE == kFew ? 1 : kBatch, GROUPS = 32 / LPH;
+  extern __shared__ __align__(128) uint8_t dyn[];        // kStaged: 2 x kStageBytes; then the items
+  uint8_t* const stages = dyn;
+  Item* const items = reinterpret_cast<Item*>(dyn + (MODE == kStaged ? 2 * kStageBytes : 0));
   __shared__ __align__(16) double2 turns[BUFS][ROWS][HALF];            // (cos, sin) of a turn's angles
   __shared__ __align__(16) float2 turns32[BUFS][ROWS][HALF];
   __shared__ double kw64[HD];
@@ -204,6 +212,23 @@ __global__ void __launch_bounds__(threads_of<MODE>(), MODE == kFew ? 1 : 2) k_he
     mbar_init(&landed[1], 1);
     fence_barrier_init();
   }
+  // the turn's items: its query heads (up to a whole warp's), then its key and value heads
+  const int nq = (RT * p.QH + GROUPS - 1) / GROUPS * GROUPS, total = nq + (RT * 2 * KVH + GROUPS - 1) / GROUPS * GROUPS;
+  for (int i = tid; i < total; i += THREADS) {
+    Item it{0u, kNoRow, 0};
+    if (i < RT * p.QH) {
+      it.row = (uint16_t)(i / p.QH);
+      it.head = (uint16_t)(i % p.QH);
+      it.src = (uint32_t)it.head * HD * ES;
+    } else if (i >= nq && i - nq < RT * 2 * KVH) {
+      const int h = (i - nq) % (2 * KVH), kvh = h < KVH ? h : h - KVH;
+      it.row = (uint16_t)((i - nq) / (2 * KVH));
+      it.head = (uint16_t)(kvh | (h < KVH ? kKey : kValue));
+      it.src = (uint32_t)(p.QH + (p.keqv ? kvh : h)) * HD * ES;
+    }
+    if (MODE == kStaged && it.row != kNoRow) it.src += it.row * row_bytes;
+    items[i] = it;
+  }
   float qw[8];
 #pragma unroll
   for (int j = 0; j < 8; j++) qw[j] = 1.f;
@@ -215,112 +240,123 @@ __global__ void __launch_bounds__(threads_of<MODE>(), MODE == kFew ? 1 : 2) k_he
     for (int i = tid; i < HD; i += THREADS) kw64[i] = (double)p.kw[i];
   }
   pdl_wait();
-  const uint32_t live = live_rows(p.d), first_row = blockIdx.x * RT, stride_rows = gridDim.x * RT;
-  const auto bring = [&](uint32_t turn_no) {             // thread 0: the rows of a turn into its stage
-    const uint64_t row = (uint64_t)first_row + (uint64_t)turn_no * stride_rows;
-    if (row >= live) return;
-    const int n = (int)min((uint64_t)RT, live - row);
+  // a CTA's rows are consecutive: they share sequences, pieces and (nearly) angles
+  const uint32_t live = live_rows(p.d);
+  const uint32_t first_row = blockIdx.x * p.rows_per_cta, end_row = min(live, first_row + p.rows_per_cta);
+  const auto bring = [&](uint32_t row, uint32_t turn_no) {             // thread 0: a turn's rows into their stage
+    if (row >= end_row) return;
+    const int n = (int)min((uint32_t)RT, end_row - row);
     uint64_t* bar = &landed[turn_no & 1];
     mbar_expect_tx(bar, n * row_bytes);
     for (int i = 0; i < n; i++)
-      bulk_g2s(stages + (turn_no & 1) * kStageBytes + i * row_bytes, qkv + (row + i) * (uint64_t)p.stride * ES, row_bytes, bar);
+      bulk_g2s(stages + (turn_no & 1) * kStageBytes + i * row_bytes, qkv + (uint64_t)(row + i) * p.stride * ES, row_bytes, bar);
   };
   if (MODE == kStaged && tid == 0) {
-    bring(0);
-    bring(1);
+    bring(first_row, 0);
+    bring(first_row + RT, 1);
   }
-  // rows of turn n, and the places of the batch that begins with it
-  const auto rows_of = [&](uint32_t n) -> int {
-    const uint64_t row = (uint64_t)first_row + (uint64_t)n * stride_rows;
-    return row >= live ? 0 : (int)min((uint64_t)RT, live - row);
-  };
-  const int batch_turns = BATCH / RT;
-  const auto look_up = [&](uint32_t n) {
+  const uint32_t batch_rows = MODE == kFew ? 1 : BATCH / RT * RT;
+  const auto look_up = [&](uint32_t row) {               // the places of the batch that begins with a row
     if constexpr (MODE == kFew) {
-      if (warp == 0 && rows_of(n)) {
-        const RowPlace pl = place_row<PB>(p.d, first_row + n * stride_rows);
+      if (warp == 0 && row < end_row) {
+        const RowPlace pl = place_row<PB>(p.d, row);
         if (tid == 0) places[0] = pl;
       }
-    } else if (tid < batch_turns * RT && tid % RT < rows_of(n + tid / RT)) {
-      places[tid] = place_one<PB>(p.d, first_row + (n + tid / RT) * stride_rows + tid % RT);
+    } else if (tid < batch_rows && row + tid < end_row) {
+      places[tid] = place_one<PB>(p.d, row + tid);
     }
     __syncthreads();
   };
-  const auto form_angles = [&](uint32_t n) {
-    const int base = (int)(n % batch_turns) * RT;
-    for (int i = tid / HALF; i < rows_of(n); i += THREADS / HALF)
-      if (pair < p.angles) {
-        double s, c;
-        sincospi((double)places[base + i].pos * freq, &s, &c);
-        turns[n % BUFS][i][pair] = make_double2(c, s);
-        turns32[n % BUFS][i][pair] = make_float2((float)c, (float)s);
+  // The angles of a turn: thread group g of HALF threads forms row g's.  A row RT
+  // positions behind the group's last one is a rotation by RT frequencies away.
+  const int group = tid / HALF;
+  double c = 1.0, s = 0.0, cr = 1.0, sr = 0.0;
+  uint64_t last = ~0ull;
+  if constexpr (MODE != kFew)
+    if (group < RT && pair < p.angles) sincospi((double)RT * freq, &sr, &cr);
+  const auto form_angles = [&](uint32_t row, int at, int buf, bool anew) {
+    for (int g = group; g < RT; g += THREADS / HALF)
+      if (row + g < end_row && pair < p.angles) {
+        const uint64_t pos = places[at + g].pos;
+        if (MODE != kFew && !anew && RT <= THREADS / HALF && pos == last + RT) {
+          const double t = c * cr - s * sr;
+          s = s * cr + c * sr;
+          c = t;
+        } else {
+          sincospi((double)pos * freq, &s, &c);
+        }
+        last = pos;
+        turns[buf][g][pair] = make_double2(c, s);
+        turns32[buf][g][pair] = make_float2((float)c, (float)s);
       }
   };
-  look_up(0);
-  form_angles(0);
+  look_up(first_row);
+  form_angles(first_row, 0, 0, true);
   __syncthreads();
-  uint32_t turn_no = 0;
+  uint32_t turn_no = 0, at_row = 0;                      // at_row: the turn's place in its batch
   bool alive = true;
-  for (uint32_t row0 = first_row; row0 < live; row0 += stride_rows, turn_no++) {
-    const int rows = rows_of(turn_no);
+  for (uint32_t row0 = first_row; row0 < end_row; row0 += RT, turn_no++) {
+    const int rows = (int)min((uint32_t)RT, end_row - row0);
     const auto& turn = turns[turn_no % BUFS];
     const auto& turn32 = turns32[turn_no % BUFS];
-    const RowPlace* place = places + (turn_no % batch_turns) * RT;
+    const RowPlace* place = places + at_row;
     if constexpr (MODE == kStaged)
       alive = __all_sync(0xffffffffu, mbar_wait(&landed[turn_no & 1], (turn_no >> 1) & 1u, p.d.status));
-    const uint8_t* const rows_at = MODE == kStaged ? stages + (turn_no & 1) * kStageBytes : qkv + (uint64_t)row0 * p.stride * ES;
-    const uint64_t rows_by = MODE == kStaged ? row_bytes : (uint64_t)p.stride * ES;
-    // Head i of the rows' query heads (then of their key and value heads) goes to lane
-    // group i % NS of pass i / NS; the passes are dealt to blockIdx.y.  Every lane of a
-    // warp makes the same turns (shuffles): a group without a head repeats the last one.
-    const int nq = alive ? rows * p.QH : 0, nkv = alive ? rows * 2 * KVH : 0, qpasses = (nq + NS - 1) / NS;
-#pragma unroll 2
-    for (int ps = blockIdx.y; ps < qpasses; ps += gridDim.y) {
-      const int at = ps * NS + sub, i = min(at, nq - 1), r = ROWS == 1 ? 0 : (int)((i * p.per_q) >> 32), h = i - r * p.QH;
-      Quad a = load_parts<XF16, MODE>(p, rows_at + r * rows_by, h * HD + 4 * l);
-      Quad b = load_parts<XF16, MODE>(p, rows_at + r * rows_by, h * HD + HALF + 4 * l);
-      float(&xa)[4] = a.x;
-      float(&xb)[4] = b.x;
-      if (p.norm) {
-        float s = 0.f;
-#pragma unroll
-        for (int j = 0; j < 4; j++) s = fmaf(xa[j], xa[j], fmaf(xb[j], xb[j], s));
-#pragma unroll
-        for (int o = 1; o < LPH; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        const float inv = rsqrt_fast(s * (1.f / HD) + p.eps);
-#pragma unroll
-        for (int j = 0; j < 4; j++) xa[j] *= inv * qw[j], xb[j] *= inv * qw[4 + j];
+    float* const q_rows = p.q_out + (size_t)row0 * p.QH * HD + 4 * l;
+    // every lane of a warp makes the same turns (shuffles): a group without a head works on row 0
+    for (int i = blockIdx.y * NS + sub; alive && i < total; i += gridDim.y * NS) {
+      const Item it = items[i];
+      const bool on = it.row < rows;
+      const int r = on ? it.row : 0;
+      Quad a, b;
+      if constexpr (MODE == kStaged) {
+        const uint8_t* src = stages + (turn_no & 1) * kStageBytes + it.src;
+        a = load_quad<XF16>(src, 4 * l);
+        b = load_quad<XF16>(src, HALF + 4 * l);
+      } else {
+        const uint8_t* src = qkv + (uint64_t)(row0 + r) * p.stride * ES + it.src;
+        a = load_parts<XF16, MODE>(p, src, 4 * l);
+        b = load_parts<XF16, MODE>(p, src, HALF + 4 * l);
       }
-      if (turned) {
-        const float4 c0 = *reinterpret_cast<const float4*>(&turn32[r][4 * l]);
-        const float4 c1 = *reinterpret_cast<const float4*>(&turn32[r][4 * l + 2]);
-        const float cs[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+      if (i < nq) {
+        float(&xa)[4] = a.x;
+        float(&xb)[4] = b.x;
+        if (p.norm) {
+          float sum = 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const float y = xa[j] * cs[2 * j] - xb[j] * cs[2 * j + 1], z = xa[j] * cs[2 * j + 1] + xb[j] * cs[2 * j];
-          if (j < turned) xa[j] = y, xb[j] = z;
+          for (int j = 0; j < 4; j++) sum = fmaf(xa[j], xa[j], fmaf(xb[j], xb[j], sum));
+#pragma unroll
+          for (int o = 1; o < LPH; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+          const float inv = rsqrt_fast(sum * (1.f / HD) + p.eps);
+#pragma unroll
+          for (int j = 0; j < 4; j++) xa[j] *= inv * qw[j], xb[j] *= inv * qw[4 + j];
         }
+        if (turned) {
+          const float4 c0 = *reinterpret_cast<const float4*>(&turn32[r][4 * l]);
+          const float4 c1 = *reinterpret_cast<const float4*>(&turn32[r][4 * l + 2]);
+          const float cs[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            const float y = xa[j] * cs[2 * j] - xb[j] * cs[2 * j + 1], z = xa[j] * cs[2 * j + 1] + xb[j] * cs[2 * j];
+            if (j < turned) xa[j] = y, xb[j] = z;
+          }
+        }
+        if (on) {
+          float* qo = q_rows + (uint32_t)(r * p.QH + it.head) * HD;
+          *reinterpret_cast<float4*>(qo) = make_float4(xa[0], xa[1], xa[2], xa[3]);
+          *reinterpret_cast<float4*>(qo + HALF) = make_float4(xb[0], xb[1], xb[2], xb[3]);
+        }
+        continue;
       }
-      if (at < nq) {
-        float* qo = p.q_out + ((size_t)row0 * p.QH + at) * HD + 4 * l;
-        *reinterpret_cast<float4*>(qo) = make_float4(xa[0], xa[1], xa[2], xa[3]);
-        *reinterpret_cast<float4*>(qo + HALF) = make_float4(xb[0], xb[1], xb[2], xb[3]);
-      }
-    }
-    const int first = (int)((blockIdx.y + gridDim.y - (uint32_t)qpasses % gridDim.y) % gridDim.y);
-    for (int i0 = first * NS; i0 < nkv; i0 += gridDim.y * NS) {
-      const int i = min(i0 + sub, nkv - 1), r = ROWS == 1 ? 0 : (int)((i * p.per_kv) >> 32), h = i - r * 2 * KVH;
-      const bool is_v = h >= KVH;
-      const int kvh = is_v ? h - KVH : h, at = (p.QH + (p.keqv ? kvh : h)) * HD + 4 * l;
-      const Quad a = load_parts<XF16, MODE>(p, rows_at + r * rows_by, at), b = load_parts<XF16, MODE>(p, rows_at + r * rows_by, at + HALF);
+      const bool is_v = (it.head & kValue) != 0;
       double inv = 1.0;
       if (p.norm) {
-        double s = 0.0;
+        double sum = 0.0;
 #pragma unroll
-        for (int j = 0; j < 4; j++) s = fma((double)a.x[j], (double)a.x[j], fma((double)b.x[j], (double)b.x[j], s));
+        for (int j = 0; j < 4; j++) sum = fma((double)a.x[j], (double)a.x[j], fma((double)b.x[j], (double)b.x[j], sum));
 #pragma unroll
-        for (int o = 1; o < LPH; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        inv = rsqrt64(s * (1.0 / HD) + (double)p.eps);
+        for (int o = 1; o < LPH; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        inv = rsqrt64(sum * (1.0 / HD) + (double)p.eps);
       }
       float fa[4], fb[4];
       if (is_v || (!p.norm && !turned)) {
@@ -344,40 +380,42 @@ __global__ void __launch_bounds__(threads_of<MODE>(), MODE == kFew ? 1 : 2) k_he
       const uint32_t w[2][2] = {{pack2(fa[0], fa[1]), pack2(fa[2], fa[3])}, {pack2(fb[0], fb[1]), pack2(fb[2], fb[3])}};
       uint32_t codes[2] = {0u, 0u}, d16[2] = {0u, 0u};
       if constexpr (BITS == 4) quantise(w, lane8, codes, d16);
-      if (i0 + sub >= nkv || !place[r].ok) continue;
-      const int s = place[r].slot;
-      uint8_t* piece = (is_v ? p.d.v : p.d.k) + place[r].offset + (uint64_t)head_bytes * kvh;
+      if (!on || !place[r].ok) continue;
+      const int slot = place[r].slot;
+      uint8_t* piece = (is_v ? p.d.v : p.d.k) + place[r].offset + (uint64_t)head_bytes * (it.head & kHeadMask);
 #pragma unroll
       for (int k = 0; k < 2; k++) {
         const int q = l + k * LPH;
         if constexpr (BITS == 16) {
-          *reinterpret_cast<uint2*>(piece + (is_v ? v16_quad(s, q) : k16_quad(s, q))) = make_uint2(w[k][0], w[k][1]);
+          *reinterpret_cast<uint2*>(piece + (is_v ? v16_quad(slot, q) : k16_quad(slot, q))) = make_uint2(w[k][0], w[k][1]);
         } else {
-          *reinterpret_cast<uint16_t*>(piece + (is_v ? v4_quad(s, q, HD) : k4_quad(s, q, HD))) = (uint16_t)codes[k];
+          *reinterpret_cast<uint16_t*>(piece + (is_v ? v4_quad(slot, q, HD) : k4_quad(slot, q, HD))) = (uint16_t)codes[k];
           if (lane8 == 0)
-            *reinterpret_cast<uint16_t*>(piece + (is_v ? v4_scale(s, q / 8, HD) : k4_scale(s, q / 8, HD))) = (uint16_t)d16[k];
+            *reinterpret_cast<uint16_t*>(piece + (is_v ? v4_scale(slot, q / 8, HD) : k4_scale(slot, q / 8, HD))) = (uint16_t)d16[k];
         }
       }
     }
+    if (row0 + RT >= end_row) break;
     // the next turn's angles, beside the others' heads; then this turn's rows, angles and
     // places have been used
-    if (row0 + stride_rows >= live) break;
-    const bool new_batch = MODE == kFew || (turn_no + 1) % batch_turns == 0;
-    if (new_batch) {
+    at_row += RT;
+    const bool anew = at_row == batch_rows;
+    if (anew) {
+      at_row = 0;
       __syncthreads();
-      look_up(turn_no + 1);
+      look_up(row0 + RT);
     }
-    form_angles(turn_no + 1);
+    form_angles(row0 + RT, at_row, (turn_no + 1) % BUFS, anew);
     if constexpr (MODE == kStaged) {
       if (!__syncthreads_and(alive)) break;
-      if (tid == 0) bring(turn_no + 2);
+      if (tid == 0) bring(row0 + 2 * RT, turn_no);
     } else {
       __syncthreads();
     }
   }
   if (MODE == kStaged && !alive)     // after a time-out: copies still in flight land (bounded)
     for (uint32_t i = 0; i < 2; i++)
-      if ((uint64_t)first_row + (uint64_t)(turn_no + i) * stride_rows < live)
+      if (first_row + (turn_no + i) * RT < end_row)
         mbar_wait(&landed[(turn_no + i) & 1], ((turn_no + i) >> 1) & 1u, p.d.status);
 }
 
@@ -452,8 +490,9 @@ template <int HD, int MODE>
 int launch_prep(e4b_ctx* c, const PrepP& p, int bits, int x_f16, dim3 grid) {
   auto kern = bits == 16 ? (x_f16 ? k_headprep_paged<HD, 16, true, MODE> : k_headprep_paged<HD, 16, false, MODE>)
                          : (x_f16 ? k_headprep_paged<HD, 4, true, MODE> : k_headprep_paged<HD, 4, false, MODE>);
-  const size_t smem = MODE == kStaged ? 2 * kStageBytes : 0;
-  if (smem) E4B_CUDA(c, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  const size_t items = (size_t)p.rows_per_turn * (p.QH + 2 * p.d.KVH) + 8;    // with the warps' padding
+  const size_t smem = (MODE == kStaged ? 2 * kStageBytes : 0) + items * sizeof(Item);
+  if (smem > 32 * 1024) E4B_CUDA(c, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   return e4b_launch(c, "headprep_paged", kern, grid, dim3(threads_of<MODE>()), smem, p);
 }
 
@@ -469,9 +508,12 @@ int launch_prep(e4b_ctx* c, PrepP& p, int bits, int x_f16) {
   const int64_t row_bytes = (int64_t)(p.QH + p.d.KVH * (p.keqv ? 1 : 2)) * HD * es;
   const bool staged = p.nparts == 1 && row_bytes <= kStageBytes && reinterpret_cast<uintptr_t>(p.qkv) % 16 == 0 &&
                       p.stride * es % 16 == 0;
-  p.rows_per_turn = staged && kStageBytes / row_bytes < turn_rows(HD) ? (int)(kStageBytes / row_bytes) : turn_rows(HD);
+  const int64_t fit = staged ? kStageBytes / row_bytes : 2048 / (p.QH + 2 * p.d.KVH);   // (direct: of the item table)
+  p.rows_per_turn = fit < 1 ? 1 : (fit < turn_rows(HD) ? (int)fit : turn_rows(HD));
   const int turns = (p.d.n_rows + p.rows_per_turn - 1) / p.rows_per_turn, resident = 2 * c->sm_count;
-  const dim3 grid(turns < resident ? turns : resident);
+  const int per_cta = (turns + resident - 1) / resident;
+  p.rows_per_cta = per_cta * p.rows_per_turn;
+  const dim3 grid((turns + per_cta - 1) / per_cta);
   return staged ? launch_prep<HD, kStaged>(c, p, bits, x_f16, grid) : launch_prep<HD, kDirect>(c, p, bits, x_f16, grid);
 }
 }  // namespace
@@ -505,10 +547,8 @@ E4B_API int e4b_headprep_paged(e4b_ctx* c, const e4b_paged_kv* kv, const void* q
   p.norm = norm ? 1 : 0;
   p.keqv = keqv ? 1 : 0;
   p.nparts = nparts;
-  p.rows_per_turn = 1;
+  p.rows_per_turn = p.rows_per_cta = 1;
   p.stride = row_stride ? row_stride : (int64_t)(QH + kv->kv_heads * (keqv ? 1 : 2)) * HD;
-  p.per_q = QH > 0 ? (((uint64_t)1 << 32) + QH - 1) / QH : 0;
-  p.per_kv = (((uint64_t)1 << 32) + 2 * kv->kv_heads - 1) / (2 * kv->kv_heads);
   p.eps = eps;
   p.log2_theta = log2((double)theta);
   return HD == 256 ? launch_prep<256>(c, p, kv->bits, x_f16)
