@@ -56,49 +56,56 @@ struct AttnP {
   float scale;
 };
 
+// kNarrow, kWide: a row per unit of up to 4 heads, one n-tile whose 8 MMA columns are
+// the heads' hi parts and lo parts.  kRows: NT tiles a warp whose 8 columns are 8 (row,
+// head) pairs, hi and lo in turn: the decoded keys and values, the softmax and the
+// scaled p are then shared by twice the columns, for prompts' and speculated rows.
+enum { kNarrow, kWide, kRows };
 constexpr int kConsumerRegs = 224, kProducerRegs = 56;
 
-template <int BITS, int HD, int NT, bool WIDE>
+template <int BITS, int HD, int MODE>
 struct Shape {
   static constexpr int NB = HD / 32;
   static constexpr int PB = BITS == 16 ? 32 * HD : 9 * HD;
   static constexpr int STAGE = 2 * PB;
-  // consumer warps: with one n-tile a warp needs 168 registers, so 12 warps fit an SM:
-  // one CTA of 11 + 1 (WIDE), or two of 5 + 1, where one's set-up and merges pass
-  // beside the other's pieces; with two tiles a warp needs more, which the producer's
-  // warpgroup gives up (setmaxnreg): 8 * 32 * 224 + 4 * 32 * 56 = 384 * 168, what the
-  // block was launched with
-  static constexpr int PER_SM = NT == 1 && !WIDE ? 2 : 1, MAX_CTAS = PER_SM * kMaxCtas / 2;
-  static constexpr int W = NT == 2 ? 8 : (!WIDE ? 5 : (BITS == 16 && HD == 256 ? 10 : 11));
+  static constexpr int NT = MODE == kRows && !(BITS == 16 && HD == 256) ? 2 : 1;
+  static constexpr int LC = NT * (MODE == kRows ? 8 : 4);               // columns of a warp
+  // consumer warps: a one-row warp needs 168 registers, so 12 warps fit an SM: one CTA
+  // of 11 + 1 (kWide), or two of 5 + 1, where one's set-up and merges pass beside the
+  // other's pieces; a kRows warp needs more, which the producer's warpgroup gives up
+  // (setmaxnreg): 8 * 32 * 224 + 4 * 32 * 56 = 384 * 168, what the block was launched with
+  static constexpr int PER_SM = MODE == kNarrow ? 2 : 1, MAX_CTAS = PER_SM * kMaxCtas / 2;
+  static constexpr int W = MODE == kRows ? 8 : (MODE == kNarrow ? 5 : (BITS == 16 && HD == 256 ? 10 : 11));
   // ring depth: a multiple of W, so a stage's uses within a unit belong to the same
   // warps (a warp then never waits for a phase before the stage's last one is done)
   static constexpr int S = W * (BITS == 16 ? (HD == 256 ? 1 : (HD == 128 ? 2 : 4)) :
-                                NT == 2 ? (HD == 64 ? 8 : 4) : (HD == 256 ? 3 : (HD == 128 ? 5 : 8)));
+                                MODE == kRows ? (HD == 256 ? 2 : (HD == 128 ? 4 : 8)) : (HD == 256 ? 3 : (HD == 128 ? 5 : 8)));
   // what a unit costs beside its pieces (q, the merge, the outputs), in pieces
-  static constexpr int U = BITS == 16 ? (HD == 256 ? 6 : (HD == 128 ? 8 : 12)) : (HD == 256 ? 12 : 16);
+  static constexpr int U = MODE == kRows ? 48 : (BITS == 16 ? (HD == 256 ? 6 : (HD == 128 ? 8 : 12)) : (HD == 256 ? 12 : 16));
   static constexpr int LN = S <= 32 ? S : (W == 11 ? 11 : (W == 5 ? (S == 40 ? 20 : 25) : 32));   // producer lanes; S is a multiple
-  static constexpr int THREADS = NT == 1 ? 32 * (W + 1) : 384, CT = 32 * W;
-  static constexpr int COLS = NT == 1 ? 4 : 64;                         // columns (row, head) of a unit at most
+  static constexpr int THREADS = MODE == kRows ? 384 : 32 * (W + 1), CT = 32 * W;
+  static constexpr int COLS = MODE == kRows ? W * LC : LC;              // columns (row, head) of a unit at most
   static constexpr size_t PART = (size_t)COLS * (HD + 2);               // floats of a partial
-  static constexpr int TILES = W * NT;                                  // n-tiles of a unit at most
+  static constexpr int TILES = W * NT, QPARTS = MODE == kRows ? 2 : 1;  // n-tiles of a unit at most; fragments of a tile
   static constexpr size_t RING = (size_t)S * STAGE;
-  // q fragments [TILES][NB][32] while a unit's pieces pass, then the warps' O [W][NT*4][HD]
-  static constexpr size_t MERGE = (size_t)W * NT * 4 * HD * 4;
+  // q fragments [TILES][NB][QPARTS][32] while a unit's pieces pass, then the warps' O [W][LC][HD]
+  static constexpr size_t MERGE = (size_t)W * LC * HD * 4;
   static constexpr size_t SMEM = RING + MERGE;
-  static_assert((size_t)TILES * NB * 32 * 16 <= MERGE, "q fragments fit the merge buffer");
+  static_assert((size_t)TILES * NB * QPARTS * 32 * 16 <= MERGE, "q fragments fit the merge buffer");
 };
 
-// Rows and heads of a unit in n-tiles: a row of up to 4 heads is one tile, of up
-// to 8 heads two; a warp has NT tiles.
-template <int W, int NT>
+// Rows and heads of a unit in n-tiles.
+template <int W, int NT, int MODE>
 struct Rows {
-  int per_warp;                      // rows of a warp
-  E4B_DEV explicit Rows(int G) : per_warp(G > 4 ? NT / 2 : NT) {}
-  E4B_DEV uint32_t per_unit() const { return per_warp * W; }
+  int slots;                         // columns of a row in a tile: its heads, up to a power of two (one row: 4)
+  E4B_DEV explicit Rows(int G) : slots(MODE != kRows ? 4 : (G > 4 ? 8 : (G > 2 ? 4 : G))) {}
+  E4B_DEV int per_tile() const { return MODE == kRows ? 8 / slots : 1; }
+  E4B_DEV uint32_t per_warp() const { return NT * per_tile(); }
+  E4B_DEV uint32_t per_unit() const { return per_warp() * W; }
   // warps that share a piece, for a unit of r rows: a power of two
   E4B_DEV uint32_t sharing(uint32_t r) const {
     uint32_t wc = 1;
-    while (wc * per_warp < r) wc *= 2;
+    while (wc * per_warp() < r) wc *= 2;
     return wc;
   }
 };
@@ -110,9 +117,9 @@ struct SeqWork {
   uint32_t full, tail_wc;            // units of W sharing warps, sharing warps of the last unit (0: none)
   uint64_t cost;                     // sum over units and KV heads of U + pieces * sharing warps
 };
-template <int W, int NT, int U>
+template <int W, int NT, int U, int MODE>
 E4B_DEV SeqWork seq_work(const AttnP& p, int s) {
-  const Rows<W, NT> rows(p.G);
+  const Rows<W, NT, MODE> rows(p.G);
   SeqWork w;
   uint32_t r0 = (uint32_t)s, r1 = r0 + 1;
   if (p.d.rows) r0 = p.d.rows[s], r1 = min(p.d.rows[s + 1], (uint32_t)p.d.n_rows);
@@ -140,7 +147,7 @@ E4B_DEV uint64_t udiv(uint64_t a, uint64_t b) {
 }
 
 // Walks a CTA's run [g, end) of the work, unit by unit.
-template <int W, int NT, int U>
+template <int W, int NT, int U, int MODE>
 struct Walk {
   uint64_t g, end, base;             // base: where the current sequence's work begins
   int s;
@@ -157,13 +164,13 @@ struct Walk {
         g = end;
         return false;
       }
-      w = seq_work<W, NT, U>(p, s);
+      w = seq_work<W, NT, U, MODE>(p, s);
     }
-    const Rows<W, NT> rows(p.G);
+    const Rows<W, NT, MODE> rows(p.G);
     const uint32_t KVH = p.d.KVH, np = w.range.count;
     const uint64_t off = g - base, full_cost = ((uint64_t)np * W + U) * w.full * KVH;
     uint32_t group, unit;
-    if (NT > 1 && off < full_cost) {
+    if (MODE == kRows && off < full_cost) {
       wc = W;
       unit = (uint32_t)udiv(off, np * W + U);
       unit0 = base + (uint64_t)unit * (np * W + U);
@@ -267,23 +274,24 @@ __device__ __noinline__ bool wait_slow(uint64_t* b, uint32_t parity, uint32_t* s
   return mbar_wait(b, parity, status);
 }
 
-template <int BITS, int HD, int NT, bool WIDE>
-__global__ void __launch_bounds__(Shape<BITS, HD, NT, WIDE>::THREADS, Shape<BITS, HD, NT, WIDE>::PER_SM) k_attn_paged(const AttnP p) {
-  using Sh = Shape<BITS, HD, NT, WIDE>;
-  constexpr int NB = Sh::NB, PB = Sh::PB, W = Sh::W, S = Sh::S, LN = Sh::LN, CT = Sh::CT, LC = NT * 4;
+template <int BITS, int HD, int MODE>
+__global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD, MODE>::PER_SM) k_attn_paged(const AttnP p) {
+  using Sh = Shape<BITS, HD, MODE>;
+  constexpr int NB = Sh::NB, PB = Sh::PB, W = Sh::W, S = Sh::S, LN = Sh::LN, CT = Sh::CT, NT = Sh::NT, LC = Sh::LC;
+  constexpr int TC = LC / NT, QP = Sh::QPARTS;           // columns of a tile
   static_assert(S % W == 0 && S % LN == 0 && LN <= 32 && S <= Sh::THREADS, "ring");
   constexpr int OT = HD / 16;        // m16 tiles of O
   constexpr int U = Sh::U;
-  using Unit = Walk<W, NT, U>;
+  using Unit = Walk<W, NT, U, MODE>;
   extern __shared__ __align__(128) uint8_t smem[];
   uint8_t* ring = smem;
   float* merge = reinterpret_cast<float*>(smem + Sh::RING);            // [W][LC][HD]
-  uint4* qfrag = reinterpret_cast<uint4*>(smem + Sh::RING);            // [TILES][NB][32]
+  uint4* qfrag = reinterpret_cast<uint4*>(smem + Sh::RING);            // [TILES][NB][QP][32]
   __shared__ uint64_t landed[S], freed[S];
   __shared__ int usable[S];
   __shared__ uint64_t warp_sum_[Sh::THREADS / 32];
   __shared__ uint2 qzero[BITS == 4 ? Sh::TILES * 32 : 1];               // B of the -8 term: -8 sum q per block, hi and lo
-  __shared__ float qfac[Sh::TILES * 4];
+  __shared__ float qfac[Sh::TILES * TC];
   __shared__ float ml[W * LC * 2];
   __shared__ int last_one, more_units;
   __shared__ Unit start, unit;
@@ -304,7 +312,7 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT, WIDE>::THREADS, Shape<BITS
   SeqWork own;                       // of the thread's first sequence
   const int per = (p.d.nseq + Sh::THREADS - 1) / Sh::THREADS;
   for (int s = tid * per; s < min(p.d.nseq, (tid + 1) * per); s++) {
-    const SeqWork w = seq_work<W, NT, U>(p, s);
+    const SeqWork w = seq_work<W, NT, U, MODE>(p, s);
     if (s == tid * per) own = w;
     mine += w.cost;
   }
@@ -363,7 +371,7 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT, WIDE>::THREADS, Shape<BITS
 
   if (warp >= W) {
     // ---- producer: lane i brings the CTA's pieces i, i + LN, .., piece j into stage j % S
-    if constexpr (NT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProducerRegs));
+    if constexpr (MODE == kRows) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProducerRegs));
     if (warp > W || lane >= LN) return;
     constexpr uint32_t kLanes = LN == 32 ? 0xffffffffu : (1u << (LN & 31)) - 1u;
     uint32_t j = lane, seg0 = 0, seg1 = 0, page = 0, piece = 0, in_page = 0;
@@ -423,7 +431,7 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT, WIDE>::THREADS, Shape<BITS
     return;
   }
 
-  if constexpr (NT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kConsumerRegs));
+  if constexpr (MODE == kRows) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kConsumerRegs));
   const auto consumers = []() { asm volatile("bar.sync 1, %0;" ::"n"(CT) : "memory"); };
   uint32_t j0 = 0;                   // the CTA's pieces before the unit's
   bool alive = true;                 // no wait has run out
@@ -449,9 +457,11 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT, WIDE>::THREADS, Shape<BITS
     const uint32_t WC = unit.wc, WS = W / WC;
     const int wc = warp % WC, ws = warp / WC;
     const uint32_t row0 = (p.d.rows ? p.d.rows[unit.s] : (uint32_t)unit.s) + (unit.pmin - unit.w.p0);
-    // column c of the unit: tile c / 4 -> row of the unit, head
-    const auto col_row = [&](int c) { return p.G > 4 ? c >> 3 : c >> 2; };
-    const auto col_head = [&](int c) { return p.G > 4 ? c & 7 : c & 3; };
+    const Rows<W, NT, MODE> rows(p.G);
+    const int slots = rows.slots, per_tile = rows.per_tile();
+    // column c of the unit -> row of the unit, head
+    const auto col_row = [&](int c) { return c / TC * per_tile + c % TC / slots; };
+    const auto col_head = [&](int c) { return c % TC % slots; };
     const auto col_live = [&](int c) { return col_head(c) < p.G && (uint32_t)col_row(c) < unit.nrows; };
     const int cols = WC * LC;
 
@@ -459,8 +469,9 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT, WIDE>::THREADS, Shape<BITS
     {
       constexpr int LPC = HD / 8;
       const int sub = tid / LPC, l = tid % LPC, blk = l >> 2, tt = l & 3;
+#pragma unroll 4
       for (int c0 = 0; c0 < cols; c0 += CT / LPC) {
-        const int c = c0 + sub, tile = c >> 2, cc = c & 3;
+        const int c = c0 + sub, tile = c / TC, cc = c % TC;
         float x[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) x[i] = 0.f;
@@ -500,8 +511,10 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT, WIDE>::THREADS, Shape<BITS
           fl = make_uint4(pack2(lo[0], lo[1]), pack2(lo[2], lo[3]), pack2(lo[4], lo[5]), pack2(lo[6], lo[7]));
         }
         if (c < cols) {
-          qfrag[(tile * NB + blk) * 32 + cc * 4 + tt] = fh;
-          qfrag[(tile * NB + blk) * 32 + (cc + 4) * 4 + tt] = fl;
+          // the lo part: the tile's second fragment, or its columns 4-7
+          uint4* at = qfrag + ((size_t)(tile * NB + blk) * QP) * 32 + cc * 4 + tt;
+          at[0] = fh;
+          at[MODE == kRows ? 32 : 16] = fl;
           if constexpr (BITS == 4) {
             // B[k][col] of -8 sum q / 2^8: k = block (hi part), 8 + block (lo part); the rest stays zero
             if (tt == 0) {
@@ -519,24 +532,29 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT, WIDE>::THREADS, Shape<BITS
     consumers();
     float top[NT][2], lsum[NT][2], fac[NT][2], lift = kLift, slack = kSlack;  // reference score; sum of p; score factor
     bool live[NT];
-    uint32_t pos[NT];
+    uint32_t pos0[NT], pos1[NT], pos[NT][2], posg[NT];   // of the tile's first and last row, the lane's score columns, its p column
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
       const int tile = wc * NT + nt;
-      pos[nt] = unit.pmin + col_row(tile * 4);
-      live[nt] = (uint32_t)col_row(tile * 4) < unit.nrows && col_head(tile * 4) < p.G;
+      const auto position = [&](int row) { return min(unit.pmin + row, unit.pmax); };
+      live[nt] = (uint32_t)(tile * per_tile) < unit.nrows;
+      pos0[nt] = position(tile * per_tile);
+      pos1[nt] = position(tile * per_tile + per_tile - 1);
+      posg[nt] = position(col_row(tile * TC + g % TC));
 #pragma unroll
       for (int i = 0; i < 2; i++) {
+        const int c = tile * TC + (MODE == kRows ? 2 * t : 2 * (t & 1)) + i;
+        pos[nt][i] = position(col_row(c));
         top[nt][i] = -INFINITY;
         lsum[nt][i] = 0.f;
-        fac[nt][i] = qfac[tile * 4 + 2 * (t & 1) + i];
+        fac[nt][i] = qfac[c];
       }
 #pragma unroll
       for (int i = 0; i < OT; i++)
 #pragma unroll
         for (int k = 0; k < 4; k++) O[nt][i][k] = 0.f;
     }
-    const uint4* qf = qfrag + (size_t)wc * NT * NB * 32 + lane;
+    const uint4* qf = qfrag + (size_t)wc * NT * NB * QP * 32 + lane;
 
     const PieceSpan span = unit.span;
     const uint32_t turn = j0 % WS;   // group (j % WS) takes the CTA's piece j
@@ -581,10 +599,15 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT, WIDE>::THREADS, Shape<BITS
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
               if (NT > 1 && !live[nt]) continue;
-              const uint4 qb = qf[(nt * NB + b) * 32];
+              const uint4 qb = qf[(nt * NB + b) * QP * 32];
               float acc[4];
               mma16816_zero(acc, wa[q] & kLowCodes, wb[q] & kLowCodes, sa & kLowCodes, sb & kLowCodes, qb.x, qb.y);
               mma16816(acc, wa[q] & kHighCodes, wb[q] & kHighCodes, sa & kHighCodes, sb & kHighCodes, qb.z, qb.w);
+              if constexpr (MODE == kRows) {
+                const uint4 ql = qf[((nt * NB + b) * QP + 1) * 32];
+                mma16816(acc, wa[q] & kLowCodes, wb[q] & kLowCodes, sa & kLowCodes, sb & kLowCodes, ql.x, ql.y);
+                mma16816(acc, wa[q] & kHighCodes, wb[q] & kHighCodes, sa & kHighCodes, sb & kHighCodes, ql.z, ql.w);
+              }
               s[nt][0] = fmaf(d0, acc[0], s[nt][0]);
               s[nt][1] = fmaf(d0, acc[1], s[nt][1]);
               s[nt][2] = fmaf(d1, acc[2], s[nt][2]);
@@ -607,10 +630,15 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT, WIDE>::THREADS, Shape<BITS
 #pragma unroll
           for (int nt = 0; nt < NT; nt++) {
             if (NT > 1 && !live[nt]) continue;
-            const uint4 qb = qf[(nt * NB + b) * 32];
+            const uint4 qb = qf[(nt * NB + b) * QP * 32];
             float acc[4];
             mma16816_zero(acc, wa.x, wb.x, wa.y, wb.y, qb.x, qb.y);
             mma16816(acc, wa.z, wb.z, wa.w, wb.w, qb.z, qb.w);
+            if constexpr (MODE == kRows) {
+              const uint4 ql = qf[((nt * NB + b) * QP + 1) * 32];
+              mma16816(acc, wa.x, wb.x, wa.y, wb.y, ql.x, ql.y);
+              mma16816(acc, wa.z, wb.z, wa.w, wb.w, ql.z, ql.w);
+            }
 #pragma unroll
             for (int k = 0; k < 4; k++) s[nt][k] += acc[k];
           }
@@ -643,26 +671,25 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT, WIDE>::THREADS, Shape<BITS
       bool full[NT];
 #pragma unroll
       for (int nt = 0; nt < NT; nt++) {
-        full[nt] = here && t0 + kPieceSlots - 1 <= pos[nt] &&
-                   (p.window == 0 || pos[nt] - t0 < p.window || t0 + kPieceSlots <= p.sinks);
+        full[nt] = here && t0 + kPieceSlots - 1 <= pos0[nt] &&
+                   (p.window == 0 || pos1[nt] - t0 < p.window || t0 + kPieceSlots <= p.sinks);
         if (NT > 1 && !live[nt]) continue;
         float v[4];
+        bool see[4] = {true, true, true, true};
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-          s[nt][k] += __shfl_xor_sync(0xffffffffu, s[nt][k], 2);     // hi + lo columns
+          if constexpr (MODE != kRows) s[nt][k] += __shfl_xor_sync(0xffffffffu, s[nt][k], 2);     // hi + lo columns
           v[k] = s[nt][k] * fac[nt][k & 1];
         }
-        bool va = true, vb = true;
         if (!full[nt]) {
-          va = here && slot_visible(t0 + g, pos[nt], p.window, p.sinks);
-          vb = here && slot_visible(t0 + g + 8, pos[nt], p.window, p.sinks);
-          if (!va) v[0] = v[1] = -INFINITY;
-          if (!vb) v[2] = v[3] = -INFINITY;
           keep[nt][0] = keep[nt][1] = 0;
 #pragma unroll
-          for (int k = 0; k < 4; k++)
-            if (here && slot_visible(t0 + 2 * t + (k & 1) + 8 * (k >> 1), pos[nt], p.window, p.sinks))
+          for (int k = 0; k < 4; k++) {
+            see[k] = here && slot_visible(t0 + g + 8 * (k >> 1), pos[nt][k & 1], p.window, p.sinks);
+            if (!see[k]) v[k] = -INFINITY;
+            if (here && slot_visible(t0 + 2 * t + (k & 1) + 8 * (k >> 1), posg[nt], p.window, p.sinks))
               keep[nt][k >> 1] |= 0xffffu << (16 * (k & 1));
+          }
         }
         const bool grow = fmaxf(v[0], v[2]) > top[nt][0] + slack || fmaxf(v[1], v[3]) > top[nt][1] + slack;
         if (__any_sync(0xffffffffu, grow)) {
@@ -687,8 +714,9 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT, WIDE>::THREADS, Shape<BITS
 #pragma unroll
         for (int k = 0; k < 4; k++) e[k] = ex2(v[k] - ref[k & 1]);
         if (!full[nt]) {
-          if (!va) e[0] = e[1] = 0.f;
-          if (!vb) e[2] = e[3] = 0.f;
+#pragma unroll
+          for (int k = 0; k < 4; k++)
+            if (!see[k]) e[k] = 0.f;
         }
         lsum[nt][0] += e[0] + e[2];
         lsum[nt][1] += e[1] + e[3];
@@ -697,7 +725,10 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT, WIDE>::THREADS, Shape<BITS
           const uint32_t h = pack2(e[2 * k], e[2 * k + 1]);
           const float2 hf = __half22float2(*reinterpret_cast<const __half2*>(&h));
           const uint32_t l = pack2(e[2 * k] - hf.x, e[2 * k + 1] - hf.y);
-          if constexpr (BITS == 4) {
+          if constexpr (MODE == kRows) {
+            ph[nt][k] = transpose8x8(h);
+            pl[nt][k] = transpose8x8(l);
+          } else if constexpr (BITS == 4) {
             // columns 0-3: (0, hi), columns 4-7: (hi, lo); see the product with the scales
             ph[nt][k] = transpose8x8(t < 2 ? 0u : h);
             pl[nt][k] = transpose8x8(t < 2 ? h : l);
@@ -721,6 +752,14 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT, WIDE>::THREADS, Shape<BITS
         else masked = true;
         seen[0] |= keep[nt][0], seen[1] |= keep[nt][1];
       }
+      if (MODE == kRows && masked) {                     // over the columns' rows
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+          seen[k] |= __shfl_xor_sync(0xffffffffu, seen[k], 4);
+          seen[k] |= __shfl_xor_sync(0xffffffffu, seen[k], 8);
+          seen[k] |= __shfl_xor_sync(0xffffffffu, seen[k], 16);
+        }
+      }
       uint32_t dv[BITS == 4 ? NB : 1][2];
       if constexpr (BITS == 4) {
 #pragma unroll
@@ -737,7 +776,7 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT, WIDE>::THREADS, Shape<BITS
               dv[b][k] &= seen[k];
               odd |= !finite2(dv[b][k]);
             }
-          if (NT > 1 && __any_sync(0xffffffffu, odd)) {
+          if (MODE == kRows && __any_sync(0xffffffffu, odd)) {
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) strict[nt] = true;
           }
@@ -759,12 +798,18 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT, WIDE>::THREADS, Shape<BITS
 #pragma unroll
           for (int nt = 0; nt < NT; nt++) {
             if (NT > 1 && !live[nt]) continue;
-            uint32_t bb[2];
+            uint32_t bb[2], bh[2];
 #pragma unroll
             for (int k = 0; k < 2; k++) {
-              // hi columns: f16(hi d); lo columns: lo d + (hi d - f16(hi d))
+              // hi: f16(hi d); lo: lo d + (hi d - f16(hi d)).  With (0, hi) for (hi, lo) the
+              // second is f16(hi d): the hi columns where the tile has both
               const uint32_t d = strict[nt] ? dv[b][k] & keep[nt][k] : dv[b][k];
-              bb[k] = hfma2(pl[nt][k], d, hfms2(ph[nt][k], d, hmul2(ph[nt][k], d)));
+              bh[k] = hmul2(ph[nt][k], d);
+              bb[k] = hfma2(pl[nt][k], d, hfms2(ph[nt][k], d, bh[k]));
+            }
+            if constexpr (MODE == kRows) {
+              mma16816(O[nt][2 * b], al[0], al[1], al[2], al[3], bh[0], bh[1]);
+              mma16816(O[nt][2 * b + 1], ah[0], ah[1], ah[2], ah[3], bh[0], bh[1]);
             }
             mma16816(O[nt][2 * b], al[0], al[1], al[2], al[3], bb[0], bb[1]);
             mma16816(O[nt][2 * b + 1], ah[0], ah[1], ah[2], ah[3], bb[0], bb[1]);
@@ -784,16 +829,26 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT, WIDE>::THREADS, Shape<BITS
             if (masked) {
 #pragma unroll
               for (int i2 = 0; i2 < 4; i2++) a[i2] &= seen[i2 >> 1];
-              if (NT > 1)
+              if (MODE == kRows)
                 each = __any_sync(0xffffffffu, !finite2(a[0]) || !finite2(a[1]) || !finite2(a[2]) || !finite2(a[3]));
             }
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
               if (NT > 1 && !live[nt]) continue;
-              if (!each) mma16816(O[nt][4 * q + k], a[0], a[1], a[2], a[3], ph[nt][0], ph[nt][1]);
-              else
-                mma16816(O[nt][4 * q + k], a[0] & keep[nt][0], a[1] & keep[nt][0], a[2] & keep[nt][1], a[3] & keep[nt][1],
-                         ph[nt][0], ph[nt][1]);
+              float(&o)[4] = O[nt][4 * q + k];
+              if (!each) {
+                mma16816(o, a[0], a[1], a[2], a[3], ph[nt][0], ph[nt][1]);
+                if constexpr (MODE == kRows) mma16816(o, a[0], a[1], a[2], a[3], pl[nt][0], pl[nt][1]);
+                continue;
+              }
+              if constexpr (MODE == kRows)
+                for (int r = 0; r < per_tile; r++) {     // the lanes of row r's columns give their mask and their p
+                  const int from = r * slots * 4 + t;
+                  const uint32_t k0 = __shfl_sync(0xffffffffu, keep[nt][0], from), k1 = __shfl_sync(0xffffffffu, keep[nt][1], from);
+                  const bool mine = g / slots == r;
+                  mma16816(o, a[0] & k0, a[1] & k0, a[2] & k1, a[3] & k1, mine ? ph[nt][0] : 0u, mine ? ph[nt][1] : 0u);
+                  mma16816(o, a[0] & k0, a[1] & k0, a[2] & k1, a[3] & k1, mine ? pl[nt][0] : 0u, mine ? pl[nt][1] : 0u);
+                }
             }
           }
         }
@@ -816,23 +871,30 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT, WIDE>::THREADS, Shape<BITS
         l += __shfl_xor_sync(0xffffffffu, l, 4);
         l += __shfl_xor_sync(0xffffffffu, l, 8);
         l += __shfl_xor_sync(0xffffffffu, l, 16);
-        if (lane < 2) {
-          ml[(warp * LC + nt * 4 + 2 * t + k) * 2] = top[nt][k] - lift;
-          ml[(warp * LC + nt * 4 + 2 * t + k) * 2 + 1] = l;
+        if (lane < TC / 2) {
+          ml[(warp * LC + nt * TC + 2 * t + k) * 2] = top[nt][k] - lift;
+          ml[(warp * LC + nt * TC + 2 * t + k) * 2 + 1] = l;
         }
       }
-      // hi + lo: lanes t < 2 (the hi columns) take the even tiles, their partners the odd ones
+      const auto dim_of = [&](int o, int k) {
+        return BITS == 4 ? (o / 2) * 32 + 4 * g + (o & 1) + 2 * (k >> 1) : (o / 4) * 64 + 8 * g + 2 * (o & 3) + (k >> 1);
+      };
+      if constexpr (MODE == kRows) {
 #pragma unroll
-      for (int o = 0; o < OT; o += 2)
+        for (int o = 0; o < OT; o++)
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-          const float give = t < 2 ? O[nt][o + 1][k] : O[nt][o][k], keep_ = t < 2 ? O[nt][o][k] : O[nt][o + 1][k];
-          const float x = keep_ + __shfl_xor_sync(0xffffffffu, give, 2);
-          const int tile = o + (t >> 1);
-          const int dim = BITS == 4 ? (o / 2) * 32 + 4 * g + (t >> 1) + 2 * (k >> 1)
-                                    : (o / 4) * 64 + 8 * g + 2 * (tile & 3) + (k >> 1);
-          merge[(size_t)(warp * LC + nt * 4 + 2 * (t & 1) + (k & 1)) * HD + dim] = x;
-        }
+          for (int k = 0; k < 4; k++) merge[(size_t)(warp * LC + nt * TC + 2 * t + (k & 1)) * HD + dim_of(o, k)] = O[nt][o][k];
+      } else {
+        // hi + lo: lanes t < 2 (the hi columns) take the even tiles, their partners the odd ones
+#pragma unroll
+        for (int o = 0; o < OT; o += 2)
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            const float give = t < 2 ? O[nt][o + 1][k] : O[nt][o][k], mine = t < 2 ? O[nt][o][k] : O[nt][o + 1][k];
+            const float x = mine + __shfl_xor_sync(0xffffffffu, give, 2);
+            merge[(size_t)(warp * LC + 2 * (t & 1) + (k & 1)) * HD + dim_of(o, k) + (t >> 1) * (dim_of(1, 0) - dim_of(0, 0))] = x;
+          }
+      }
     }
     consumers();
     const uint32_t c0 = unit_c0, c1 = unit_c1;
@@ -859,7 +921,7 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT, WIDE>::THREADS, Shape<BITS
     for (int e = tid; e < cols * (HD / 4); e += CT) {
       const int c = e / (HD / 4), dim = e % (HD / 4) * 4;
       if (!col_live(c)) continue;
-      const int w0 = (c >> 2) / NT, lc = ((c >> 2) % NT) * 4 + (c & 3);
+      const int w0 = c / LC, lc = c % LC;
       float M = -INFINITY, L = 0.f;
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
@@ -952,28 +1014,26 @@ __global__ void __launch_bounds__(Shape<BITS, HD, NT, WIDE>::THREADS, Shape<BITS
   }
 }
 
-template <int BITS, int HD, int NT, bool WIDE>
+template <int BITS, int HD, int MODE>
 int launch(e4b_ctx* c, const AttnP& p) {
-  using Sh = Shape<BITS, HD, NT, WIDE>;
+  using Sh = Shape<BITS, HD, MODE>;
   static_assert(Sh::PER_SM * (Sh::SMEM + 8 * 1024) < 228 * 1024, "shared memory");
-  E4B_CUDA(c, cudaFuncSetAttribute(k_attn_paged<BITS, HD, NT, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Sh::SMEM));
+  E4B_CUDA(c, cudaFuncSetAttribute(k_attn_paged<BITS, HD, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Sh::SMEM));
   const int ctas = Sh::PER_SM * c->sm_count < Sh::MAX_CTAS ? Sh::PER_SM * c->sm_count : Sh::MAX_CTAS;
-  return e4b_launch(c, "attn_paged", k_attn_paged<BITS, HD, NT, WIDE>, dim3(ctas), dim3(Sh::THREADS), Sh::SMEM, p);
+  return e4b_launch(c, "attn_paged", k_attn_paged<BITS, HD, MODE>, dim3(ctas), dim3(Sh::THREADS), Sh::SMEM, p);
 }
 template <int BITS, int HD>
-int launch_nt(e4b_ctx* c, const AttnP& p) {
-  // a warp's n-tiles of 4 heads: one, or two where a sequence may have several rows
-  // (they share the decoded keys and values) and for more than 4 heads
-  if (p.G > 4 || p.d.rows) return launch<BITS, HD, 2, false>(c, p);
+int launch_mode(e4b_ctx* c, const AttnP& p) {
+  if (p.G > 4 || p.d.rows) return launch<BITS, HD, kRows>(c, p);
   // few units: all of an SM's warps on one (a 131K-token sequence of 2 KV heads 32 us
   // against 40 us); more units than SMs: two CTAs per SM (64 x 1..8000 tokens of 4 KV
   // heads, f16: 33 us against 60 us; 64 x 1035 tokens, 4 bits: 37 us against 41 us)
-  if (p.d.nseq * p.d.KVH <= c->sm_count) return launch<BITS, HD, 1, true>(c, p);
-  return launch<BITS, HD, 1, false>(c, p);
+  if (p.d.nseq * p.d.KVH <= c->sm_count) return launch<BITS, HD, kWide>(c, p);
+  return launch<BITS, HD, kNarrow>(c, p);
 }
 template <int BITS>
 int launch_hd(e4b_ctx* c, const AttnP& p, int HD) {
-  return HD == 256 ? launch_nt<BITS, 256>(c, p) : (HD == 128 ? launch_nt<BITS, 128>(c, p) : launch_nt<BITS, 64>(c, p));
+  return HD == 256 ? launch_mode<BITS, 256>(c, p) : (HD == 128 ? launch_mode<BITS, 128>(c, p) : launch_mode<BITS, 64>(c, p));
 }
 }  // namespace
 
@@ -981,7 +1041,7 @@ extern "C" {
 
 E4B_API size_t e4b_paged_scratch_bytes(void) {
   // two partials for each of kMaxCtas / 2 CTAs of the shape with the largest ones
-  return kMaxCtas * (3 * sizeof(uint32_t) + Shape<4, 256, 2, false>::PART * sizeof(float));
+  return kMaxCtas * (3 * sizeof(uint32_t) + Shape<4, 256, kRows>::PART * sizeof(float));
 }
 
 E4B_API int e4b_attn_paged(e4b_ctx* c, const e4b_paged_kv* kv, const float* q, uint16_t* out_h, float* out_f,
