@@ -29,6 +29,8 @@
 // n - 8.  A value block's scale multiplies p, again as hi + lo; p is lifted by 2^8
 // unless a scale of the piece is 2 or more, so that the lo parts stay clear of
 // f16's subnormals.
+#include <type_traits>
+
 #include "paged.cuh"
 #include "stream.cuh"
 
@@ -80,8 +82,9 @@ struct Shape {
   // warps (a warp then never waits for a phase before the stage's last one is done)
   static constexpr int S = W * (BITS == 16 ? (HD == 256 ? 1 : (HD == 128 ? 2 : 4)) :
                                 MODE == kRows ? (HD == 256 ? 2 : (HD == 128 ? 4 : 8)) : (HD == 256 ? 3 : (HD == 128 ? 5 : 8)));
-  // what a unit costs beside its pieces (q, the merge, the outputs), in pieces
-  static constexpr int U = MODE == kRows ? 48 : (BITS == 16 ? (HD == 256 ? 6 : (HD == 128 ? 8 : 12)) : (HD == 256 ? 12 : 16));
+  // what a unit of wc sharing warps costs beside its pieces (q, the merge, the outputs),
+  // in a warp's pieces: set_up(wc)
+  static constexpr int U = MODE == kRows ? 16 : (BITS == 16 ? (HD == 256 ? 6 : (HD == 128 ? 8 : 12)) : (HD == 256 ? 12 : 16));
   static constexpr int LN = S <= 32 ? S : (W == 11 ? 11 : (W == 5 ? (S == 40 ? 20 : 25) : 32));   // producer lanes; S is a multiple
   static constexpr int THREADS = MODE == kRows ? 384 : 32 * (W + 1), CT = 32 * W;
   static constexpr int COLS = MODE == kRows ? W * LC : LC;              // columns (row, head) of a unit at most
@@ -100,6 +103,7 @@ struct Rows {
   int slots;                         // columns of a row in a tile: its heads, up to a power of two (one row: 4)
   E4B_DEV explicit Rows(int G) : slots(MODE != kRows ? 4 : (G > 4 ? 8 : (G > 2 ? 4 : G))) {}
   E4B_DEV int per_tile() const { return MODE == kRows ? 8 / slots : 1; }
+  static E4B_DEV uint32_t set_up(int U, uint32_t wc) { return MODE == kRows ? U + 8 * wc : U; }
   E4B_DEV uint32_t per_warp() const { return NT * per_tile(); }
   E4B_DEV uint32_t per_unit() const { return per_warp() * W; }
   // warps that share a piece, for a unit of r rows: a power of two
@@ -137,7 +141,7 @@ E4B_DEV SeqWork seq_work(const AttnP& p, int s) {
     const uint32_t rest = w.nq % rows.per_unit();
     w.tail_wc = rest ? rows.sharing(rest) : 0u;
     const uint64_t np = w.range.count;
-    w.cost = p.d.KVH * (w.full * (U + np * W) + (rest ? U + np * w.tail_wc : 0));
+    w.cost = p.d.KVH * (w.full * (rows.set_up(U, W) + np * W) + (rest ? rows.set_up(U, w.tail_wc) + np * w.tail_wc : 0));
   }
   return w;
 }
@@ -152,7 +156,8 @@ struct Walk {
   uint64_t g, end, base;             // base: where the current sequence's work begins
   int s;
   SeqWork w;
-  uint64_t unit0, unit1;             // the unit's work
+  uint64_t unit0, unit1;             // the unit's work, the first `lead` of it its set-up
+  uint32_t lead;
   uint32_t kvh, wc, nrows;           // KV head, sharing warps, rows
   uint32_t pmin, pmax;               // positions of the unit's rows
   PieceSpan span;                    // this CTA's pieces of it
@@ -168,29 +173,30 @@ struct Walk {
     }
     const Rows<W, NT, MODE> rows(p.G);
     const uint32_t KVH = p.d.KVH, np = w.range.count;
-    const uint64_t off = g - base, full_cost = ((uint64_t)np * W + U) * w.full * KVH;
+    const uint64_t off = g - base, full_cost = ((uint64_t)np * W + rows.set_up(U, W)) * w.full * KVH;
     uint32_t group, unit;
     if (MODE == kRows && off < full_cost) {
       wc = W;
-      unit = (uint32_t)udiv(off, np * W + U);
-      unit0 = base + (uint64_t)unit * (np * W + U);
+      unit = (uint32_t)udiv(off, np * W + rows.set_up(U, W));
+      unit0 = base + (uint64_t)unit * (np * W + rows.set_up(U, W));
       group = unit / KVH;
       kvh = unit % KVH;
       nrows = rows.per_unit();
     } else {
       wc = w.tail_wc;
-      kvh = (uint32_t)udiv(off - full_cost, np * wc + U);
-      unit0 = base + full_cost + (uint64_t)kvh * (np * wc + U);
+      kvh = (uint32_t)udiv(off - full_cost, np * wc + rows.set_up(U, wc));
+      unit0 = base + full_cost + (uint64_t)kvh * (np * wc + rows.set_up(U, wc));
       group = w.full;
       nrows = w.nq - group * rows.per_unit();
     }
-    unit1 = unit0 + np * wc + U;
+    lead = rows.set_up(U, wc);
+    unit1 = unit0 + np * wc + lead;
     pmin = w.p0 + group * rows.per_unit();
     pmax = pmin + nrows - 1;
     const uint64_t stop = min(unit1, end);
     const uint32_t o0 = (uint32_t)(g - unit0), o1 = (uint32_t)(stop - unit0);
     const int sh = 31 - __clz((int)wc);                  // wc is a power of two
-    const uint32_t k0 = o0 <= U ? 0u : (o0 - U + wc - 1) >> sh, k1 = o1 <= U ? 0u : (o1 - U + wc - 1) >> sh;
+    const uint32_t k0 = o0 <= lead ? 0u : (o0 - lead + wc - 1) >> sh, k1 = o1 <= lead ? 0u : (o1 - lead + wc - 1) >> sh;
     const uint32_t p1 = min(pmax, p.d.cap - 1);
     span = piece_span(w.range, k0, k1, min(pmin, p1), p1, p.window, p.sinks);
     g = stop;
@@ -290,7 +296,7 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
   __shared__ uint64_t landed[S], freed[S];
   __shared__ int usable[S];
   __shared__ uint64_t warp_sum_[Sh::THREADS / 32];
-  __shared__ uint2 qzero[BITS == 4 ? Sh::TILES * 32 : 1];               // B of the -8 term: -8 sum q per block, hi and lo
+  __shared__ uint2 qzero[BITS == 4 ? Sh::TILES * 32 : 32];               // B of the -8 term: -8 sum q per block, hi and lo
   __shared__ float qfac[Sh::TILES * TC];
   __shared__ float ml[W * LC * 2];
   __shared__ int last_one, more_units;
@@ -332,8 +338,8 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
     T += warp_sum_[i];
   }
   upto += before;
-  // runs of 2 U at least; an end that falls within U of a unit's start or end moves
-  // there, so short units stay whole and no fragment is shorter than U
+  // runs of 2 U at least; an end that falls within a unit's set-up cost of its start or
+  // end moves there, so short units stay whole and no fragment is shorter than that
   const uint64_t want = udiv(T, 2 * U);
   const uint32_t C = T == 0 ? 0u : (want < 1 ? 1u : (want < gridDim.x ? (uint32_t)want : gridDim.x));
   const uint32_t cta = blockIdx.x;
@@ -354,7 +360,7 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
           v.end = raw + 1;
           v.next(p);
         }
-        const uint64_t at = raw - v.unit0 < U ? v.unit0 : (v.unit1 - raw < U ? v.unit1 : raw);
+        const uint64_t at = raw - v.unit0 < v.lead ? v.unit0 : (v.unit1 - raw < v.lead ? v.unit1 : raw);
         run_end[i] = at;
         if (i == 0) {
           v.g = at;
@@ -442,12 +448,8 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
     more_units = v.next(p);
     unit = v;
     const auto run_of = [&](uint64_t x) { return (uint32_t)udiv((x + 1) * C - 1, T); };
-    uint32_t c0 = run_of(v.unit0), c1 = run_of(v.unit1 - 1);
-    if (c1 > c0) {
-      const uint64_t after = udiv(T * (c0 + 1), C), inside = udiv(T * c1, C);
-      if (inside - v.unit0 >= U && v.unit1 - inside < U) c1--;
-      if (after > v.unit0 && after < v.unit1 && after - v.unit0 < U) c0++;
-    }
+    const uint32_t c0 = run_of(min(v.unit0 + v.lead, v.unit1) - 1);
+    const uint32_t c1 = v.unit1 - v.unit0 < 2 * v.lead ? c0 : run_of(v.unit1 - v.lead);
     unit_c0 = c0;
     unit_c1 = c1;
   };
@@ -472,15 +474,13 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
 #pragma unroll 4
       for (int c0 = 0; c0 < cols; c0 += CT / LPC) {
         const int c = c0 + sub, tile = c / TC, cc = c % TC;
-        float x[8];
+        const bool on = c < cols && col_live(c);
+        const float4* src = reinterpret_cast<const float4*>(
+            p.q + ((size_t)(row0 + (on ? col_row(c) : 0)) * p.QH + unit.kvh * p.G + (on ? col_head(c) : 0)) * HD + 8 * l);
+        const float4 xa = src[0], xb = src[1];
+        float x[8] = {xa.x, xa.y, xa.z, xa.w, xb.x, xb.y, xb.z, xb.w};
 #pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = 0.f;
-        if (c < cols && col_live(c)) {
-          const float4* src = reinterpret_cast<const float4*>(
-              p.q + ((size_t)(row0 + col_row(c)) * p.QH + unit.kvh * p.G + col_head(c)) * HD + 8 * l);
-          const float4 a = src[0], b = src[1];
-          x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-        }
+        for (int i = 0; i < 8; i++) x[i] = on ? x[i] : 0.f;
         float m = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(x[i]));
@@ -531,13 +531,11 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
     }
     consumers();
     float top[NT][2], lsum[NT][2], fac[NT][2], lift = kLift, slack = kSlack;  // reference score; sum of p; score factor
-    bool live[NT];
     uint32_t pos0[NT], pos1[NT], pos[NT][2], posg[NT];   // of the tile's first and last row, the lane's score columns, its p column
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
       const int tile = wc * NT + nt;
       const auto position = [&](int row) { return min(unit.pmin + row, unit.pmax); };
-      live[nt] = (uint32_t)(tile * per_tile) < unit.nrows;
       pos0[nt] = position(tile * per_tile);
       pos1[nt] = position(tile * per_tile + per_tile - 1);
       posg[nt] = position(col_row(tile * TC + g % TC));
@@ -554,6 +552,7 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
 #pragma unroll
         for (int k = 0; k < 4; k++) O[nt][i][k] = 0.f;
     }
+    const int live_tiles = NT > 1 && (uint32_t)((wc * NT + NT - 1) * per_tile) < unit.nrows ? NT : 1;
     const uint4* qf = qfrag + (size_t)wc * NT * NB * QP * 32 + lane;
 
     const PieceSpan span = unit.span;
@@ -561,26 +560,21 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
     bool fresh = true;               // O is zero
     const uint32_t i0 = (uint32_t)ws >= turn ? ws - turn : ws + WS - turn;
     uint32_t st = (j0 + i0) % S, phase = (j0 + i0) / S & 1u;
-    for (uint32_t i = i0; i < span.count; i += WS) {
-      const uint32_t t0 = span.at(i) * kPieceSlots;
-      if (!__all_sync(0xffffffffu, mbar_try_wait(&landed[st], phase)) && alive)
-        alive = __all_sync(0xffffffffu, wait_slow(&landed[st], phase, p.d.status));
-      const bool here = alive && usable[st] != 0;
-      const uint8_t* kp = ring + (size_t)st * Sh::STAGE;
-      const uint8_t* vp = kp + PB;
-
+    // a piece's work for the warp's first N tiles (the others hold no row)
+    const auto work = [&](auto tiles, const uint8_t* kp, const uint8_t* vp, uint32_t t0, bool here) {
+      constexpr int N = decltype(tiles)::value;
       // ---- scores
-      float s[NT][4];
-      if constexpr (BITS == 4) {
+      float s[N][4];
+      if (BITS == 4) {
         constexpr int RUN = NB < 4 ? NB : 4;
         uint32_t da[NB / 2], db[NB / 2];                 // scales of slots g, g + 8
         lds_words<NB / 2>(da, kp + g * NB * 2);
         lds_words<NB / 2>(db, kp + (g + 8) * NB * 2);
-        float z[NT][4];
+        float z[N][4];
         const uint32_t dz0 = t < NB / 2 ? *reinterpret_cast<const uint32_t*>(kp + g * NB * 2 + t * 4) : 0u;
         const uint32_t dz1 = t < NB / 2 ? *reinterpret_cast<const uint32_t*>(kp + (g + 8) * NB * 2 + t * 4) : 0u;
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
+        for (int nt = 0; nt < N; nt++) {
           const uint2 zb = qzero[(wc * NT + nt) * 32 + lane];
           mma16816_zero(z[nt], dz0, dz1, dz0, dz1, zb.x, zb.y);
 #pragma unroll
@@ -597,13 +591,12 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
             const uint32_t sa = wa[q] >> 8, sb = wb[q] >> 8;
             const float d0 = half_of(da[b / 2], b & 1), d1 = half_of(db[b / 2], b & 1);
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-              if (NT > 1 && !live[nt]) continue;
+            for (int nt = 0; nt < N; nt++) {
               const uint4 qb = qf[(nt * NB + b) * QP * 32];
               float acc[4];
               mma16816_zero(acc, wa[q] & kLowCodes, wb[q] & kLowCodes, sa & kLowCodes, sb & kLowCodes, qb.x, qb.y);
               mma16816(acc, wa[q] & kHighCodes, wb[q] & kHighCodes, sa & kHighCodes, sb & kHighCodes, qb.z, qb.w);
-              if constexpr (MODE == kRows) {
+              if (MODE == kRows) {
                 const uint4 ql = qf[((nt * NB + b) * QP + 1) * 32];
                 mma16816(acc, wa[q] & kLowCodes, wb[q] & kLowCodes, sa & kLowCodes, sb & kLowCodes, ql.x, ql.y);
                 mma16816(acc, wa[q] & kHighCodes, wb[q] & kHighCodes, sa & kHighCodes, sb & kHighCodes, ql.z, ql.w);
@@ -616,25 +609,24 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
           }
         }
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++)
+        for (int nt = 0; nt < N; nt++)
 #pragma unroll
           for (int k = 0; k < 4; k++) s[nt][k] = fmaf(s[nt][k], kTwo24, z[nt][k] * 256.f);
       } else {
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++)
+        for (int nt = 0; nt < N; nt++)
 #pragma unroll
           for (int k = 0; k < 4; k++) s[nt][k] = 0.f;
 #pragma unroll
         for (int b = 0; b < NB; b++) {
           const uint4 wa = lds128(kp + (b * 16 + g) * 64 + t * 16), wb = lds128(kp + (b * 16 + g + 8) * 64 + t * 16);
 #pragma unroll
-          for (int nt = 0; nt < NT; nt++) {
-            if (NT > 1 && !live[nt]) continue;
+          for (int nt = 0; nt < N; nt++) {
             const uint4 qb = qf[(nt * NB + b) * QP * 32];
             float acc[4];
             mma16816_zero(acc, wa.x, wb.x, wa.y, wb.y, qb.x, qb.y);
             mma16816(acc, wa.z, wb.z, wa.w, wb.w, qb.z, qb.w);
-            if constexpr (MODE == kRows) {
+            if (MODE == kRows) {
               const uint4 ql = qf[((nt * NB + b) * QP + 1) * 32];
               mma16816(acc, wa.x, wb.x, wa.y, wb.y, ql.x, ql.y);
               mma16816(acc, wa.z, wb.z, wa.w, wb.w, ql.z, ql.w);
@@ -646,7 +638,7 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
       }
 
       // ---- value scales of slots (2t, 2t+1) and (2t+8, 2t+9); one of 2 or more ends the lift of p
-      if constexpr (BITS == 4) {
+      if (BITS == 4) {
         uint32_t any = 0;
 #pragma unroll
         for (int b = 0; b < NB; b += 2) {
@@ -656,7 +648,7 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
         if (__any_sync(0xffffffffu, (any & 0x40004000u) != 0) && lift != 0.f) {
           lift = slack = 0.f;
 #pragma unroll
-          for (int nt = 0; nt < NT; nt++) {
+          for (int nt = 0; nt < N; nt++) {
             lsum[nt][0] *= 1.f / 256.f, lsum[nt][1] *= 1.f / 256.f;
 #pragma unroll
             for (int o = 0; o < OT; o++)
@@ -667,18 +659,17 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
       }
 
       // ---- softmax state and p as B fragments
-      uint32_t ph[NT][2], pl[NT][2], keep[NT][2];        // slots (2t, 2t+1), (2t+8, 2t+9); keep: mask of visible halves
-      bool full[NT];
+      uint32_t ph[N][2], pl[N][2], keep[N][2];        // slots (2t, 2t+1), (2t+8, 2t+9); keep: mask of visible halves
+      bool full[N];
 #pragma unroll
-      for (int nt = 0; nt < NT; nt++) {
+      for (int nt = 0; nt < N; nt++) {
         full[nt] = here && t0 + kPieceSlots - 1 <= pos0[nt] &&
                    (p.window == 0 || pos1[nt] - t0 < p.window || t0 + kPieceSlots <= p.sinks);
-        if (NT > 1 && !live[nt]) continue;
         float v[4];
         bool see[4] = {true, true, true, true};
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-          if constexpr (MODE != kRows) s[nt][k] += __shfl_xor_sync(0xffffffffu, s[nt][k], 2);     // hi + lo columns
+          if (MODE != kRows) s[nt][k] += __shfl_xor_sync(0xffffffffu, s[nt][k], 2);     // hi + lo columns
           v[k] = s[nt][k] * fac[nt][k & 1];
         }
         if (!full[nt]) {
@@ -725,10 +716,10 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
           const uint32_t h = pack2(e[2 * k], e[2 * k + 1]);
           const float2 hf = __half22float2(*reinterpret_cast<const __half2*>(&h));
           const uint32_t l = pack2(e[2 * k] - hf.x, e[2 * k + 1] - hf.y);
-          if constexpr (MODE == kRows) {
+          if (MODE == kRows) {
             ph[nt][k] = transpose8x8(h);
             pl[nt][k] = transpose8x8(l);
-          } else if constexpr (BITS == 4) {
+          } else if (BITS == 4) {
             // columns 0-3: (0, hi), columns 4-7: (hi, lo); see the product with the scales
             ph[nt][k] = transpose8x8(t < 2 ? 0u : h);
             pl[nt][k] = transpose8x8(t < 2 ? h : l);
@@ -741,13 +732,12 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
       // ---- slots that no row of the warp sees may hold anything: their scales (values)
       // become zero.  strict: a row does not see a slot that another row sees and that
       // holds an infinity or NaN, so its own mask goes on every operand.
-      bool strict[NT];
+      bool strict[N];
       uint32_t seen[2] = {0u, 0u};
       bool masked = false;
 #pragma unroll
-      for (int nt = 0; nt < NT; nt++) {
+      for (int nt = 0; nt < N; nt++) {
         strict[nt] = false;
-        if (NT > 1 && !live[nt]) continue;
         if (full[nt]) keep[nt][0] = keep[nt][1] = 0xffffffffu;
         else masked = true;
         seen[0] |= keep[nt][0], seen[1] |= keep[nt][1];
@@ -760,8 +750,8 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
           seen[k] |= __shfl_xor_sync(0xffffffffu, seen[k], 16);
         }
       }
-      uint32_t dv[BITS == 4 ? NB : 1][2];
-      if constexpr (BITS == 4) {
+      uint32_t dv[NB][2];
+      if (BITS == 4) {
 #pragma unroll
         for (int b = 0; b < NB; b += 2) {
           const uint4 d4 = lds128(vp + (t * NB + b) * 8);
@@ -778,13 +768,13 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
             }
           if (MODE == kRows && __any_sync(0xffffffffu, odd)) {
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) strict[nt] = true;
+            for (int nt = 0; nt < N; nt++) strict[nt] = true;
           }
         }
       }
 
       // ---- O += V^T p
-      if constexpr (BITS == 4) {
+      if (BITS == 4) {
         uint32_t vw[4][NB / 2];
 #pragma unroll
         for (int k = 0; k < 4; k++) lds_words<NB / 2>(vw[k], vp + HD + (k * 32 + lane) * (NB * 2));
@@ -796,8 +786,7 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
           const uint32_t al[4] = {low_codes(x), low_codes(xs), low_codes(y), low_codes(ys)};
           const uint32_t ah[4] = {high_codes(x), high_codes(xs), high_codes(y), high_codes(ys)};
 #pragma unroll
-          for (int nt = 0; nt < NT; nt++) {
-            if (NT > 1 && !live[nt]) continue;
+          for (int nt = 0; nt < N; nt++) {
             uint32_t bb[2], bh[2];
 #pragma unroll
             for (int k = 0; k < 2; k++) {
@@ -807,7 +796,7 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
               bh[k] = hmul2(ph[nt][k], d);
               bb[k] = hfma2(pl[nt][k], d, hfms2(ph[nt][k], d, bh[k]));
             }
-            if constexpr (MODE == kRows) {
+            if (MODE == kRows) {
               mma16816(O[nt][2 * b], al[0], al[1], al[2], al[3], bh[0], bh[1]);
               mma16816(O[nt][2 * b + 1], ah[0], ah[1], ah[2], ah[3], bh[0], bh[1]);
             }
@@ -833,15 +822,14 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
                 each = __any_sync(0xffffffffu, !finite2(a[0]) || !finite2(a[1]) || !finite2(a[2]) || !finite2(a[3]));
             }
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-              if (NT > 1 && !live[nt]) continue;
+            for (int nt = 0; nt < N; nt++) {
               float(&o)[4] = O[nt][4 * q + k];
               if (!each) {
                 mma16816(o, a[0], a[1], a[2], a[3], ph[nt][0], ph[nt][1]);
-                if constexpr (MODE == kRows) mma16816(o, a[0], a[1], a[2], a[3], pl[nt][0], pl[nt][1]);
+                if (MODE == kRows) mma16816(o, a[0], a[1], a[2], a[3], pl[nt][0], pl[nt][1]);
                 continue;
               }
-              if constexpr (MODE == kRows)
+              if (MODE == kRows)
                 for (int r = 0; r < per_tile; r++) {     // the lanes of row r's columns give their mask and their p
                   const int from = r * slots * 4 + t;
                   const uint32_t k0 = __shfl_sync(0xffffffffu, keep[nt][0], from), k1 = __shfl_sync(0xffffffffu, keep[nt][1], from);
@@ -853,6 +841,17 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
           }
         }
       }
+    };
+    for (uint32_t i = i0; i < span.count; i += WS) {
+      const uint32_t t0 = span.at(i) * kPieceSlots;
+      if (!__all_sync(0xffffffffu, mbar_try_wait(&landed[st], phase)) && alive)
+        alive = __all_sync(0xffffffffu, wait_slow(&landed[st], phase, p.d.status));
+      const bool here = alive && usable[st] != 0;
+      const uint8_t* kp = ring + (size_t)st * Sh::STAGE;
+      const uint8_t* vp = kp + PB;
+
+      if (live_tiles == NT) work(std::integral_constant<int, NT>{}, kp, vp, t0, here);
+      else work(std::integral_constant<int, 1>{}, kp, vp, t0, here);
       __syncwarp();
       if (lane == 0 && alive) mbar_arrive_n(&freed[st], WS);
       fresh = false;
@@ -899,11 +898,9 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
     consumers();
     const uint32_t c0 = unit_c0, c1 = unit_c1;
     const bool whole = c0 == c1;
-    const auto finish = [&](int c, int dim, const float4& o, float M, float L) {
+    const auto store = [&](int c, int dim, const float4& x) {
       const int head = unit.kvh * p.G + col_head(c);
       const size_t row = row0 + col_row(c);
-      const float r = L != 0.f ? 1.f / L : 0.f;          // a NaN sum stays one
-      const float4 x = make_float4(o.x * r, o.y * r, o.z * r, o.w * r);
       if (p.out_f) *reinterpret_cast<float4*>(p.out_f + (row * p.QH + head) * HD + dim) = x;
       if (p.out_h) {
         uint16_t* out = p.out_h + row * p.QH * HD;
@@ -915,32 +912,71 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
           *reinterpret_cast<uint2*>(out + at) = make_uint2(pack2(x.x, x.y), pack2(x.z, x.w));
         }
       }
-      if (p.lse && dim == 0) p.lse[row * p.QH + head] = L != 0.f ? (M + log2f(L)) * 0.6931471805599453f : -INFINITY;
+    };
+    // a column's logarithm of the sum; what its sum is divided by (a NaN sum stays one)
+    const auto close_column = [&](int c, float M, float L) {
+      if (p.lse)
+        p.lse[(row0 + col_row(c)) * (size_t)p.QH + unit.kvh * p.G + col_head(c)] = L != 0.f ? (M + log2f(L)) * 0.6931471805599453f : -INFINITY;
+      return L != 0.f ? 1.f / L : 0.f;
     };
     float* part = p.parts + (2 * (size_t)cta + (cta == c0 ? 1 : 0)) * Sh::PART;  // a run ends with at most one cut unit, and begins with one
-    for (int e = tid; e < cols * (HD / 4); e += CT) {
-      const int c = e / (HD / 4), dim = e % (HD / 4) * 4;
-      if (!col_live(c)) continue;
-      const int w0 = c / LC, lc = c % LC;
-      float M = -INFINITY, L = 0.f;
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (uint32_t i = 0; i < W; i++)
-        if (i < WS) M = fmaxf(M, ml[((i * WC + w0) * LC + lc) * 2]);
-#pragma unroll
-      for (uint32_t i = 0; i < W; i++) {
-        if (i >= WS) continue;
-        const int at = (i * WC + w0) * LC + lc;
-        const float mi = ml[at * 2], a = mi == M ? 1.f : ex2(mi - M);
-        const float4 x = *reinterpret_cast<const float4*>(merge + (size_t)at * HD + dim);
-        L = fmaf(a, ml[at * 2 + 1], L);
-        o.x = fmaf(a, x.x, o.x), o.y = fmaf(a, x.y, o.y), o.z = fmaf(a, x.z, o.z), o.w = fmaf(a, x.w, o.w);
+    if constexpr (MODE == kRows) {
+      for (int c = tid; c < cols; c += CT) {               // the weights of the WS states of each column
+        const int w0 = c / LC, lc = c % LC;
+        float M = -INFINITY, L = 0.f;
+        for (uint32_t i = 0; i < WS; i++) M = fmaxf(M, ml[((i * WC + w0) * LC + lc) * 2]);
+        for (uint32_t i = 0; i < WS; i++) {
+          float* at = ml + ((i * WC + w0) * LC + lc) * 2;
+          const float a = at[0] == M ? 1.f : ex2(at[0] - M);
+          L = fmaf(a, at[1], L);
+          at[0] = a;
+        }
+        float r = 1.f;
+        if (!col_live(c)) r = 0.f;
+        else if (whole) r = close_column(c, M, L);
+        else *reinterpret_cast<float2*>(part + Sh::COLS * HD + 2 * c) = make_float2(M, L);
+        for (uint32_t i = 0; i < WS; i++) ml[((i * WC + w0) * LC + lc) * 2] *= r;
       }
-      if (whole) {
-        finish(c, dim, o, M, L);
-      } else {
-        *reinterpret_cast<float4*>(part + c * HD + dim) = o;
-        if (dim == 0) part[Sh::COLS * HD + 2 * c] = M, part[Sh::COLS * HD + 2 * c + 1] = L;
+      consumers();
+#pragma unroll 4
+      for (int e = tid; e < cols * (HD / 4); e += CT) {
+        const int c = e / (HD / 4), dim = e % (HD / 4) * 4;
+        const int w0 = c / LC, lc = c % LC;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (uint32_t i = 0; i < WS; i++) {
+          const int at = (i * WC + w0) * LC + lc;
+          const float a = ml[at * 2];
+          const float4 x = *reinterpret_cast<const float4*>(merge + (size_t)at * HD + dim);
+          o.x = fmaf(a, x.x, o.x), o.y = fmaf(a, x.y, o.y), o.z = fmaf(a, x.z, o.z), o.w = fmaf(a, x.w, o.w);
+        }
+        if (!col_live(c)) continue;
+        if (whole) store(c, dim, o);
+        else *reinterpret_cast<float4*>(part + c * HD + dim) = o;
+      }
+    } else {                         // few columns: every thread forms its column's weights
+      for (int e = tid; e < LC * (HD / 4); e += CT) {
+        const int c = e / (HD / 4), dim = e % (HD / 4) * 4;
+        if (!col_live(c)) continue;
+        float M = -INFINITY, L = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < W; i++) M = fmaxf(M, ml[(i * LC + c) * 2]);
+#pragma unroll
+        for (int i = 0; i < W; i++) {
+          const int at = i * LC + c;
+          const float mi = ml[at * 2], w = mi == M ? 1.f : ex2(mi - M);
+          const float4 x = *reinterpret_cast<const float4*>(merge + (size_t)at * HD + dim);
+          L = fmaf(w, ml[at * 2 + 1], L);
+          o.x = fmaf(w, x.x, o.x), o.y = fmaf(w, x.y, o.y), o.z = fmaf(w, x.z, o.z), o.w = fmaf(w, x.w, o.w);
+        }
+        if (whole) {
+          const float r = L != 0.f ? 1.f / L : 0.f;
+          store(c, dim, make_float4(o.x * r, o.y * r, o.z * r, o.w * r));
+          if (dim == 0) close_column(c, M, L);
+        } else {
+          *reinterpret_cast<float4*>(part + c * HD + dim) = o;
+          if (dim == 0) *reinterpret_cast<float2*>(part + Sh::COLS * HD + 2 * c) = make_float2(M, L);
+        }
       }
     }
     if (!whole) {
@@ -963,33 +999,90 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
         for (uint32_t e = tid; e < n * cols; e += CT)
           part_ml[e] = __ldcg(reinterpret_cast<const float2*>(part_of(a + e / cols * step) + Sh::COLS * HD + 2 * (e % cols)));
         consumers();
-        for (int e = tid; e < cols * (HD / 4); e += CT) {
-          const int c = e / (HD / 4), dim = e % (HD / 4) * 4;
-          if (!col_live(c)) continue;
-          float M = -INFINITY, L = 0.f;
-          for (uint32_t i = 0; i < n; i++) M = fmaxf(M, part_ml[i * cols + c].x);
-          float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        if constexpr (MODE != kRows) {
+          for (int e = tid; e < LC * (HD / 4); e += CT) {
+            const int c = e / (HD / 4), dim = e % (HD / 4) * 4;
+            if (!col_live(c)) continue;
+            float M = -INFINITY, L = 0.f;
+            for (uint32_t i = 0; i < n; i++) M = fmaxf(M, part_ml[i * LC + c].x);
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
-          for (uint32_t i0 = 0; i0 < n; i0 += 8) {        // eight parts' loads in flight
-            float4 x[8];
+            for (uint32_t i0 = 0; i0 < n; i0 += 8) {      // eight parts' loads in flight
+              float4 x[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++)
-              x[i] = __ldcg(reinterpret_cast<const float4*>(part_of(a + min(i0 + i, n - 1) * step) + c * HD + dim));
+              for (int i = 0; i < 8; i++)
+                x[i] = __ldcg(reinterpret_cast<const float4*>(part_of(a + min(i0 + i, n - 1) * step) + c * HD + dim));
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-              if (i0 + i >= n) continue;
-              const float2 y = part_ml[(i0 + i) * cols + c];
-              const float f = y.x == M ? 1.f : ex2(y.x - M);
-              L = fmaf(f, y.y, L);
-              o.x = fmaf(f, x[i].x, o.x), o.y = fmaf(f, x[i].y, o.y);
-              o.z = fmaf(f, x[i].z, o.z), o.w = fmaf(f, x[i].w, o.w);
+              for (int i = 0; i < 8; i++) {
+                if (i0 + i >= n) continue;
+                const float2 y = part_ml[(i0 + i) * LC + c];
+                const float f = y.x == M ? 1.f : ex2(y.x - M);
+                L = fmaf(f, y.y, L);
+                o.x = fmaf(f, x[i].x, o.x), o.y = fmaf(f, x[i].y, o.y);
+                o.z = fmaf(f, x[i].z, o.z), o.w = fmaf(f, x[i].w, o.w);
+              }
+            }
+            if (final) {
+              const float r = L != 0.f ? 1.f / L : 0.f;
+              store(c, dim, make_float4(o.x * r, o.y * r, o.z * r, o.w * r));
+              if (dim == 0) close_column(c, M, L);
+            } else {
+              *reinterpret_cast<float4*>(part_of(a) + c * HD + dim) = o;
+              if (dim == 0) *reinterpret_cast<float2*>(part_of(a) + Sh::COLS * HD + 2 * c) = make_float2(M, L);
             }
           }
+          return;
+        }
+        for (int c = tid; c < cols; c += CT) {           // the parts' weights
+          float M = -INFINITY, L = 0.f;
+          for (uint32_t i = 0; i < n; i++) M = fmaxf(M, part_ml[i * cols + c].x);
+          for (uint32_t i = 0; i < n; i++) {
+            float2& y = part_ml[i * cols + c];
+            y.x = y.x == M ? 1.f : ex2(y.x - M);
+            L = fmaf(y.x, y.y, L);
+          }
+          if (!col_live(c)) continue;
           if (final) {
-            finish(c, dim, o, M, L);
+            const float r = close_column(c, M, L);
+            for (uint32_t i = 0; i < n; i++) part_ml[i * cols + c].x *= r;
           } else {
-            *reinterpret_cast<float4*>(part_of(a) + c * HD + dim) = o;
-            if (dim == 0) *reinterpret_cast<float2*>(part_of(a) + Sh::COLS * HD + 2 * c) = make_float2(M, L);
+            *reinterpret_cast<float2*>(part_of(a) + Sh::COLS * HD + 2 * c) = make_float2(M, L);
+          }
+        }
+        consumers();
+        constexpr int kE = 4, kI = 2;    // eight loads in flight
+        for (int e0 = tid; e0 < cols * (HD / 4); e0 += kE * CT) {
+          float4 o[kE];
+#pragma unroll
+          for (int j = 0; j < kE; j++) o[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+          for (uint32_t i0 = 0; i0 < n; i0 += kI) {
+            float4 x[kI][kE];
+#pragma unroll
+            for (int i = 0; i < kI; i++)
+#pragma unroll
+              for (int j = 0; j < kE; j++) {
+                const int e = min(e0 + j * CT, cols * (HD / 4) - 1);
+                x[i][j] = __ldcg(reinterpret_cast<const float4*>(part_of(a + min(i0 + i, n - 1) * step)) + e);
+              }
+#pragma unroll
+            for (int i = 0; i < kI; i++) {
+              if (i0 + i >= n) continue;
+#pragma unroll
+              for (int j = 0; j < kE; j++) {
+                const int e = min(e0 + j * CT, cols * (HD / 4) - 1);
+                const float f = part_ml[(i0 + i) * cols + e / (HD / 4)].x;
+                o[j].x = fmaf(f, x[i][j].x, o[j].x), o[j].y = fmaf(f, x[i][j].y, o[j].y);
+                o[j].z = fmaf(f, x[i][j].z, o[j].z), o[j].w = fmaf(f, x[i][j].w, o[j].w);
+              }
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < kE; j++) {
+            const int e = e0 + j * CT, c = e / (HD / 4);
+            if (e >= cols * (HD / 4) || !col_live(c)) continue;
+            if (final) store(c, e % (HD / 4) * 4, o[j]);
+            else *(reinterpret_cast<float4*>(part_of(a)) + e) = o[j];
           }
         }
       };

@@ -214,21 +214,23 @@ __global__ void __launch_bounds__(threads_of<MODE>(), MODE == kFew ? 1 : 2) k_he
   }
   // the turn's items: its query heads (up to a whole warp's), then its key and value heads
   const int nq = (RT * p.QH + GROUPS - 1) / GROUPS * GROUPS, total = nq + (RT * 2 * KVH + GROUPS - 1) / GROUPS * GROUPS;
-  for (int i = tid; i < total; i += THREADS) {
+  const auto item_of = [&](int i) {
     Item it{0u, kNoRow, 0};
     if (i < RT * p.QH) {
-      it.row = (uint16_t)(i / p.QH);
-      it.head = (uint16_t)(i % p.QH);
+      it.row = (uint16_t)(RT == 1 ? 0 : i / p.QH);
+      it.head = (uint16_t)(i - it.row * p.QH);
       it.src = (uint32_t)it.head * HD * ES;
     } else if (i >= nq && i - nq < RT * 2 * KVH) {
-      const int h = (i - nq) % (2 * KVH), kvh = h < KVH ? h : h - KVH;
-      it.row = (uint16_t)((i - nq) / (2 * KVH));
+      it.row = (uint16_t)(RT == 1 ? 0 : (i - nq) / (2 * KVH));
+      const int h = i - nq - it.row * 2 * KVH, kvh = h < KVH ? h : h - KVH;
       it.head = (uint16_t)(kvh | (h < KVH ? kKey : kValue));
       it.src = (uint32_t)(p.QH + (p.keqv ? kvh : h)) * HD * ES;
     }
     if (MODE == kStaged && it.row != kNoRow) it.src += it.row * row_bytes;
-    items[i] = it;
-  }
+    return it;
+  };
+  if (MODE != kFew)
+    for (int i = tid; i < total; i += THREADS) items[i] = item_of(i);
   float qw[8];
 #pragma unroll
   for (int j = 0; j < 8; j++) qw[j] = 1.f;
@@ -305,7 +307,7 @@ __global__ void __launch_bounds__(threads_of<MODE>(), MODE == kFew ? 1 : 2) k_he
     float* const q_rows = p.q_out + (size_t)row0 * p.QH * HD + 4 * l;
     // every lane of a warp makes the same turns (shuffles): a group without a head works on row 0
     for (int i = blockIdx.y * NS + sub; alive && i < total; i += gridDim.y * NS) {
-      const Item it = items[i];
+      const Item it = MODE == kFew ? item_of(i) : items[i];
       const bool on = it.row < rows;
       const int r = on ? it.row : 0;
       Quad a, b;
