@@ -8,7 +8,7 @@
 // bulk copy for the keys, one for the values) through a ring of stages, a lane
 // per stage, into the next units too.  The consumer warps form WS x WC: WC warps
 // share a piece, each with its own query rows, and WS such groups take pieces in
-// turn.  A unit of one row has WC = 1, one of a prompt's chunk WC = W; a stage is
+// turn.  A unit of a few rows has WC = 1, one of a prompt's chunk WC = 2; a stage is
 // free after W arrivals, so its WC users arrive W / WC times each.  Every warp
 // keeps its own softmax state; at a unit's end the WS states are merged in shared
 // memory.  A unit cut between CTAs leaves partials in the scratch, which the last
@@ -64,6 +64,8 @@ struct AttnP {
 // scaled p are then shared by twice the columns, for prompts' and speculated rows.
 enum { kNarrow, kWide, kRows };
 constexpr int kConsumerRegs = 224, kProducerRegs = 56;
+constexpr int kShare = 2;            // kRows: warps that share a piece at most (a larger unit's merge and partials cost more than its
+                                     // pieces' second trip from L2)
 
 template <int BITS, int HD, int MODE>
 struct Shape {
@@ -87,9 +89,9 @@ struct Shape {
   static constexpr int U = MODE == kRows ? 16 : (BITS == 16 ? (HD == 256 ? 6 : (HD == 128 ? 8 : 12)) : (HD == 256 ? 12 : 16));
   static constexpr int LN = S <= 32 ? S : (W == 11 ? 11 : (W == 5 ? (S == 40 ? 20 : 25) : 32));   // producer lanes; S is a multiple
   static constexpr int THREADS = MODE == kRows ? 384 : 32 * (W + 1), CT = 32 * W;
-  static constexpr int COLS = MODE == kRows ? W * LC : LC;              // columns (row, head) of a unit at most
+  static constexpr int COLS = MODE == kRows ? kShare * LC : LC;         // columns (row, head) of a unit at most
   static constexpr size_t PART = (size_t)COLS * (HD + 2);               // floats of a partial
-  static constexpr int TILES = W * NT, QPARTS = MODE == kRows ? 2 : 1;  // n-tiles of a unit at most; fragments of a tile
+  static constexpr int TILES = (MODE == kRows ? kShare : 1) * NT, QPARTS = MODE == kRows ? 2 : 1;  // n-tiles of a unit at most; fragments of a tile
   static constexpr size_t RING = (size_t)S * STAGE;
   // q fragments [TILES][NB][QPARTS][32] while a unit's pieces pass, then the warps' O [W][LC][HD]
   static constexpr size_t MERGE = (size_t)W * LC * HD * 4;
@@ -105,7 +107,7 @@ struct Rows {
   E4B_DEV int per_tile() const { return MODE == kRows ? 8 / slots : 1; }
   static E4B_DEV uint32_t set_up(int U, uint32_t wc) { return MODE == kRows ? U + 8 * wc : U; }
   E4B_DEV uint32_t per_warp() const { return NT * per_tile(); }
-  E4B_DEV uint32_t per_unit() const { return per_warp() * W; }
+  E4B_DEV uint32_t per_unit() const { return per_warp() * kShare; }   // (one row: never full)
   // warps that share a piece, for a unit of r rows: a power of two
   E4B_DEV uint32_t sharing(uint32_t r) const {
     uint32_t wc = 1;
@@ -118,7 +120,7 @@ struct Rows {
 struct SeqWork {
   uint32_t p0, nq;                   // first row's position, rows
   PieceRange range;
-  uint32_t full, tail_wc;            // units of W sharing warps, sharing warps of the last unit (0: none)
+  uint32_t full, tail_wc;            // units of kShare sharing warps, sharing warps of the last unit (0: none)
   uint64_t cost;                     // sum over units and KV heads of U + pieces * sharing warps
 };
 template <int W, int NT, int U, int MODE>
@@ -141,7 +143,7 @@ E4B_DEV SeqWork seq_work(const AttnP& p, int s) {
     const uint32_t rest = w.nq % rows.per_unit();
     w.tail_wc = rest ? rows.sharing(rest) : 0u;
     const uint64_t np = w.range.count;
-    w.cost = p.d.KVH * (w.full * (rows.set_up(U, W) + np * W) + (rest ? rows.set_up(U, w.tail_wc) + np * w.tail_wc : 0));
+    w.cost = p.d.KVH * (w.full * (rows.set_up(U, kShare) + np * kShare) + (rest ? rows.set_up(U, w.tail_wc) + np * w.tail_wc : 0));
   }
   return w;
 }
@@ -173,12 +175,12 @@ struct Walk {
     }
     const Rows<W, NT, MODE> rows(p.G);
     const uint32_t KVH = p.d.KVH, np = w.range.count;
-    const uint64_t off = g - base, full_cost = ((uint64_t)np * W + rows.set_up(U, W)) * w.full * KVH;
+    const uint64_t off = g - base, full_cost = ((uint64_t)np * kShare + rows.set_up(U, kShare)) * w.full * KVH;
     uint32_t group, unit;
     if (MODE == kRows && off < full_cost) {
-      wc = W;
-      unit = (uint32_t)udiv(off, np * W + rows.set_up(U, W));
-      unit0 = base + (uint64_t)unit * (np * W + rows.set_up(U, W));
+      wc = kShare;
+      unit = (uint32_t)udiv(off, np * kShare + rows.set_up(U, kShare));
+      unit0 = base + (uint64_t)unit * (np * kShare + rows.set_up(U, kShare));
       group = unit / KVH;
       kvh = unit % KVH;
       nrows = rows.per_unit();
@@ -471,16 +473,21 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
     {
       constexpr int LPC = HD / 8;
       const int sub = tid / LPC, l = tid % LPC, blk = l >> 2, tt = l & 3;
-#pragma unroll 4
-      for (int c0 = 0; c0 < cols; c0 += CT / LPC) {
-        const int c = c0 + sub, tile = c / TC, cc = c % TC;
+      constexpr int AHEAD = MODE == kRows ? (Sh::COLS * LPC + CT - 1) / CT : 1;   // columns of a lane group, loaded together
+      float4 xa[AHEAD], xb[AHEAD];
+#pragma unroll
+      for (int n = 0; n < AHEAD; n++) {
+        const int c = sub + n * (CT / LPC);
         const bool on = c < cols && col_live(c);
         const float4* src = reinterpret_cast<const float4*>(
             p.q + ((size_t)(row0 + (on ? col_row(c) : 0)) * p.QH + unit.kvh * p.G + (on ? col_head(c) : 0)) * HD + 8 * l);
-        const float4 xa = src[0], xb = src[1];
-        float x[8] = {xa.x, xa.y, xa.z, xa.w, xb.x, xb.y, xb.z, xb.w};
+        xa[n] = on ? src[0] : make_float4(0.f, 0.f, 0.f, 0.f);
+        xb[n] = on ? src[1] : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
 #pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = on ? x[i] : 0.f;
+      for (int n = 0; n < AHEAD; n++) {
+        const int c = sub + n * (CT / LPC), tile = c / TC, cc = c % TC;
+        const float x[8] = {xa[n].x, xa[n].y, xa[n].z, xa[n].w, xb[n].x, xb[n].y, xb[n].z, xb[n].w};
         float m = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(x[i]));
@@ -943,6 +950,7 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
         const int c = e / (HD / 4), dim = e % (HD / 4) * 4;
         const int w0 = c / LC, lc = c % LC;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  #pragma unroll 4
         for (uint32_t i = 0; i < WS; i++) {
           const int at = (i * WC + w0) * LC + lc;
           const float a = ml[at * 2];
