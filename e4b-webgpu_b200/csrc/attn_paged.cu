@@ -5,14 +5,11 @@
 // of 16 slots that its rows can see; the work of all units, one after the other,
 // is cut into equal runs, one per CTA, so ragged lengths and few long sequences
 // alike fill the machine.  In a CTA a producer warp streams the run's pieces (one
-// bulk copy for the keys, one for the values) through a ring of stages, a lane
-// per stage, into the next units too.  The consumer warps form WS x WC: WC warps
-// share a piece, each with its own query rows, and WS such groups take pieces in
-// turn.  A unit of a few rows has WC = 1, one of a prompt's chunk WC = 2; a stage is
-// free after W arrivals, so its WC users arrive W / WC times each.  Every warp
-// keeps its own softmax state; at a unit's end the WS states are merged in shared
-// memory.  A unit cut between CTAs leaves partials in the scratch, which the last
-// CTA to arrive merges in CTA order (the same bits every time).
+// bulk copy for the keys, one for the values) through a ring of stages, a lane per
+// stage, into the next units too, and the consumer warps take pieces in turn, each
+// with its own softmax state; at a unit's end the states are merged in shared memory.
+// A unit cut between CTAs leaves partials in the scratch, which the last CTA to
+// arrive merges in CTA order (the same bits every time).
 //
 // Products, per piece and 8 MMA columns (m16n8k16, f32 accumulators):
 //   S[slot][col]  = K[slot][:] . q[:][col]      A = keys,   B = q
@@ -64,8 +61,6 @@ struct AttnP {
 // scaled p are then shared by twice the columns, for prompts' and speculated rows.
 enum { kNarrow, kWide, kRows };
 constexpr int kConsumerRegs = 224, kProducerRegs = 56;
-constexpr int kShare = 2;            // kRows: warps that share a piece at most (a larger unit's merge and partials cost more than its
-                                     // pieces' second trip from L2)
 
 template <int BITS, int HD, int MODE>
 struct Shape {
@@ -84,14 +79,13 @@ struct Shape {
   // warps (a warp then never waits for a phase before the stage's last one is done)
   static constexpr int S = W * (BITS == 16 ? (HD == 256 ? 1 : (HD == 128 ? 2 : 4)) :
                                 MODE == kRows ? (HD == 256 ? 2 : (HD == 128 ? 4 : 8)) : (HD == 256 ? 3 : (HD == 128 ? 5 : 8)));
-  // what a unit of wc sharing warps costs beside its pieces (q, the merge, the outputs),
-  // in a warp's pieces: set_up(wc)
+  // what a unit costs beside its pieces (q, the merge, the outputs), in pieces
   static constexpr int U = MODE == kRows ? 16 : (BITS == 16 ? (HD == 256 ? 6 : (HD == 128 ? 8 : 12)) : (HD == 256 ? 12 : 16));
   static constexpr int LN = S <= 32 ? S : (W == 11 ? 11 : (W == 5 ? (S == 40 ? 20 : 25) : 32));   // producer lanes; S is a multiple
   static constexpr int THREADS = MODE == kRows ? 384 : 32 * (W + 1), CT = 32 * W;
-  static constexpr int COLS = MODE == kRows ? kShare * LC : LC;         // columns (row, head) of a unit at most
+  static constexpr int COLS = LC;                                       // columns (row, head) of a unit
   static constexpr size_t PART = (size_t)COLS * (HD + 2);               // floats of a partial
-  static constexpr int TILES = (MODE == kRows ? kShare : 1) * NT, QPARTS = MODE == kRows ? 2 : 1;  // n-tiles of a unit at most; fragments of a tile
+  static constexpr int TILES = NT, QPARTS = MODE == kRows ? 2 : 1;  // n-tiles of a unit; fragments of a tile
   static constexpr size_t RING = (size_t)S * STAGE;
   // q fragments [TILES][NB][QPARTS][32] while a unit's pieces pass, then the warps' O [W][LC][HD]
   static constexpr size_t MERGE = (size_t)W * LC * HD * 4;
@@ -100,32 +94,22 @@ struct Shape {
 };
 
 // Rows and heads of a unit in n-tiles.
-template <int W, int NT, int MODE>
+template <int NT, int MODE>
 struct Rows {
   int slots;                         // columns of a row in a tile: its heads, up to a power of two (one row: 4)
   E4B_DEV explicit Rows(int G) : slots(MODE != kRows ? 4 : (G > 4 ? 8 : (G > 2 ? 4 : G))) {}
   E4B_DEV int per_tile() const { return MODE == kRows ? 8 / slots : 1; }
-  static E4B_DEV uint32_t set_up(int U, uint32_t wc) { return MODE == kRows ? U + 8 * wc : U; }
-  E4B_DEV uint32_t per_warp() const { return NT * per_tile(); }
-  E4B_DEV uint32_t per_unit() const { return per_warp() * kShare; }   // (one row: never full)
-  // warps that share a piece, for a unit of r rows: a power of two
-  E4B_DEV uint32_t sharing(uint32_t r) const {
-    uint32_t wc = 1;
-    while (wc * per_warp() < r) wc *= 2;
-    return wc;
-  }
+  E4B_DEV uint32_t per_unit() const { return NT * per_tile(); }
 };
 
 // One sequence's rows of the call, the pieces they see and what they cost.
 struct SeqWork {
   uint32_t p0, nq;                   // first row's position, rows
   PieceRange range;
-  uint32_t full, tail_wc;            // units of kShare sharing warps, sharing warps of the last unit (0: none)
-  uint64_t cost;                     // sum over units and KV heads of U + pieces * sharing warps
+  uint64_t cost;                     // sum over groups of rows and KV heads of U + pieces
 };
-template <int W, int NT, int U, int MODE>
+template <int NT, int U, int MODE>
 E4B_DEV SeqWork seq_work(const AttnP& p, int s) {
-  const Rows<W, NT, MODE> rows(p.G);
   SeqWork w;
   uint32_t r0 = (uint32_t)s, r1 = r0 + 1;
   if (p.d.rows) r0 = p.d.rows[s], r1 = min(p.d.rows[s + 1], (uint32_t)p.d.n_rows);
@@ -133,17 +117,12 @@ E4B_DEV SeqWork seq_work(const AttnP& p, int s) {
   const uint32_t len = p.d.lens[s];
   w.p0 = min(len, 0xfffffff0u - w.nq);
   w.cost = 0;
-  w.full = w.tail_wc = 0;
   if (w.nq) {
     // positions past the table are clamped: no such slot is visible
     if ((uint64_t)len + w.nq > p.d.cap) set_status(p.d.status, E4B_ST_BADINDEX);
-    const uint32_t p1 = min(w.p0 + w.nq - 1, p.d.cap - 1);
+    const uint32_t p1 = min(w.p0 + w.nq - 1, p.d.cap - 1), per = Rows<NT, MODE>(p.G).per_unit();
     w.range = piece_range(min(w.p0, p1), p1, p.window, p.sinks);
-    w.full = w.nq / rows.per_unit();
-    const uint32_t rest = w.nq % rows.per_unit();
-    w.tail_wc = rest ? rows.sharing(rest) : 0u;
-    const uint64_t np = w.range.count;
-    w.cost = p.d.KVH * (w.full * (rows.set_up(U, kShare) + np * kShare) + (rest ? rows.set_up(U, w.tail_wc) + np * w.tail_wc : 0));
+    w.cost = (uint64_t)(U + w.range.count) * p.d.KVH * (MODE == kRows ? (w.nq + per - 1) / per : 1);
   }
   return w;
 }
@@ -153,14 +132,13 @@ E4B_DEV uint64_t udiv(uint64_t a, uint64_t b) {
 }
 
 // Walks a CTA's run [g, end) of the work, unit by unit.
-template <int W, int NT, int U, int MODE>
+template <int NT, int U, int MODE>
 struct Walk {
   uint64_t g, end, base;             // base: where the current sequence's work begins
   int s;
   SeqWork w;
-  uint64_t unit0, unit1;             // the unit's work, the first `lead` of it its set-up
-  uint32_t lead;
-  uint32_t kvh, wc, nrows;           // KV head, sharing warps, rows
+  uint64_t unit0, unit1;             // the unit's work, the first U of it its set-up
+  uint32_t kvh, nrows;               // KV head, rows
   uint32_t pmin, pmax;               // positions of the unit's rows
   PieceSpan span;                    // this CTA's pieces of it
   E4B_DEV bool next(const AttnP& p) {
@@ -171,36 +149,21 @@ struct Walk {
         g = end;
         return false;
       }
-      w = seq_work<W, NT, U, MODE>(p, s);
+      w = seq_work<NT, U, MODE>(p, s);
     }
-    const Rows<W, NT, MODE> rows(p.G);
-    const uint32_t KVH = p.d.KVH, np = w.range.count;
-    const uint64_t off = g - base, full_cost = ((uint64_t)np * kShare + rows.set_up(U, kShare)) * w.full * KVH;
-    uint32_t group, unit;
-    if (MODE == kRows && off < full_cost) {
-      wc = kShare;
-      unit = (uint32_t)udiv(off, np * kShare + rows.set_up(U, kShare));
-      unit0 = base + (uint64_t)unit * (np * kShare + rows.set_up(U, kShare));
-      group = unit / KVH;
-      kvh = unit % KVH;
-      nrows = rows.per_unit();
-    } else {
-      wc = w.tail_wc;
-      kvh = (uint32_t)udiv(off - full_cost, np * wc + rows.set_up(U, wc));
-      unit0 = base + full_cost + (uint64_t)kvh * (np * wc + rows.set_up(U, wc));
-      group = w.full;
-      nrows = w.nq - group * rows.per_unit();
-    }
-    lead = rows.set_up(U, wc);
-    unit1 = unit0 + np * wc + lead;
-    pmin = w.p0 + group * rows.per_unit();
+    const uint32_t per = Rows<NT, MODE>(p.G).per_unit(), KVH = p.d.KVH, np = w.range.count;
+    const uint64_t unit = udiv(g - base, np + U);
+    const uint32_t group = MODE == kRows ? (uint32_t)udiv(unit, KVH) : 0u;
+    kvh = (uint32_t)unit - group * KVH;
+    unit0 = base + unit * (np + U);
+    unit1 = unit0 + np + U;
+    nrows = min(per, w.nq - group * per);
+    pmin = w.p0 + group * per;
     pmax = pmin + nrows - 1;
     const uint64_t stop = min(unit1, end);
     const uint32_t o0 = (uint32_t)(g - unit0), o1 = (uint32_t)(stop - unit0);
-    const int sh = 31 - __clz((int)wc);                  // wc is a power of two
-    const uint32_t k0 = o0 <= lead ? 0u : (o0 - lead + wc - 1) >> sh, k1 = o1 <= lead ? 0u : (o1 - lead + wc - 1) >> sh;
     const uint32_t p1 = min(pmax, p.d.cap - 1);
-    span = piece_span(w.range, k0, k1, min(pmin, p1), p1, p.window, p.sinks);
+    span = piece_span(w.range, o0 <= U ? 0u : o0 - U, o1 <= U ? 0u : o1 - U, min(pmin, p1), p1, p.window, p.sinks);
     g = stop;
     return true;
   }
@@ -274,10 +237,6 @@ E4B_DEV void lds_words(uint32_t (&w)[WORDS], const uint8_t* p) {
     w[0] = *reinterpret_cast<const uint32_t*>(p);
   }
 }
-E4B_DEV void mbar_arrive_n(uint64_t* b, uint32_t n) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(b)), "r"(n) : "memory");
-}
-
 __device__ __noinline__ bool wait_slow(uint64_t* b, uint32_t parity, uint32_t* status) {
   return mbar_wait(b, parity, status);
 }
@@ -290,7 +249,7 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
   static_assert(S % W == 0 && S % LN == 0 && LN <= 32 && S <= Sh::THREADS, "ring");
   constexpr int OT = HD / 16;        // m16 tiles of O
   constexpr int U = Sh::U;
-  using Unit = Walk<W, NT, U, MODE>;
+  using Unit = Walk<NT, U, MODE>;
   extern __shared__ __align__(128) uint8_t smem[];
   uint8_t* ring = smem;
   float* merge = reinterpret_cast<float*>(smem + Sh::RING);            // [W][LC][HD]
@@ -308,7 +267,7 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
 
   if (tid < S) {
     mbar_init(&landed[tid], 1);
-    mbar_init(&freed[tid], W);
+    mbar_init(&freed[tid], 1);
   }
   if (tid == 0) fence_barrier_init();
   if constexpr (BITS == 4)
@@ -320,7 +279,7 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
   SeqWork own;                       // of the thread's first sequence
   const int per = (p.d.nseq + Sh::THREADS - 1) / Sh::THREADS;
   for (int s = tid * per; s < min(p.d.nseq, (tid + 1) * per); s++) {
-    const SeqWork w = seq_work<W, NT, U, MODE>(p, s);
+    const SeqWork w = seq_work<NT, U, MODE>(p, s);
     if (s == tid * per) own = w;
     mine += w.cost;
   }
@@ -340,8 +299,8 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
     T += warp_sum_[i];
   }
   upto += before;
-  // runs of 2 U at least; an end that falls within a unit's set-up cost of its start or
-  // end moves there, so short units stay whole and no fragment is shorter than that
+  // runs of 2 U at least; an end that falls within U of a unit's start or end moves
+  // there, so short units stay whole and no fragment is shorter than U
   const uint64_t want = udiv(T, 2 * U);
   const uint32_t C = T == 0 ? 0u : (want < 1 ? 1u : (want < gridDim.x ? (uint32_t)want : gridDim.x));
   const uint32_t cta = blockIdx.x;
@@ -362,7 +321,7 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
           v.end = raw + 1;
           v.next(p);
         }
-        const uint64_t at = raw - v.unit0 < v.lead ? v.unit0 : (v.unit1 - raw < v.lead ? v.unit1 : raw);
+        const uint64_t at = raw - v.unit0 < U ? v.unit0 : (v.unit1 - raw < U ? v.unit1 : raw);
         run_end[i] = at;
         if (i == 0) {
           v.g = at;
@@ -450,24 +409,23 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
     more_units = v.next(p);
     unit = v;
     const auto run_of = [&](uint64_t x) { return (uint32_t)udiv((x + 1) * C - 1, T); };
-    const uint32_t c0 = run_of(min(v.unit0 + v.lead, v.unit1) - 1);
-    const uint32_t c1 = v.unit1 - v.unit0 < 2 * v.lead ? c0 : run_of(v.unit1 - v.lead);
+    // (an end less than U behind the unit's start moved there, one less than U before its end there)
+    const uint32_t c0 = run_of(min(v.unit0 + U, v.unit1) - 1);
+    const uint32_t c1 = v.unit1 - v.unit0 < 2 * U ? c0 : run_of(v.unit1 - U);
     unit_c0 = c0;
     unit_c1 = c1;
   };
   if (tid == 0) next_unit(u);
   consumers();
   while (more_units) {
-    const uint32_t WC = unit.wc, WS = W / WC;
-    const int wc = warp % WC, ws = warp / WC;
     const uint32_t row0 = (p.d.rows ? p.d.rows[unit.s] : (uint32_t)unit.s) + (unit.pmin - unit.w.p0);
-    const Rows<W, NT, MODE> rows(p.G);
+    const Rows<NT, MODE> rows(p.G);
     const int slots = rows.slots, per_tile = rows.per_tile();
     // column c of the unit -> row of the unit, head
     const auto col_row = [&](int c) { return c / TC * per_tile + c % TC / slots; };
     const auto col_head = [&](int c) { return c % TC % slots; };
     const auto col_live = [&](int c) { return col_head(c) < p.G && (uint32_t)col_row(c) < unit.nrows; };
-    const int cols = WC * LC;
+    constexpr int cols = LC;
 
     // ---- q as B fragments: HD/8 lanes take a column, a lane the 8 dims of one (block, t)
     {
@@ -541,7 +499,7 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
     uint32_t pos0[NT], pos1[NT], pos[NT][2], posg[NT];   // of the tile's first and last row, the lane's score columns, its p column
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
-      const int tile = wc * NT + nt;
+      const int tile = nt;
       const auto position = [&](int row) { return min(unit.pmin + row, unit.pmax); };
       pos0[nt] = position(tile * per_tile);
       pos1[nt] = position(tile * per_tile + per_tile - 1);
@@ -559,13 +517,13 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
 #pragma unroll
         for (int k = 0; k < 4; k++) O[nt][i][k] = 0.f;
     }
-    const int live_tiles = NT > 1 && (uint32_t)((wc * NT + NT - 1) * per_tile) < unit.nrows ? NT : 1;
-    const uint4* qf = qfrag + (size_t)wc * NT * NB * QP * 32 + lane;
+    const int live_tiles = NT > 1 && (uint32_t)((NT - 1) * per_tile) < unit.nrows ? NT : 1;
+    const uint4* qf = qfrag + lane;
 
     const PieceSpan span = unit.span;
-    const uint32_t turn = j0 % WS;   // group (j % WS) takes the CTA's piece j
+    const uint32_t turn = j0 % W;    // warp j % W takes the CTA's piece j
     bool fresh = true;               // O is zero
-    const uint32_t i0 = (uint32_t)ws >= turn ? ws - turn : ws + WS - turn;
+    const uint32_t i0 = (uint32_t)warp >= turn ? warp - turn : warp + W - turn;
     uint32_t st = (j0 + i0) % S, phase = (j0 + i0) / S & 1u;
     // a piece's work for the warp's first N tiles (the others hold no row)
     const auto work = [&](auto tiles, const uint8_t* kp, const uint8_t* vp, uint32_t t0, bool here) {
@@ -582,7 +540,7 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
         const uint32_t dz1 = t < NB / 2 ? *reinterpret_cast<const uint32_t*>(kp + (g + 8) * NB * 2 + t * 4) : 0u;
 #pragma unroll
         for (int nt = 0; nt < N; nt++) {
-          const uint2 zb = qzero[(wc * NT + nt) * 32 + lane];
+          const uint2 zb = qzero[nt * 32 + lane];
           mma16816_zero(z[nt], dz0, dz1, dz0, dz1, zb.x, zb.y);
 #pragma unroll
           for (int k = 0; k < 4; k++) s[nt][k] = 0.f;
@@ -849,7 +807,7 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
         }
       }
     };
-    for (uint32_t i = i0; i < span.count; i += WS) {
+    for (uint32_t i = i0; i < span.count; i += W) {
       const uint32_t t0 = span.at(i) * kPieceSlots;
       if (!__all_sync(0xffffffffu, mbar_try_wait(&landed[st], phase)) && alive)
         alive = __all_sync(0xffffffffu, wait_slow(&landed[st], phase, p.d.status));
@@ -860,9 +818,9 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
       if (live_tiles == NT) work(std::integral_constant<int, NT>{}, kp, vp, t0, here);
       else work(std::integral_constant<int, 1>{}, kp, vp, t0, here);
       __syncwarp();
-      if (lane == 0 && alive) mbar_arrive_n(&freed[st], WS);
+      if (lane == 0 && alive) mbar_arrive(&freed[st]);
       fresh = false;
-      st += WS;
+      st += W;
       if (st >= (uint32_t)S) st -= S, phase ^= 1u;
     }
     j0 += unit.span.count;
@@ -928,12 +886,13 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
     };
     float* part = p.parts + (2 * (size_t)cta + (cta == c0 ? 1 : 0)) * Sh::PART;  // a run ends with at most one cut unit, and begins with one
     if constexpr (MODE == kRows) {
-      for (int c = tid; c < cols; c += CT) {               // the weights of the WS states of each column
-        const int w0 = c / LC, lc = c % LC;
+      for (int c = tid; c < cols; c += CT) {             // the weights of the warps' states of each column
         float M = -INFINITY, L = 0.f;
-        for (uint32_t i = 0; i < WS; i++) M = fmaxf(M, ml[((i * WC + w0) * LC + lc) * 2]);
-        for (uint32_t i = 0; i < WS; i++) {
-          float* at = ml + ((i * WC + w0) * LC + lc) * 2;
+#pragma unroll
+        for (int i = 0; i < W; i++) M = fmaxf(M, ml[(i * LC + c) * 2]);
+#pragma unroll
+        for (int i = 0; i < W; i++) {
+          float* at = ml + (i * LC + c) * 2;
           const float a = at[0] == M ? 1.f : ex2(at[0] - M);
           L = fmaf(a, at[1], L);
           at[0] = a;
@@ -942,17 +901,17 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
         if (!col_live(c)) r = 0.f;
         else if (whole) r = close_column(c, M, L);
         else *reinterpret_cast<float2*>(part + Sh::COLS * HD + 2 * c) = make_float2(M, L);
-        for (uint32_t i = 0; i < WS; i++) ml[((i * WC + w0) * LC + lc) * 2] *= r;
+#pragma unroll
+        for (int i = 0; i < W; i++) ml[(i * LC + c) * 2] *= r;
       }
       consumers();
-#pragma unroll 4
+#pragma unroll 2
       for (int e = tid; e < cols * (HD / 4); e += CT) {
         const int c = e / (HD / 4), dim = e % (HD / 4) * 4;
-        const int w0 = c / LC, lc = c % LC;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  #pragma unroll 4
-        for (uint32_t i = 0; i < WS; i++) {
-          const int at = (i * WC + w0) * LC + lc;
+#pragma unroll
+        for (int i = 0; i < W; i++) {
+          const int at = i * LC + c;
           const float a = ml[at * 2];
           const float4 x = *reinterpret_cast<const float4*>(merge + (size_t)at * HD + dim);
           o.x = fmaf(a, x.x, o.x), o.y = fmaf(a, x.y, o.y), o.z = fmaf(a, x.z, o.z), o.w = fmaf(a, x.w, o.w);
