@@ -106,7 +106,8 @@ struct Rows {
 struct SeqWork {
   uint32_t p0, nq;                   // first row's position, rows
   PieceRange range;
-  uint64_t cost;                     // sum over groups of rows and KV heads of U + pieces
+  uint32_t units;                    // groups of rows times KV heads
+  uint64_t cost;                     // U + pieces, for each unit
 };
 template <int NT, int U, int MODE>
 E4B_DEV SeqWork seq_work(const AttnP& p, int s) {
@@ -116,13 +117,15 @@ E4B_DEV SeqWork seq_work(const AttnP& p, int s) {
   w.nq = r1 > r0 ? r1 - r0 : 0u;
   const uint32_t len = p.d.lens[s];
   w.p0 = min(len, 0xfffffff0u - w.nq);
+  w.units = 0;
   w.cost = 0;
   if (w.nq) {
     // positions past the table are clamped: no such slot is visible
     if ((uint64_t)len + w.nq > p.d.cap) set_status(p.d.status, E4B_ST_BADINDEX);
     const uint32_t p1 = min(w.p0 + w.nq - 1, p.d.cap - 1), per = Rows<NT, MODE>(p.G).per_unit();
     w.range = piece_range(min(w.p0, p1), p1, p.window, p.sinks);
-    w.cost = (uint64_t)(U + w.range.count) * p.d.KVH * (MODE == kRows ? (w.nq + per - 1) / per : 1);
+    w.units = p.d.KVH * (MODE == kRows ? (w.nq + per - 1) / per : 1u);
+    w.cost = (uint64_t)(U + w.range.count) * w.units;
   }
   return w;
 }
@@ -257,6 +260,7 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
   __shared__ uint64_t landed[S], freed[S];
   __shared__ int usable[S];
   __shared__ uint64_t warp_sum_[Sh::THREADS / 32];
+  __shared__ uint32_t warp_units[Sh::THREADS / 32];
   __shared__ uint2 qzero[BITS == 4 ? Sh::TILES * 32 : 32];               // B of the -8 term: -8 sum q per block, hi and lo
   __shared__ float qfac[Sh::TILES * TC];
   __shared__ float ml[W * LC * 2];
@@ -276,12 +280,14 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
 
   // ---- the run of this CTA: the work of all units, cut evenly
   uint64_t mine = 0;
+  uint32_t units = 0;
   SeqWork own;                       // of the thread's first sequence
   const int per = (p.d.nseq + Sh::THREADS - 1) / Sh::THREADS;
   for (int s = tid * per; s < min(p.d.nseq, (tid + 1) * per); s++) {
     const SeqWork w = seq_work<NT, U, MODE>(p, s);
     if (s == tid * per) own = w;
     mine += w.cost;
+    units += w.units;
   }
   if (blockIdx.x == 0) live_rows(p.d);                   // records a row count past n_rows
   uint64_t upto = mine;                                  // inclusive sum over the threads
@@ -290,18 +296,21 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
     const uint64_t v = __shfl_up_sync(0xffffffffu, upto, o);
     if (lane >= o) upto += v;
   }
-  if (lane == 31) warp_sum_[warp] = upto;
+  units = __reduce_add_sync(0xffffffffu, min(units, 0xffffffu));
+  if (lane == 31) warp_sum_[warp] = upto, warp_units[warp] = units;
   __syncthreads();
   uint64_t before = 0, T = 0;
+  units = 0;
 #pragma unroll
   for (int i = 0; i < Sh::THREADS / 32; i++) {
     if (i < warp) before += warp_sum_[i];
     T += warp_sum_[i];
+    units += warp_units[i];
   }
   upto += before;
-  // runs of 2 U at least; an end that falls within U of a unit's start or end moves
+  // runs of 2 U at least, or a unit's length (no two on a CTA while others idle); an end that falls within U of a unit's start or end moves
   // there, so short units stay whole and no fragment is shorter than U
-  const uint64_t want = udiv(T, 2 * U);
+  const uint64_t want = max(udiv(T, 2 * U), min((uint64_t)units, udiv(T, U)));
   const uint32_t C = T == 0 ? 0u : (want < 1 ? 1u : (want < gridDim.x ? (uint32_t)want : gridDim.x));
   const uint32_t cta = blockIdx.x;
   if (cta >= C) return;
