@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
   __shared__ uint64_t landed[S], freed[S];
   __shared__ int usable[S];
   __shared__ uint64_t warp_sum_[Sh::THREADS / 32];
-  __shared__ uint32_t warp_units[Sh::THREADS / 32];
+  __shared__ uint32_t warp_units[Sh::THREADS / 32], warp_longest[Sh::THREADS / 32];
   __shared__ uint2 qzero[BITS == 4 ? Sh::TILES * 32 : 32];               // B of the -8 term: -8 sum q per block, hi and lo
   __shared__ float qfac[Sh::TILES * TC];
   __shared__ float ml[W * LC * 2];
@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
 
   // ---- the run of this CTA: the work of all units, cut evenly
   uint64_t mine = 0;
-  uint32_t units = 0;
+  uint32_t units = 0, longest = 0;
   SeqWork own;                       // of the thread's first sequence
   const int per = (p.d.nseq + Sh::THREADS - 1) / Sh::THREADS;
   for (int s = tid * per; s < min(p.d.nseq, (tid + 1) * per); s++) {
@@ -288,6 +288,7 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
     if (s == tid * per) own = w;
     mine += w.cost;
     units += w.units;
+    if (w.units) longest = max(longest, w.range.count + U);
   }
   if (blockIdx.x == 0) live_rows(p.d);                   // records a row count past n_rows
   uint64_t upto = mine;                                  // inclusive sum over the threads
@@ -297,7 +298,8 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
     if (lane >= o) upto += v;
   }
   units = __reduce_add_sync(0xffffffffu, min(units, 0xffffffu));
-  if (lane == 31) warp_sum_[warp] = upto, warp_units[warp] = units;
+  longest = __reduce_max_sync(0xffffffffu, longest);
+  if (lane == 31) warp_sum_[warp] = upto, warp_units[warp] = units, warp_longest[warp] = longest;
   __syncthreads();
   uint64_t before = 0, T = 0;
   units = 0;
@@ -306,12 +308,17 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
     if (i < warp) before += warp_sum_[i];
     T += warp_sum_[i];
     units += warp_units[i];
+    longest = max(longest, warp_longest[i]);
   }
   upto += before;
-  // runs of 2 U at least, or a unit's length (no two on a CTA while others idle); an end that falls within U of a unit's start or end moves
-  // there, so short units stay whole and no fragment is shorter than U
+  // Runs of 2 U at least, or a unit's length (no two on a CTA while others idle); an end
+  // that falls within U of a unit's start or end moves there, so short units stay whole
+  // and no fragment is shorter than U.  Units of about one length, and nearly as many as
+  // CTAs, are not cut at all: an end then moves to the nearer one.
+  const bool uncut = units <= gridDim.x && 10 * units >= 7 * gridDim.x && 20 * (uint64_t)longest * units <= 23 * T;
   const uint64_t want = max(udiv(T, 2 * U), min((uint64_t)units, udiv(T, U)));
-  const uint32_t C = T == 0 ? 0u : (want < 1 ? 1u : (want < gridDim.x ? (uint32_t)want : gridDim.x));
+  const uint32_t C = T == 0 ? 0u : (uncut ? units : (want < 1 ? 1u : (want < gridDim.x ? (uint32_t)want : gridDim.x)));
+  const auto reach = [&](const Unit& v) { return uncut ? (uint32_t)(v.unit1 - v.unit0) / 2 + 1 : (uint32_t)U; };
   const uint32_t cta = blockIdx.x;
   if (cta >= C) return;
   __shared__ uint64_t run_end[2];
@@ -330,7 +337,7 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
           v.end = raw + 1;
           v.next(p);
         }
-        const uint64_t at = raw - v.unit0 < U ? v.unit0 : (v.unit1 - raw < U ? v.unit1 : raw);
+        const uint64_t at = raw - v.unit0 < reach(v) ? v.unit0 : (v.unit1 - raw < reach(v) ? v.unit1 : raw);
         run_end[i] = at;
         if (i == 0) {
           v.g = at;
@@ -418,9 +425,9 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
     more_units = v.next(p);
     unit = v;
     const auto run_of = [&](uint64_t x) { return (uint32_t)udiv((x + 1) * C - 1, T); };
-    // (an end less than U behind the unit's start moved there, one less than U before its end there)
-    const uint32_t c0 = run_of(min(v.unit0 + U, v.unit1) - 1);
-    const uint32_t c1 = v.unit1 - v.unit0 < 2 * U ? c0 : run_of(v.unit1 - U);
+    // (a run's end less than `reach` behind the unit's start moved there, one less before its end there)
+    const uint32_t F = reach(v), c0 = run_of(min(v.unit0 + F, v.unit1) - 1);
+    const uint32_t c1 = v.unit1 - v.unit0 < 2 * F ? c0 : run_of(v.unit1 - F);
     unit_c0 = c0;
     unit_c1 = c1;
   };
