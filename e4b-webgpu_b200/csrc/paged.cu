@@ -446,7 +446,7 @@ __global__ void __launch_bounds__(128) k_kvread_paged(const PagedDev d, void* k_
         const int q0 = BITS == 4 && is_v ? (w >> 3) * 16 + (w & 7) : 2 * w, q1 = BITS == 4 && is_v ? q0 + 8 : 2 * w + 1;
         const uint8_t* piece = pool + (uint64_t)head_bytes * h;
         uint32_t y[4] = {0u, 0u, 0u, 0u};                // the two quads as f16 pairs
-        float sc[2] = {0.f, 0.f};
+        uint16_t sc[2] = {0, 0};
         uint32_t codes = 0x88888888u;
         if (pl.ok) {
           if constexpr (BITS == 16) {
@@ -454,29 +454,36 @@ __global__ void __launch_bounds__(128) k_kvread_paged(const PagedDev d, void* k_
             y[0] = v.x, y[1] = v.y, y[2] = v.z, y[3] = v.w;
           } else {
             codes = *reinterpret_cast<const uint32_t*>(piece + (is_v ? v4_quad(s, q0, HD) : k4_quad(s, q0, HD)));
-            sc[0] = h2f(*reinterpret_cast<const uint16_t*>(piece + (is_v ? v4_scale(s, q0 / 8, HD) : k4_scale(s, q0 / 8, HD))));
-            sc[1] = is_v ? h2f(*reinterpret_cast<const uint16_t*>(piece + v4_scale(s, q1 / 8, HD))) : sc[0];
+            sc[0] = *reinterpret_cast<const uint16_t*>(piece + (is_v ? v4_scale(s, q0 / 8, HD) : k4_scale(s, q0 / 8, HD)));
+            sc[1] = is_v ? *reinterpret_cast<const uint16_t*>(piece + v4_scale(s, q1 / 8, HD)) : sc[0];
           }
         }
         const size_t o0 = at + (size_t)h * HD + 4 * q0, o1 = at + (size_t)h * HD + 4 * q1;
-        if (BITS == 16 && !out_f32) {
-          *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + o0) = make_uint4(y[0], y[1], y[2], y[3]);
+        if (!out_f32) {
+          uint16_t* const to = static_cast<uint16_t*>(out);
+          if constexpr (BITS == 16) {
+            *reinterpret_cast<uint4*>(to + o0) = make_uint4(y[0], y[1], y[2], y[3]);
+          } else {
+            // pairs (code j of the first quad, of the second) as f16 n - 8, times (d, d): the
+            // product has 15 bits, so its f16 is the value's
+            const __half2 d2 = as_h2(sc[0] | (uint32_t)sc[1] << 16);
+            uint32_t x[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+              x[j] = as_u32(__hmul2(__hsub2(as_h2(((codes >> (4 * j)) & 0x000F000Fu) | 0x64006400u), as_h2(0x64086408u)), d2));
+            *reinterpret_cast<uint2*>(to + o0) = make_uint2(__byte_perm(x[0], x[1], 0x5410), __byte_perm(x[2], x[3], 0x5410));
+            *reinterpret_cast<uint2*>(to + o1) = make_uint2(__byte_perm(x[0], x[1], 0x7632), __byte_perm(x[2], x[3], 0x7632));
+          }
           continue;
         }
         float x[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) {
           if constexpr (BITS == 16) x[j] = h2f((uint16_t)(y[j >> 1] >> (16 * (j & 1))));
-          else x[j] = sc[j >> 2] * (float)((int)((codes >> (4 * j)) & 15u) - 8);
+          else x[j] = h2f(sc[j >> 2]) * (float)((int)((codes >> (4 * j)) & 15u) - 8);
         }
-        if (out_f32) {
-          *reinterpret_cast<float4*>(static_cast<float*>(out) + o0) = make_float4(x[0], x[1], x[2], x[3]);
-          *reinterpret_cast<float4*>(static_cast<float*>(out) + o1) = make_float4(x[4], x[5], x[6], x[7]);
-        } else {
-          const uint2 a = make_uint2(pack2(x[0], x[1]), pack2(x[2], x[3])), b = make_uint2(pack2(x[4], x[5]), pack2(x[6], x[7]));
-          *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + o0) = a;
-          *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + o1) = b;
-        }
+        *reinterpret_cast<float4*>(static_cast<float*>(out) + o0) = make_float4(x[0], x[1], x[2], x[3]);
+        *reinterpret_cast<float4*>(static_cast<float*>(out) + o1) = make_float4(x[4], x[5], x[6], x[7]);
       }
     }
   }
