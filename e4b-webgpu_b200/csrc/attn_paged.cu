@@ -424,7 +424,7 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
   const auto next_unit = [&](Unit& v) {                  // thread 0; with the CTAs whose runs hold the unit, c0..c1
     more_units = v.next(p);
     unit = v;
-    const auto run_of = [&](uint64_t x) { return (uint32_t)udiv((x + 1) * C - 1, T); };
+    const auto run_of = [&](uint64_t x) { return min((uint32_t)udiv((x + 1) * C - 1, T), C - 1); };
     // (a run's end less than `reach` behind the unit's start moved there, one less before its end there)
     const uint32_t F = reach(v), c0 = run_of(min(v.unit0 + F, v.unit1) - 1);
     const uint32_t c1 = v.unit1 - v.unit0 < 2 * F ? c0 : run_of(v.unit1 - F);
@@ -1014,58 +1014,58 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
               if (dim == 0) *reinterpret_cast<float2*>(part_of(a) + Sh::COLS * HD + 2 * c) = make_float2(M, L);
             }
           }
-          return;
-        }
-        for (int c = tid; c < cols; c += CT) {           // the parts' weights
-          float M = -INFINITY, L = 0.f;
-          for (uint32_t i = 0; i < n; i++) M = fmaxf(M, part_ml[i * cols + c].x);
-          for (uint32_t i = 0; i < n; i++) {
-            float2& y = part_ml[i * cols + c];
-            y.x = y.x == M ? 1.f : ex2(y.x - M);
-            L = fmaf(y.x, y.y, L);
-          }
-          if (!col_live(c)) continue;
-          if (final) {
-            const float r = close_column(c, M, L);
-            for (uint32_t i = 0; i < n; i++) part_ml[i * cols + c].x *= r;
-          } else {
-            *reinterpret_cast<float2*>(part_of(a) + Sh::COLS * HD + 2 * c) = make_float2(M, L);
-          }
-        }
-        consumers();
-        constexpr int kE = 4, kI = 2;    // eight loads in flight
-        for (int e0 = tid; e0 < cols * (HD / 4); e0 += kE * CT) {
-          float4 o[kE];
-#pragma unroll
-          for (int j = 0; j < kE; j++) o[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 1
-          for (uint32_t i0 = 0; i0 < n; i0 += kI) {
-            float4 x[kI][kE];
-#pragma unroll
-            for (int i = 0; i < kI; i++)
-#pragma unroll
-              for (int j = 0; j < kE; j++) {
-                const int e = min(e0 + j * CT, cols * (HD / 4) - 1);
-                x[i][j] = __ldcg(reinterpret_cast<const float4*>(part_of(a + min(i0 + i, n - 1) * step)) + e);
-              }
-#pragma unroll
-            for (int i = 0; i < kI; i++) {
-              if (i0 + i >= n) continue;
-#pragma unroll
-              for (int j = 0; j < kE; j++) {
-                const int e = min(e0 + j * CT, cols * (HD / 4) - 1);
-                const float f = part_ml[(i0 + i) * cols + e / (HD / 4)].x;
-                o[j].x = fmaf(f, x[i][j].x, o[j].x), o[j].y = fmaf(f, x[i][j].y, o[j].y);
-                o[j].z = fmaf(f, x[i][j].z, o[j].z), o[j].w = fmaf(f, x[i][j].w, o[j].w);
-              }
+        } else {
+          for (int c = tid; c < cols; c += CT) {           // the parts' weights
+            float M = -INFINITY, L = 0.f;
+            for (uint32_t i = 0; i < n; i++) M = fmaxf(M, part_ml[i * cols + c].x);
+            for (uint32_t i = 0; i < n; i++) {
+              float2& y = part_ml[i * cols + c];
+              y.x = y.x == M ? 1.f : ex2(y.x - M);
+              L = fmaf(y.x, y.y, L);
+            }
+            if (!col_live(c)) continue;
+            if (final) {
+              const float r = close_column(c, M, L);
+              for (uint32_t i = 0; i < n; i++) part_ml[i * cols + c].x *= r;
+            } else {
+              *reinterpret_cast<float2*>(part_of(a) + Sh::COLS * HD + 2 * c) = make_float2(M, L);
             }
           }
+          consumers();
+          constexpr int kE = 4, kI = 2;    // eight loads in flight
+          for (int e0 = tid; e0 < cols * (HD / 4); e0 += kE * CT) {
+            float4 o[kE];
 #pragma unroll
-          for (int j = 0; j < kE; j++) {
-            const int e = e0 + j * CT, c = e / (HD / 4);
-            if (e >= cols * (HD / 4) || !col_live(c)) continue;
-            if (final) store(c, e % (HD / 4) * 4, o[j]);
-            else *(reinterpret_cast<float4*>(part_of(a)) + e) = o[j];
+            for (int j = 0; j < kE; j++) o[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+            for (uint32_t i0 = 0; i0 < n; i0 += kI) {
+              float4 x[kI][kE];
+#pragma unroll
+              for (int i = 0; i < kI; i++)
+#pragma unroll
+                for (int j = 0; j < kE; j++) {
+                  const int e = min(e0 + j * CT, cols * (HD / 4) - 1);
+                  x[i][j] = __ldcg(reinterpret_cast<const float4*>(part_of(a + min(i0 + i, n - 1) * step)) + e);
+                }
+#pragma unroll
+              for (int i = 0; i < kI; i++) {
+                if (i0 + i >= n) continue;
+#pragma unroll
+                for (int j = 0; j < kE; j++) {
+                  const int e = min(e0 + j * CT, cols * (HD / 4) - 1);
+                  const float f = part_ml[(i0 + i) * cols + e / (HD / 4)].x;
+                  o[j].x = fmaf(f, x[i][j].x, o[j].x), o[j].y = fmaf(f, x[i][j].y, o[j].y);
+                  o[j].z = fmaf(f, x[i][j].z, o[j].z), o[j].w = fmaf(f, x[i][j].w, o[j].w);
+                }
+              }
+            }
+#pragma unroll
+            for (int j = 0; j < kE; j++) {
+              const int e = e0 + j * CT, c = e / (HD / 4);
+              if (e >= cols * (HD / 4) || !col_live(c)) continue;
+              if (final) store(c, e % (HD / 4) * 4, o[j]);
+              else *(reinterpret_cast<float4*>(part_of(a)) + e) = o[j];
+            }
           }
         }
       };

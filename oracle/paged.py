@@ -38,7 +38,7 @@ def scale_place(HD: int, value: bool):
 
 def quantise(x16: np.ndarray):
     """f16 rows [..., HD] -> (codes 0..15, f16 scale per 32 dims): the q4_0 rule with a true division."""
-    b = x16.astype(F64).reshape(*x16.shape[:-1], -1, 32)
+    b = x16.astype(F64).reshape(*x16.shape[:-1], x16.shape[-1] // 32, 32)
     with np.errstate(all="ignore"):
         at = np.abs(b).argmax(-1)
         d = np.take_along_axis(b, at[..., None], -1) / -8.0
@@ -50,7 +50,7 @@ def quantise(x16: np.ndarray):
 
 
 def dequantise(q, d16):
-    b = (q - 8.0).reshape(*q.shape[:-1], -1, 32) * d16.astype(F64)[..., None]
+    b = (q - 8.0).reshape(*q.shape[:-1], q.shape[-1] // 32, 32) * d16.astype(F64)[..., None]
     return b.reshape(q.shape)
 
 
@@ -80,6 +80,27 @@ class Pool:
             words = (q.reshape(-1, 4) << np.array([0, 4, 8, 12])).sum(-1)
             w[b + self.at[s][::4] // 2] = words.astype(np.uint16)
             w[b + self.at_d[s] // 2] = d.view(np.uint16)
+
+    def write_all(self, pageids, slots, rows16):
+        """As write, for tokens [n]: rows16 [n][KVH][HD]."""
+        w, s = self.raw.view(np.uint16), slots % 16
+        b = self._word(pageids[:, None], np.arange(self.KVH)[None], slots[:, None])[..., None]
+        if self.bits == 16:
+            w[b + self.at[s][:, None] // 2] = rows16.astype(np.float16).view(np.uint16)
+            return
+        q, d = quantise(rows16.astype(np.float16))
+        words = (q.reshape(*q.shape[:-1], q.shape[-1] // 4, 4) << np.array([0, 4, 8, 12])).sum(-1)
+        w[b + self.at[s][:, None, ::4] // 2] = words.astype(np.uint16)
+        w[b + self.at_d[s][:, None] // 2] = d.view(np.uint16)
+
+    def read_all(self, pageids, slots):
+        """As read, for tokens [n]: [n][KVH][HD] in 64 bits."""
+        w, s = self.raw.view(np.uint16), slots % 16
+        b = self._word(pageids[:, None], np.arange(self.KVH)[None], slots[:, None])[..., None]
+        x = w[b + self.at[s][:, None] // 2]
+        if self.bits == 16:
+            return x.view(np.float16).astype(F64)
+        return dequantise(((x >> self.shift[s][:, None]) & 15).astype(F64), w[b + self.at_d[s][:, None] // 2].view(np.float16))
 
     def read(self, pageid, slot):
         """[KVH][HD] in 64 bits."""

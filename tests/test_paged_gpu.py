@@ -54,7 +54,7 @@ class Cache:
     def pools(self, fill=0xff):
         return [op.Pool(self.bits, self.page, self.n_pages, self.KVH, self.HD, v, fill) for v in (False, True)]
 
-    def fill(self, rng, upto=None, scale=1.0):
+    def fill(self, rng, upto=None, scale=1.0, grow=0.0):
         """Random keys and values at every position below lens + counts, through the numpy layout; returns what the
         pages stand for, per sequence [slots][KVH][HD] in 64 bits."""
         pk, pv = self.pools()
@@ -62,12 +62,14 @@ class Cache:
         for s in range(self.nseq):
             n = self.lens[s] + self.counts[s] if upto is None else upto[s]
             kk, vv = np.zeros((n, self.KVH, self.HD)), np.zeros((n, self.KVH, self.HD))
-            x = (rng.standard_normal((n, 2, self.KVH, self.HD)) * scale).astype(np.float16)
-            for t in range(n):
-                pid = int(self.table[s, t // self.page])
-                pk.write(pid, t % self.page, x[t, 0])
-                pv.write(pid, t % self.page, x[t, 1])
-                kk[t], vv[t] = pk.read(pid, t % self.page), pv.read(pid, t % self.page)
+            x = rng.standard_normal((n, 2, self.KVH, self.HD)) * scale
+            if grow:                                     # values that grow along the sequence
+                x[:, 1] *= np.linspace(1, grow, n)[:, None, None]
+            x, t = x.astype(np.float16), np.arange(n)
+            pid = self.table[s, t // self.page].astype(np.int64)
+            pk.write_all(pid, t % self.page, x[:, 0])
+            pv.write_all(pid, t % self.page, x[:, 1])
+            kk[:], vv[:] = pk.read_all(pid, t % self.page), pv.read_all(pid, t % self.page)
             out.append((kk, vv))
         self.dev.write(self.kv.struct.k, pk.raw)
         self.dev.write(self.kv.struct.v, pv.raw)
@@ -97,7 +99,7 @@ def attend(c, scratch, q, QH, *, window=0, sinks=0, scale=1.0, xfo=0, dev=None):
     c.e4b.ops.attn_paged(dev, c.kv, dev.upload(q.astype(F32)), oh, of, lse, scratch, Q_HEADS=QH, WINDOW=window, SINKS=sinks,
                          SCALE=scale, XFO=xfo, ROWS=c.n_rows)
     dev.sync()
-    return (dev.read(oh, np.float16, n).reshape(c.n_rows, -1), dev.read(of, F32, n).reshape(c.n_rows, QH, c.HD),
+    return (dev.read(oh, np.float16, n).reshape(c.n_rows, QH * c.HD), dev.read(of, F32, n).reshape(c.n_rows, QH, c.HD),
             dev.read(lse, F32, c.n_rows * QH).reshape(c.n_rows, QH))
 
 
@@ -137,6 +139,17 @@ APPEND = [  # bits, HD, QH, KVH, page, lens, counts, options
     (4, 256, 0, 2, 16, [9], [20], dict(stride=64)),
     (4, 128, 8, 8, 16, [70000, 131], [3, 2], dict(nparts=3)),
     (16, 256, 16, 4, 64, [100000], [4], dict(stride=4, theta=1e6)),
+    # many rows: whole rows by bulk copies, or (partial sums, rows of 8-byte alignment or over 48 KB) by loads;
+    # several turns and look-ups a CTA, sequences that begin and end within one
+    (4, 64, 1, 1, 16, [0, 5, 100000, 3, 9, 31], [7000, 0, 13, 6487, 1, 7000], dict(half=1)),
+    (4, 64, 1, 1, 32, [0, 5, 100000, 3, 9, 31], [7000, 0, 13, 6487, 1, 7000], dict(nparts=2)),
+    (16, 256, 8, 2, 64, [0, 77, 1000], [333, 1, 400], dict(pad=9)),
+    (4, 128, 16, 2, 16, [5, 0], [700, 640], dict(half=1, offset=8)),
+    (4, 256, 64, 2, 64, [0, 9], [100, 90], {}),
+    (4, 256, 40, 4, 16, [0], [200], {}),
+    (16, 64, 14, 2, 48, [3], [801], dict(half=1, keqv=1, frac=0.3, stride=4, norm=0)),
+    (16, 64, 14, 2, 48, [3], [801], dict(half=1, keqv=1, frac=0.3, stride=8, theta=1e6)),
+    (4, 128, 0, 6, 16, [0] * 900, [1] * 900, {}),
 ]
 
 
@@ -154,7 +167,9 @@ def test_append_and_read_back(e4b, dev, case):
     x = rng.standard_normal((nparts, c.n_rows, stride)).astype(np.float16 if half else F32)
     qw, kw = (1 + 0.2 * rng.standard_normal(HD)).astype(F32), (1 + 0.2 * rng.standard_normal(HD)).astype(F32)
     bq = dev.upload(np.full(max(1, c.n_rows * QH * HD), 9, F32))
-    args = (dev.upload(x), dev.upload(qw), dev.upload(kw), bq if QH else None)
+    off = o.get("offset", 0) // x.itemsize
+    bx = dev.upload(np.concatenate([np.zeros(off, x.dtype), x.ravel()]))
+    args = (bx.ptr + off * x.itemsize, dev.upload(qw), dev.upload(kw), bq if QH else None)
     kws = dict(QH=QH, ROPE_ANGLES=angles, THETA=theta, NORM=norm, KEQV=keqv, XF16=half, NPARTS=nparts, ROWS=c.n_rows,
                STRIDE=stride if o.get("stride") else 0)
     e4b.ops.headprep_paged(dev, c.kv, *args, **kws)
@@ -184,14 +199,34 @@ def test_append_and_read_back(e4b, dev, case):
         for g, x16 in ((got_k, k16), (got_v, v16)):
             assert np.array_equal(g[:c.n].astype(F64), op.dequantise(*op.quantise(x16[:c.n].astype(np.float16))))
     pools = c.pools()
-    for r in range(c.n):
-        s, p = c.place(r)
-        for pool, x16 in zip(pools, (k16, v16)):
-            pool.write(int(c.table[s, p // page]), p % page, x16[r])
+    seqs, at = np.array([c.place(r)[0] for r in range(c.n)]), np.array(pos)
+    for pool, x16 in zip(pools, (k16, v16)):
+        pool.write_all(c.table[seqs, at // page].astype(np.int64), at % page, x16[:c.n])
     for pool, ptr in zip(pools, (c.kv.struct.k, c.kv.struct.v)):   # every other byte is what it was
         assert np.array_equal(dev.read(ptr, np.uint8, c.kv.pool_bytes), pool.raw)
     k2, v2 = c.read_rows(f32=0)
     assert np.array_equal(k2[:c.n], got_k[:c.n].astype(np.float16)) and np.array_equal(v2[:c.n], got_v[:c.n].astype(np.float16))
+
+
+def test_codes_between_two_and_of_two_largest(e4b, dev):
+    """Blocks of halves and small integers (quotients exactly between two codes, largest magnitudes of both signs in
+    either order, repeated), of f16's smallest and largest values, and random ones, code by code."""
+    rng = np.random.default_rng(4)
+    HD, n = 128, 1500                                    # (few rows and many use one quantiser; this is the staged path)
+    x = rng.integers(-16, 17, (n, 2, HD)) * 0.5
+    x[300:600] = rng.integers(-3, 4, (300, 2, HD))
+    x[600:700] *= 2.0 ** -24 * 2
+    x[700:800] = rng.choice([65504.0, -65504.0, 32752.0, 4094.0], (100, 2, HD))
+    x[800:] = rng.standard_normal((700, 2, HD)) * 2.0 ** rng.integers(-20, 12, (700, 1, 1))
+    x16 = x.astype(np.float16)
+    c = Cache(e4b, dev, [0], [n], bits=4, page=64, KVH=1, HD=HD, ragged=True)
+    e4b.ops.headprep_paged(dev, c.kv, dev.upload(x16), None, None, None, QH=0, ROPE_ANGLES=0, THETA=1e4, NORM=0, XF16=1,
+                           ROWS=n)
+    assert dev.status() == 0
+    for ptr, pool, i in zip((c.kv.struct.k, c.kv.struct.v), c.pools(), (0, 1)):
+        t = np.arange(n)
+        pool.write_all(c.table[0, t // 64].astype(np.int64), t % 64, x16[:, i:i + 1])
+        assert np.array_equal(dev.read(ptr, np.uint8, c.kv.pool_bytes), pool.raw)
 
 
 def test_append_of_infinities_and_zeros(e4b, dev):
@@ -376,6 +411,124 @@ def test_many_short_sequences_and_a_long_one(e4b, dev, scratch):
     got = attend(c, scratch, q, 2)
     assert dev.status() == 0
     check_rows(c, held, q, got, 2, 0, 0, 1.0)
+
+
+SHAPES = {  # lens, counts, QH, KVH: which rows, heads and lengths choose the kernel's forms and how its work is cut
+    "two CTAs per SM": (lambda r: [int(x) for x in r.integers(0, 260, 40)], [1] * 40, 16, 4),
+    "equal units, two CTAs per SM": (lambda r: [200] * 64, [1] * 64, 8, 4),
+    "equal units, one CTA per SM": (lambda r: [333] * 40, [1] * 40, 6, 3),
+    "nearly equal units": (lambda r: [int(x) for x in 300 + r.integers(0, 16, 35)], [1] * 35, 16, 4),
+    "long and short": (lambda r: [9000, 7], [1, 1], 3, 1),
+    "long, 8 heads": (lambda r: [0, 9000], [1, 1], 8, 1),
+    "long, rows": (lambda r: [8000, 3], [9, 40], 7, 1),
+    "prompts": (lambda r: [0, 100, 0, 31], [130, 70, 0, 1], 4, 2),
+    "equal prompts": (lambda r: [64] * 10, [16] * 10, 8, 2),
+    "short rows of one head": (lambda r: [5] * 50, [3] * 50, 4, 4),
+    "six heads": (lambda r: [int(x) for x in r.integers(0, 700, 9)], [2] * 9, 12, 2),
+}
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (150, 20)])
+@pytest.mark.parametrize("bits,HD", [(4, 64), (4, 128), (4, 256), (16, 64), (16, 128), (16, 256)])
+def test_attention_however_the_work_is_cut(e4b, dev, scratch, bits, HD, window, sinks):
+    for i, (name, (lens, counts, QH, KVH)) in enumerate(SHAPES.items()):
+        rng = np.random.default_rng(100 * i + HD)
+        lens = lens(rng)
+        c = Cache(e4b, dev, lens, counts, bits=bits, page=(16, 48, 64)[i % 3], KVH=KVH, HD=HD, ragged=any(n != 1 for n in counts))
+        held = c.fill(rng)
+        q = (rng.standard_normal((c.n_rows, QH, HD)) * (3.0 / np.sqrt(HD))).astype(F32)
+        got = attend(c, scratch, q, QH, window=window, sinks=sinks)
+        assert dev.status() == 0, name
+        check_rows(c, held, q, got, QH, window, sinks, 1.0)
+        clean = dev.alloc(int(e4b.lib().e4b_paged_scratch_bytes()))    # scratch used by other shapes: no trace
+        again = attend(c, clean, q, QH, window=window, sinks=sinks)
+        dev.free(clean)
+        for a, b in zip(got, again):
+            assert np.array_equal(a.view(np.uint8), b.view(np.uint8)), name
+        c.kv.free()
+
+
+@pytest.mark.parametrize("bits", [4, 16])
+@pytest.mark.parametrize("QH,counts", [(4, [1, 1]), (8, [1, 1]), (4, [9, 4])])
+def test_values_that_grow_large(e4b, dev, scratch, bits, QH, counts):
+    """Value scales from far below 2 to hundreds within a sequence: p gives up its lift on the way."""
+    rng = np.random.default_rng(21)
+    c = Cache(e4b, dev, [900, 500], counts, bits=bits, page=32, KVH=1, HD=128, ragged=max(counts) > 1)
+    held = c.fill(rng, grow=4000.0)
+    q = (rng.standard_normal((c.n_rows, QH, 128)) * 0.3).astype(F32)
+    got = attend(c, scratch, q, QH)
+    assert dev.status() == 0
+    check_rows(c, held, q, got, QH, 0, 0, 1.0)
+
+
+def test_no_rows_and_only_padding(e4b, dev, scratch):
+    c = Cache(e4b, dev, [20, 5, 40], [0, 0, 0], bits=4, page=16, KVH=2, HD=64, ragged=True, rows_cap=4)
+    held = c.fill(np.random.default_rng(1))
+    before = dev.read(c.kv.struct.k, np.uint8, c.kv.pool_bytes)
+    q = np.ones((4, 4, 64), F32)
+    check_rows(c, held, q, attend(c, scratch, q, 4), 4, 0, 0, 1.0)
+    x = dev.upload(np.ones((4, 4 * 64), F32))
+    for rows in (4, 0):
+        e4b.ops.headprep_paged(dev, c.kv, x, None, None, None, QH=0, ROPE_ANGLES=0, THETA=1e4, NORM=0, ROWS=rows)
+    c.n_rows = 0
+    attend(c, scratch, np.ones((1, 4, 64), F32), 4)
+    assert dev.status() == 0
+    assert np.array_equal(dev.read(c.kv.struct.k, np.uint8, c.kv.pool_bytes), before)
+
+
+def test_as_many_sequences_as_there_may_be(e4b, dev, scratch):
+    rng = np.random.default_rng(31)
+    n = 4096
+    lens = [int(x) for x in rng.integers(0, 40, n)]
+    c = Cache(e4b, dev, lens, [1] * n, bits=4, page=16, KVH=1, HD=64, ragged=False)
+    held = c.fill(rng)
+    q = (rng.standard_normal((n, 1, 64)) * 0.3).astype(F32)
+    got = attend(c, scratch, q, 1)
+    assert dev.status() == 0
+    check_rows(c, held, q, got, 1, 0, 0, 1.0, rows=range(0, n, 7))
+    # the same cache under a rows table: every row its own sequence's, some sequences without one
+    counts = np.array([s % 3 for s in range(n)])
+    first = np.concatenate([[0], np.cumsum(counts)]).astype(np.uint32)
+    c.kv.set_tables(lens=np.array(lens) + 1 - np.minimum(counts, np.array(lens) + 1), rows=dev.upload(first).ptr)
+    q2 = (rng.standard_normal((int(first[-1]), 1, 64)) * 0.3).astype(F32)
+    c.n_rows = int(first[-1])
+    got = attend(c, scratch, q2, 1)
+    assert dev.status() == 0
+    for s in range(0, n, 11):
+        for j in range(counts[s]):
+            r, p = int(first[s]) + j, lens[s] + 1 - min(counts[s], lens[s] + 1) + j
+            if p > lens[s]:
+                continue                                 # a slot that nobody wrote
+            ro, _ = op.attention(q2[r], p, held[s][0], held[s][1], 0, 0, 1.0)
+            assert np.abs(got[1][r] - ro).max() <= np.abs(held[s][1]).max() * 2.0 ** -10
+
+
+def test_two_contexts_at_once(e4b, dev):
+    """Calls of two contexts overlap on the device, each with its own scratch; the results are those of one at a time."""
+    other = e4b.Device(0)
+    try:
+        sets = []
+        for d, seed in ((dev, 1), (other, 2)):
+            rng = np.random.default_rng(seed)
+            c = Cache(e4b, d, [6000, 100, 3000], [5, 1, 2], bits=4, page=64, KVH=2, HD=128, ragged=True)
+            c.fill(rng)
+            s = d.alloc(int(e4b.lib().e4b_paged_scratch_bytes()))
+            q = d.upload((rng.standard_normal((c.n_rows, 8, 128)) * 0.3).astype(F32))
+            sets.append((d, c, s, q, [d.alloc(c.n_rows * 8 * 128 * 4) for _ in range(2)]))
+        for which in range(2):
+            for d, c, s, q, outs in sets:
+                for _ in range(1 if which == 0 else 20):
+                    e4b.ops.attn_paged(d, c.kv, q, None, outs[which], None, s, Q_HEADS=8, ROWS=c.n_rows)
+                if which == 0:
+                    d.sync()
+            for d, *_ in sets:
+                d.sync()
+        for d, c, s, q, outs in sets:
+            assert d.status() == 0
+            a, b = (d.read(o, np.uint8, c.n_rows * 8 * 128 * 4) for o in outs)
+            assert np.array_equal(a, b) and a.any()
+    finally:
+        other.close()
 
 
 def test_offsets_past_4_gib(e4b, dev, scratch):
