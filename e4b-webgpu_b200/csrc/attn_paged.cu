@@ -240,6 +240,11 @@ E4B_DEV void lds_words(uint32_t (&w)[WORDS], const uint8_t* p) {
     w[0] = *reinterpret_cast<const uint32_t*>(p);
   }
 }
+E4B_DEV uint32_t inc_acq_rel(uint32_t* at, uint32_t last) {
+  uint32_t was;
+  asm volatile("atom.acq_rel.gpu.global.inc.u32 %0, [%1], %2;" : "=r"(was) : "l"(at), "r"(last) : "memory");
+  return was;
+}
 __device__ __noinline__ bool wait_slow(uint64_t* b, uint32_t parity, uint32_t* status) {
   return mbar_wait(b, parity, status);
 }
@@ -265,7 +270,8 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
   __shared__ float qfac[Sh::TILES * TC];
   __shared__ float ml[W * LC * 2];
   __shared__ int last_one, more_units;
-  __shared__ Unit start, unit;
+  __shared__ struct { uint64_t at, base; int s; SeqWork w; } start;
+  __shared__ Unit unit;
   __shared__ uint32_t unit_c0, unit_c1;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
 
@@ -318,39 +324,39 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
   const bool uncut = units <= gridDim.x && 10 * units >= 7 * gridDim.x && 20 * (uint64_t)longest * units <= 23 * T;
   const uint64_t want = max(udiv(T, 2 * U), min((uint64_t)units, udiv(T, U)));
   const uint32_t C = T == 0 ? 0u : (uncut ? units : (want < 1 ? 1u : (want < gridDim.x ? (uint32_t)want : gridDim.x)));
-  const auto reach = [&](const Unit& v) { return uncut ? (uint32_t)(v.unit1 - v.unit0) / 2 + 1 : (uint32_t)U; };
+  const auto reach_of = [](uint64_t length, bool uncut) { return uncut ? (uint32_t)length / 2 + 1 : (uint32_t)U; };
   const uint32_t cta = blockIdx.x;
   if (cta >= C) return;
-  __shared__ uint64_t run_end[2];
-  {
-    Unit v;                          // at an end of the run, formed by the thread whose sequences hold it
-    v.unit0 = v.unit1 = 0;
+  __shared__ uint64_t run_end, work_all;                 // (read back where they are needed: the loops need the registers)
+  __shared__ uint32_t work_ctas;
+  __shared__ bool work_uncut;
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-      const uint64_t raw = udiv(T * (cta + i), C);
-      if (upto - mine <= raw && raw < upto) {
-        if (raw < v.unit0 || raw >= v.unit1) {
-          v.base = upto - mine;
-          v.s = tid * per;
-          v.w = own;
-          v.g = raw;
-          v.end = raw + 1;
-          v.next(p);
-        }
-        const uint64_t at = raw - v.unit0 < reach(v) ? v.unit0 : (v.unit1 - raw < reach(v) ? v.unit1 : raw);
-        run_end[i] = at;
-        if (i == 0) {
-          v.g = at;
-          start = v;
-        }
-      } else if (i == 1 && raw == T && tid == 0) {
-        run_end[1] = T;
+  for (int i = 0; i < 2; i++) {      // an end of the run, formed by the thread whose sequences hold it
+    const uint64_t raw = udiv(T * (cta + i), C);
+    if (upto - mine <= raw && raw < upto) {
+      uint64_t base = upto - mine;
+      int s = tid * per;
+      SeqWork w = own;
+      while (raw >= base + w.cost && s + 1 < p.d.nseq) {
+        base += w.cost;
+        w = seq_work<NT, U, MODE>(p, ++s);
       }
+      const uint64_t length = w.range.count + U, unit0 = base + udiv(raw - base, length) * length, unit1 = unit0 + length;
+      const uint64_t reach = reach_of(length, uncut), at = raw - unit0 < reach ? unit0 : (unit1 - raw < reach ? unit1 : raw);
+      if (i == 1) run_end = at;
+      else start.at = at, start.base = base, start.s = s, start.w = w;
+    } else if (i == 1 && raw == T && tid == 0) {
+      run_end = T;
     }
   }
+  if (tid == 0) work_all = T, work_ctas = C, work_uncut = uncut;
   __syncthreads();
-  Unit u = start;
-  u.end = run_end[1];
+  Unit u;
+  u.g = start.at;
+  u.end = run_end;
+  u.base = start.base;
+  u.s = start.s;
+  u.w = start.w;
 
   if (warp >= W) {
     // ---- producer: lane i brings the CTA's pieces i, i + LN, .., piece j into stage j % S
@@ -421,15 +427,9 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
   float O[NT][OT][4];
 
   // the unit in hand lives in shared memory: the loop over its pieces needs the registers
-  const auto next_unit = [&](Unit& v) {                  // thread 0; with the CTAs whose runs hold the unit, c0..c1
+  const auto next_unit = [&](Unit& v) {                  // thread 0
     more_units = v.next(p);
     unit = v;
-    const auto run_of = [&](uint64_t x) { return min((uint32_t)udiv((x + 1) * C - 1, T), C - 1); };
-    // (a run's end less than `reach` behind the unit's start moved there, one less before its end there)
-    const uint32_t F = reach(v), c0 = run_of(min(v.unit0 + F, v.unit1) - 1);
-    const uint32_t c1 = v.unit1 - v.unit0 < 2 * F ? c0 : run_of(v.unit1 - F);
-    unit_c0 = c0;
-    unit_c1 = c1;
   };
   if (tid == 0) next_unit(u);
   consumers();
@@ -840,6 +840,15 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
       if (st >= (uint32_t)S) st -= S, phase ^= 1u;
     }
     j0 += unit.span.count;
+    const bool whole = unit.unit0 >= start.at && unit.unit1 <= run_end;
+    if (!whole && lane == 0 && (uint32_t)warp == j0 % W) {               // the first to be idle
+      // the CTAs c0..c1 whose runs hold the unit: a run's end less than `reach` behind the
+      // unit's start moved there, one less before its end there
+      const auto run_of = [&](uint64_t x) { return min((uint32_t)udiv((x + 1) * work_ctas - 1, work_all), work_ctas - 1); };
+      const uint32_t F = reach_of(unit.unit1 - unit.unit0, work_uncut), c0 = run_of(min(unit.unit0 + F, unit.unit1) - 1);
+      unit_c0 = c0;
+      unit_c1 = unit.unit1 - unit.unit0 < 2 * F ? c0 : run_of(unit.unit1 - F);
+    }
 
     // ---- the warps' states
     consumers();                     // the q fragments have been read
@@ -877,8 +886,7 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
       }
     }
     consumers();
-    const uint32_t c0 = unit_c0, c1 = unit_c1;
-    const bool whole = c0 == c1;
+    const uint32_t c0 = unit_c0, c1 = unit_c1;             // (of a unit that is cut)
     const auto store = [&](int c, int dim, const float4& x) {
       const int head = unit.kvh * p.G + col_head(c);
       const size_t row = row0 + col_row(c);
@@ -967,40 +975,40 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
       // kGroup merges the group's into its first CTA's, and the last of those the rest.
       const auto part_of = [&](uint32_t c) { return p.parts + (2 * (size_t)c + (c == c0 ? 1 : 0)) * Sh::PART; };
       const auto arrive = [&](uint32_t* counter, uint32_t n) {
-        __threadfence();
-        consumers();
-        if (tid == 0) {
-          last_one = atomicInc(counter, n - 1) == n - 1;               // wraps to zero with the last arrival
-          __threadfence();
-        }
+        consumers();                   // the part is written: the arrival releases it, and acquires the others'
+        if (tid == 0) last_one = inc_acq_rel(counter, n - 1) == n - 1; // wraps to zero with the last arrival
         consumers();
         return last_one != 0;
       };
       // parts of CTAs a, a + step, .. (n of them): into the outputs, or into a's part
       const auto combine = [&](uint32_t a, uint32_t step, uint32_t n, bool final) {
-        float2* part_ml = reinterpret_cast<float2*>(merge);            // [n][cols]
-        for (uint32_t e = tid; e < n * cols; e += CT)
-          part_ml[e] = __ldcg(reinterpret_cast<const float2*>(part_of(a + e / cols * step) + Sh::COLS * HD + 2 * (e % cols)));
-        consumers();
         if constexpr (MODE != kRows) {
           for (int e = tid; e < LC * (HD / 4); e += CT) {
             const int c = e / (HD / 4), dim = e % (HD / 4) * 4;
             if (!col_live(c)) continue;
             float M = -INFINITY, L = 0.f;
-            for (uint32_t i = 0; i < n; i++) M = fmaxf(M, part_ml[i * LC + c].x);
             float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
             for (uint32_t i0 = 0; i0 < n; i0 += 8) {      // eight parts' loads in flight
               float4 x[8];
+              float2 y[8];
 #pragma unroll
-              for (int i = 0; i < 8; i++)
-                x[i] = __ldcg(reinterpret_cast<const float4*>(part_of(a + min(i0 + i, n - 1) * step) + c * HD + dim));
+              for (int i = 0; i < 8; i++) {
+                const float* from = part_of(a + min(i0 + i, n - 1) * step);
+                y[i] = __ldcg(reinterpret_cast<const float2*>(from + Sh::COLS * HD + 2 * c));
+                x[i] = __ldcg(reinterpret_cast<const float4*>(from + c * HD + dim));
+              }
+              float top = M;
+#pragma unroll
+              for (int i = 0; i < 8; i++) top = fmaxf(top, y[i].x);
+              const float f0 = M == top ? 1.f : ex2(M - top);
+              M = top;
+              L *= f0, o.x *= f0, o.y *= f0, o.z *= f0, o.w *= f0;
 #pragma unroll
               for (int i = 0; i < 8; i++) {
                 if (i0 + i >= n) continue;
-                const float2 y = part_ml[(i0 + i) * LC + c];
-                const float f = y.x == M ? 1.f : ex2(y.x - M);
-                L = fmaf(f, y.y, L);
+                const float f = y[i].x == M ? 1.f : ex2(y[i].x - M);
+                L = fmaf(f, y[i].y, L);
                 o.x = fmaf(f, x[i].x, o.x), o.y = fmaf(f, x[i].y, o.y);
                 o.z = fmaf(f, x[i].z, o.z), o.w = fmaf(f, x[i].w, o.w);
               }
@@ -1015,6 +1023,10 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
             }
           }
         } else {
+          float2* part_ml = reinterpret_cast<float2*>(merge);          // [n][cols]
+          for (uint32_t e = tid; e < n * cols; e += CT)
+            part_ml[e] = __ldcg(reinterpret_cast<const float2*>(part_of(a + e / cols * step) + Sh::COLS * HD + 2 * (e % cols)));
+          consumers();
           for (int c = tid; c < cols; c += CT) {           // the parts' weights
             float M = -INFINITY, L = 0.f;
             for (uint32_t i = 0; i < n; i++) M = fmaxf(M, part_ml[i * cols + c].x);
