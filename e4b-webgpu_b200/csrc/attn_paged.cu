@@ -36,6 +36,7 @@ using namespace e4b;
 
 constexpr int kMaxCtas = 320;
 constexpr int kGroup = 12;           // CTAs whose parts are merged first
+constexpr int kMostParts = 9;        // CTAs that share a unit evenly (10 to 12: merging them costs more than equal runs, 17.3 us against 15.1 us)
 constexpr uint32_t kLowCodes = 0x000F000Fu, kHighCodes = 0x00F000F0u;
 constexpr float kTwo24 = 16777216.f;
 // p is held as p * 2^8 relative to a maximum that may lag behind the largest score by
@@ -107,7 +108,8 @@ struct SeqWork {
   uint32_t p0, nq;                   // first row's position, rows
   PieceRange range;
   uint32_t units;                    // groups of rows times KV heads
-  uint64_t cost;                     // U + pieces, for each unit
+  uint32_t parts;                    // CTAs that share each unit evenly (kRows); 0: units are cut where the runs end
+  uint64_t cost;                     // U + pieces (or the parts), for each unit
 };
 template <int NT, int U, int MODE>
 E4B_DEV SeqWork seq_work(const AttnP& p, int s) {
@@ -117,7 +119,7 @@ E4B_DEV SeqWork seq_work(const AttnP& p, int s) {
   w.nq = r1 > r0 ? r1 - r0 : 0u;
   const uint32_t len = p.d.lens[s];
   w.p0 = min(len, 0xfffffff0u - w.nq);
-  w.units = 0;
+  w.units = w.parts = 0;
   w.cost = 0;
   if (w.nq) {
     // positions past the table are clamped: no such slot is visible
@@ -140,7 +142,7 @@ struct Walk {
   uint64_t g, end, base;             // base: where the current sequence's work begins
   int s;
   SeqWork w;
-  uint64_t unit0, unit1;             // the unit's work, the first U of it its set-up
+  uint64_t unit0, unit1;             // the unit's work, the first U of it its set-up (or its parts)
   uint32_t kvh, nrows;               // KV head, rows
   uint32_t pmin, pmax;               // positions of the unit's rows
   PieceSpan span;                    // this CTA's pieces of it
@@ -155,18 +157,21 @@ struct Walk {
       w = seq_work<NT, U, MODE>(p, s);
     }
     const uint32_t per = Rows<NT, MODE>(p.G).per_unit(), KVH = p.d.KVH, np = w.range.count;
-    const uint64_t unit = udiv(g - base, np + U);
+    const bool even = MODE == kRows && w.parts;
+    const uint32_t length = even ? w.parts : np + U;
+    const uint64_t unit = udiv(g - base, length);
     const uint32_t group = MODE == kRows ? (uint32_t)udiv(unit, KVH) : 0u;
     kvh = (uint32_t)unit - group * KVH;
-    unit0 = base + unit * (np + U);
-    unit1 = unit0 + np + U;
+    unit0 = base + unit * length;
+    unit1 = unit0 + length;
     nrows = min(per, w.nq - group * per);
     pmin = w.p0 + group * per;
     pmax = pmin + nrows - 1;
     const uint64_t stop = min(unit1, end);
     const uint32_t o0 = (uint32_t)(g - unit0), o1 = (uint32_t)(stop - unit0);
     const uint32_t p1 = min(pmax, p.d.cap - 1);
-    span = piece_span(w.range, o0 <= U ? 0u : o0 - U, o1 <= U ? 0u : o1 - U, min(pmin, p1), p1, p.window, p.sinks);
+    const auto piece_of = [&](uint32_t o) { return even ? o * np / length : (o <= U ? 0u : o - U); };
+    span = piece_span(w.range, piece_of(o0), piece_of(o1), min(pmin, p1), p1, p.window, p.sinks);
     g = stop;
     return true;
   }
@@ -266,6 +271,7 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
   __shared__ int usable[S];
   __shared__ uint64_t warp_sum_[Sh::THREADS / 32];
   __shared__ uint32_t warp_units[Sh::THREADS / 32], warp_longest[Sh::THREADS / 32];
+  __shared__ uint2 warp_parts[Sh::THREADS / 32];
   __shared__ uint2 qzero[BITS == 4 ? Sh::TILES * 32 : 32];               // B of the -8 term: -8 sum q per block, hi and lo
   __shared__ float qfac[Sh::TILES * TC];
   __shared__ float ml[W * LC * 2];
@@ -287,6 +293,7 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
   // ---- the run of this CTA: the work of all units, cut evenly
   uint64_t mine = 0;
   uint32_t units = 0, longest = 0;
+  uint32_t parts1 = 0, parts2 = 0;   // CTAs where each takes W, 2 W pieces of a unit (sums past the CTAs do not matter)
   SeqWork own;                       // of the thread's first sequence
   const int per = (p.d.nseq + Sh::THREADS - 1) / Sh::THREADS;
   for (int s = tid * per; s < min(p.d.nseq, (tid + 1) * per); s++) {
@@ -295,6 +302,10 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
     mine += w.cost;
     units += w.units;
     if (w.units) longest = max(longest, w.range.count + U);
+    if (MODE == kRows && w.units) {
+      parts1 += (uint32_t)min((uint64_t)w.units * ((w.range.count - 1) / W + 1), (uint64_t)0xffff);
+      parts2 += (uint32_t)min((uint64_t)w.units * ((w.range.count - 1) / (2 * W) + 1), (uint64_t)0xffff);
+    }
   }
   if (blockIdx.x == 0) live_rows(p.d);                   // records a row count past n_rows
   uint64_t upto = mine;                                  // inclusive sum over the threads
@@ -305,15 +316,20 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
   }
   units = __reduce_add_sync(0xffffffffu, min(units, 0xffffffu));
   longest = __reduce_max_sync(0xffffffffu, longest);
-  if (lane == 31) warp_sum_[warp] = upto, warp_units[warp] = units, warp_longest[warp] = longest;
+  if (MODE == kRows) parts1 = __reduce_add_sync(0xffffffffu, parts1), parts2 = __reduce_add_sync(0xffffffffu, parts2);
+  if (lane == 31) {
+    warp_sum_[warp] = upto, warp_units[warp] = units, warp_longest[warp] = longest;
+    if (MODE == kRows) warp_parts[warp] = make_uint2(parts1, parts2);
+  }
   __syncthreads();
   uint64_t before = 0, T = 0;
-  units = 0;
+  units = parts1 = parts2 = 0;
 #pragma unroll
   for (int i = 0; i < Sh::THREADS / 32; i++) {
     if (i < warp) before += warp_sum_[i];
     T += warp_sum_[i];
     units += warp_units[i];
+    if (MODE == kRows) parts1 += warp_parts[i].x, parts2 += warp_parts[i].y;
     longest = max(longest, warp_longest[i]);
   }
   upto += before;
@@ -321,10 +337,44 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
   // that falls within U of a unit's start or end moves there, so short units stay whole
   // and no fragment is shorter than U.  Units of about one length, and nearly as many as
   // CTAs, are not cut at all: an end then moves to the nearer one.
+  // Where the machine has a CTA for every W (or 2 W) pieces of a kRows unit, that many share
+  // it evenly, a turn (or two) of their warps, and none takes from two units (3 sequences of
+  // 64 query and 8 KV heads of 128, 1024-token windows: 18.8 us -> 14.0 us; one-row modes lose
+  // more to the longer set-up than they gain).
   const bool uncut = units <= gridDim.x && 10 * units >= 7 * gridDim.x && 20 * (uint64_t)longest * units <= 23 * T;
   const uint64_t want = max(udiv(T, 2 * U), min((uint64_t)units, udiv(T, U)));
-  const uint32_t C = T == 0 ? 0u : (uncut ? units : (want < 1 ? 1u : (want < gridDim.x ? (uint32_t)want : gridDim.x)));
-  const auto reach_of = [](uint64_t length, bool uncut) { return uncut ? (uint32_t)length / 2 + 1 : (uint32_t)U; };
+  uint32_t C = T == 0 ? 0u : (uncut ? units : (want < 1 ? 1u : (want < gridDim.x ? (uint32_t)want : gridDim.x)));
+  bool even = false;
+  if constexpr (MODE == kRows) {
+    const uint32_t most = longest - min(longest, (uint32_t)U), quota = parts1 <= gridDim.x ? W : 2 * W;
+    even = min(parts1, parts2) <= gridDim.x && most > W && most <= kMostParts * quota && per == 1;
+    if (even) {                      // a thread's one sequence measured in CTAs: the sums once more
+      if (mine) {
+        own.parts = (own.range.count - 1) / quota + 1;
+        mine = own.cost = own.parts * own.units;
+      }
+      uint32_t sum = (uint32_t)mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t v = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += v;
+      }
+      __syncthreads();
+      if (lane == 31) warp_sum_[warp] = sum;
+      __syncthreads();
+      upto = sum;
+      T = 0;
+#pragma unroll
+      for (int i = 0; i < Sh::THREADS / 32; i++) {
+        if (i < warp) upto += warp_sum_[i];
+        T += warp_sum_[i];
+      }
+      C = (uint32_t)T;
+    }
+  }
+  const auto reach_of = [](uint64_t length, bool even, bool uncut) {
+    return MODE == kRows && even ? 1u : (uncut ? (uint32_t)length / 2 + 1 : (uint32_t)U);
+  };
   const uint32_t cta = blockIdx.x;
   if (cta >= C) return;
   __shared__ uint64_t run_end, work_all;                 // (read back where they are needed: the loops need the registers)
@@ -341,8 +391,8 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
         base += w.cost;
         w = seq_work<NT, U, MODE>(p, ++s);
       }
-      const uint64_t length = w.range.count + U, unit0 = base + udiv(raw - base, length) * length, unit1 = unit0 + length;
-      const uint64_t reach = reach_of(length, uncut), at = raw - unit0 < reach ? unit0 : (unit1 - raw < reach ? unit1 : raw);
+      const uint64_t length = MODE == kRows && even ? w.parts : w.range.count + U, unit0 = base + udiv(raw - base, length) * length, unit1 = unit0 + length;
+      const uint64_t reach = reach_of(length, even, uncut), at = raw - unit0 < reach ? unit0 : (unit1 - raw < reach ? unit1 : raw);
       if (i == 1) run_end = at;
       else start.at = at, start.base = base, start.s = s, start.w = w;
     } else if (i == 1 && raw == T && tid == 0) {
@@ -845,7 +895,7 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
       // the CTAs c0..c1 whose runs hold the unit: a run's end less than `reach` behind the
       // unit's start moved there, one less before its end there
       const auto run_of = [&](uint64_t x) { return min((uint32_t)udiv((x + 1) * work_ctas - 1, work_all), work_ctas - 1); };
-      const uint32_t F = reach_of(unit.unit1 - unit.unit0, work_uncut), c0 = run_of(min(unit.unit0 + F, unit.unit1) - 1);
+      const uint32_t F = reach_of(unit.unit1 - unit.unit0, unit.w.parts, work_uncut), c0 = run_of(min(unit.unit0 + F, unit.unit1) - 1);
       unit_c0 = c0;
       unit_c1 = unit.unit1 - unit.unit0 < 2 * F ? c0 : run_of(unit.unit1 - F);
     }
