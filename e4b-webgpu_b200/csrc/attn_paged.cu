@@ -11,6 +11,16 @@
 // A unit cut between CTAs leaves partials in the scratch, which the last CTA to
 // arrive merges in CTA order (the same bits every time).
 //
+// Bounds and measurements (B200; a call's bytes at the copy rate, 6.45 TB/s, is its floor):
+// long caches in 4 bits are bound by the SM's issue slots, some 500 instructions a warp
+// for a piece of 9 KB: 32 sequences of 8000..16000 tokens, 16 query and 4 KV heads of 256,
+// 100 us = 4.1 TB/s (floor 63 us).  64 sequences of 1035 tokens take 28.6 us (floor 12 us)
+// and one of 131001 tokens and 2 KV heads 28.9 us (11.7 us): set-up, first pieces, merges
+// and the join of the parts, 6 to 8 us one after the other, come beside it; one token
+// behind 551 takes 10.3 us of them alone.  f16, 64 windows of 1024: 28.9 us (15.3 us).
+// Several rows a sequence (8 x 1..64 rows behind 300..4000 tokens, windows of 1024): 77 us,
+// bound by the latency of the products on 8 warps (tensor pipe 20 % busy).
+//
 // Products, per piece and 8 MMA columns (m16n8k16, f32 accumulators):
 //   S[slot][col]  = K[slot][:] . q[:][col]      A = keys,   B = q
 //   O[dim][col]  += V[slot][dim] p[slot][col]   A = values, B = p
@@ -336,11 +346,13 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
   // Runs of 2 U at least, or a unit's length (no two on a CTA while others idle); an end
   // that falls within U of a unit's start or end moves there, so short units stay whole
   // and no fragment is shorter than U.  Units of about one length, and nearly as many as
-  // CTAs, are not cut at all: an end then moves to the nearer one.
+  // CTAs, are not cut at all: an end then moves to the nearer one (64 sequences of 1035
+  // tokens and 4 KV heads 28.6 us against 32.6 us).
   // Where the machine has a CTA for every W (or 2 W) pieces of a kRows unit, that many share
   // it evenly, a turn (or two) of their warps, and none takes from two units (3 sequences of
-  // 64 query and 8 KV heads of 128, 1024-token windows: 18.8 us -> 14.0 us; one-row modes lose
-  // more to the longer set-up than they gain).
+  // 64 query and 8 KV heads of 128, 1024-token windows: 18.9 us -> 14.2 us).  With one row a
+  // unit the longer set-up takes back what it gives: one token behind 551 10.6 -> 10.2 us,
+  // 64 behind 1034 28.4 -> 29.1 us, one behind 131000 28.5 -> 29.0 us.
   const bool uncut = units <= gridDim.x && 10 * units >= 7 * gridDim.x && 20 * (uint64_t)longest * units <= 23 * T;
   const uint64_t want = max(udiv(T, 2 * U), min((uint64_t)units, udiv(T, U)));
   uint32_t C = T == 0 ? 0u : (uncut ? units : (want < 1 ? 1u : (want < gridDim.x ? (uint32_t)want : gridDim.x)));
@@ -1163,9 +1175,11 @@ int launch(e4b_ctx* c, const AttnP& p) {
 template <int BITS, int HD>
 int launch_mode(e4b_ctx* c, const AttnP& p) {
   if (p.G > 4 || p.d.rows) return launch<BITS, HD, kRows>(c, p);
-  // few units: all of an SM's warps on one (a 131K-token sequence of 2 KV heads 32 us
-  // against 40 us); more units than SMs: two CTAs per SM (64 x 1..8000 tokens of 4 KV
-  // heads, f16: 33 us against 60 us; 64 x 1035 tokens, 4 bits: 37 us against 41 us)
+  // few units: all of an SM's warps on one (kWide against kNarrow, 4 bits, heads of 256: a
+  // sequence of 131001 tokens and 2 KV heads 28.9 against 36.0 us, 32 of 8000..16000 tokens
+  // and 4 KV heads 100 against 109 us); more units than SMs: two CTAs per SM (64 of 1035
+  // tokens and 4 KV heads 28.6 against 34.4 us; f16, windows of 1024 in 1..8000 tokens 28.9
+  // against 43.0 us)
   if (p.d.nseq * p.d.KVH <= c->sm_count) return launch<BITS, HD, kWide>(c, p);
   return launch<BITS, HD, kNarrow>(c, p);
 }
