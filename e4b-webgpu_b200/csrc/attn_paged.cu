@@ -12,9 +12,9 @@
 // arrive merges in CTA order (the same bits every time).
 //
 // Bounds and measurements (B200; a call's bytes at the copy rate, 6.45 TB/s, is its floor):
-// long caches in 4 bits are bound by the SM's issue slots, some 500 instructions a warp
-// for a piece of 9 KB: 32 sequences of 8000..16000 tokens, 16 query and 4 KV heads of 256,
-// 100 us = 4.1 TB/s (floor 63 us).  64 sequences of 1035 tokens take 28.6 us (floor 12 us)
+// long caches in 4 bits are bound by the instructions, some 650 for a piece of 4.6 KB, of
+// which 12 warps issue one in 55 % of the cycles: 32 sequences of 8000..16000 tokens, 16
+// query and 4 KV heads of 256, 100 us = 4.1 TB/s (floor 63 us).  64 sequences of 1035 tokens take 28.6 us (floor 12 us)
 // and one of 131001 tokens and 2 KV heads 28.9 us (11.7 us): set-up, first pieces, merges
 // and the join of the parts, 6 to 8 us one after the other, come beside it; one token
 // behind 551 takes 10.3 us of them alone.  f16, 64 windows of 1024: 28.9 us (15.3 us).

@@ -177,7 +177,11 @@ E4B_DEV RowPlace place_one(const PagedDev& d, uint32_t row) {          // a thre
 // computed in f32.  Keys and values are formed in 64 bits: what is stored is then the
 // rounding of the exact value whatever the order of the sums, so the 4-bit codes do not
 // depend on it.  Bound by memory for many rows (per row of 16 q + 2 x 4 heads of 256:
-// 24.6 KB read, 16.4 KB of q and 2.3 KB of 4-bit cache written), by latency for few.
+// 24.6 KB read, 16.4 KB of q and 2.3 KB of 4-bit cache written): prompts of 16 x 1..1000
+// such rows with their read-back as f16 take 81 us, 4.3 TB/s (floor 55 us).  f16 rows whose
+// values are their keys, 8 x 1..500 into an f16 cache, 25 us (floor 12 us), are bound by the
+// lanes' conversions and 64-bit products between barriers (issue slots 53 % busy); one row,
+// 4.9 us, and 64, 6.3 us, by latency: two launches with their chains of loads.
 // A head of a turn: where its elements are, and where it goes.
 struct Item {
   uint32_t src;                      // bytes from the turn's first row (rows row_bytes apart: kStaged), or of its row
