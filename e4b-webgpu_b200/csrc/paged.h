@@ -17,6 +17,7 @@ namespace e4b {
 
 constexpr int kPieceSlots = 16;      // slots in a piece: one m16 (keys) or k16 (values) operand tile
 constexpr int kMaxSeqs = 4096;       // sequences of one paged cache
+constexpr int kMaxRows = 1 << 28;    // rows of a call, padding included (row arithmetic stays in 32 bits)
 
 // ---- layout.  A page holds its KV heads one after the other, a head's slots in
 // pieces of 16.  Inside a piece the elements are in matrix-operand order, so a
@@ -113,7 +114,7 @@ inline const char* paged_fault(const e4b_paged_kv* kv) {
 }
 // Rows of the call: with no `rows` table, row s is sequence s's one row.
 inline const char* paged_rows_fault(const e4b_paged_kv* kv, int n_rows) {
-  if (n_rows < 0) return "negative row count";
+  if (n_rows < 0 || n_rows > kMaxRows) return "n_rows must be 0..2^28";
   if (!kv->rows && n_rows != kv->nseq) return "without a rows table the call has one row per sequence";
   return nullptr;
 }

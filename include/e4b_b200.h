@@ -529,7 +529,8 @@ E4B_API int e4b_attdec_seq(e4b_ctx* ctx, const float* q, const uint16_t* kcache,
  * A position at or past max_pages*page, or a page id >= n_pages, sets
  * E4B_ST_BADINDEX in the device status word; the slot is then not written, and
  * counts as not visible (reads as zeros).  So does a row count past n_rows.
- * head_dim 64, 128 or 256; pools 16-byte aligned; nseq <= 4096. */
+ * lens, rows and pages do not change while a call runs that reads them.
+ * head_dim 64, 128 or 256; pools 16-byte aligned; nseq <= 4096; n_rows <= 2^28. */
 typedef struct {
   void* k; /* page pools, e4b_paged_pool_bytes each */
   void* v;
@@ -546,7 +547,7 @@ E4B_API size_t e4b_paged_pool_bytes(int bits, int page, int n_pages, int kv_head
  * they are (qw, kw unused).  RoPE on pairs (p, p + HD/2), p < rope_angles, at the
  * row's position, its angle in 64 bits.  q_out f32 [n_rows][QH][HD] (QH = 0: none);
  * K and V rows go to the cache (v = the k slice when keqv).  qkv 16-byte aligned
- * (f16: 8), row_stride % 4 == 0. */
+ * (f16: 8), row_stride % 4 == 0; q_out does not overlap qkv. */
 E4B_API int e4b_headprep_paged(e4b_ctx* ctx, const e4b_paged_kv* kv, const void* qkv, const float* qw,
                                const float* kw, float* q_out, int QH, int rope_angles, float theta, float eps,
                                int norm, int keqv, int x_f16, int row_stride, int nparts, int n_rows);
@@ -558,7 +559,8 @@ E4B_API int e4b_kvread_paged(e4b_ctx* ctx, const e4b_paged_kv* kv, void* k_out, 
  * t > p - window or t < sinks.  q f32 [n_rows][QH][HD]; out_h f16 (fragment order
  * when xfo) and / or out_f f32 [n_rows][QH*HD], lse f32 [n_rows][QH] or NULL; a row
  * that sees nothing gives zeros and lse = -inf.  Products carry f32 precision
- * (q and p as f16 hi + lo), sums are f32.  Pages wholly between the sinks and
+ * (q and p as f16 hi + lo), sums are f32; an infinity or NaN in a visible slot
+ * gives infinities or NaN in what it reaches.  Pages wholly between the sinks and
  * the window are not read and need no valid id.  scratch: e4b_paged_scratch_bytes(),
  * zeroed once before its first use (each call leaves it ready for the next) and
  * not shared by calls that may overlap.  q, outputs and scratch 16-byte aligned;

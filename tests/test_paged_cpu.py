@@ -208,6 +208,8 @@ def test_bad_arguments_are_refused(e4b, shim):
                 dict(oh=None, of=4096, xfo=1), dict(oh=4104), dict(of=4100), dict(lse=4098)):
         assert _attn(shim, kv, **bad), bad
     assert _attn(shim, ragged, n=-1) and _attn(shim, ragged, n=0) is None
+    for call in (_prep, _attn):
+        assert call(shim, ragged, n=1 << 28) is None and call(shim, ragged, n=(1 << 28) + 1) and call(shim, ragged, n=(1 << 31) - 1)
     assert shim.f_read(ctypes.byref(kv), None, None, 2) and shim.f_read(ctypes.byref(kv), ctypes.c_void_p(8), None, 2)
 
 
