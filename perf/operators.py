@@ -296,16 +296,15 @@ def _plain_attn(s):
 
 
 # ------------------------------------------------------------------ the framework's calls
-_dev = _scratch = None
+_dev = None
 
 
 def _own(s):
-    """The device context with its scratch and the cache's handle, as a program holds them."""
-    global _dev, _scratch
+    """The device context and the cache's handle, as a program holds them."""
+    global _dev
     e4b = importlib.import_module("e4b-webgpu_b200")
     if _dev is None:
         _dev = e4b.Device(torch.cuda.current_device())
-        _scratch = _dev.alloc(e4b.lib().e4b_paged_scratch_bytes(), "scratch")  # zeroed, once
     c = s["case"]
     s["kv"] = e4b.PagedKV(_dev, BITS=c["bits"], PAGE=c["page"], PAGES=s["n_pages"], MAX_PAGES=s["table"].shape[1], SEQS=c["nseq"],
                           KV_HEADS=c["kvh"], HEAD_DIM=c["hd"], k=s["k"].data_ptr(), v=s["v"].data_ptr(),
@@ -332,7 +331,7 @@ def run(s):
         ops.kvread_paged(_dev, s["kv"], p["k_out"], p["v_out"], ROWS=s["n"])
         return {"q": s["q_out"], "k": s["k_out"], "v": s["v_out"]}
     half = c["out"] == "f16"
-    ops.attn_paged(_dev, s["kv"], p["q"], p["out"] if half else None, None if half else p["out"], p["lse"], _scratch,
+    ops.attn_paged(_dev, s["kv"], p["q"], p["out"] if half else None, None if half else p["out"], p["lse"], p["scratch"],
                    Q_HEADS=c["qh"], WINDOW=c["window"], SINKS=c["sinks"], ROWS=s["n"])
     return {"o": s["out"], "lse": s["lse"]}
 
