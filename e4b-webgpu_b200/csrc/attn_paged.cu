@@ -1081,8 +1081,13 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
               if (dim == 0) close_column(c, M, L);
             } else {
               *reinterpret_cast<float4*>(part_of(a) + c * HD + dim) = o;
-              if (dim == 0) *reinterpret_cast<float2*>(part_of(a) + Sh::COLS * HD + 2 * c) = make_float2(M, L);
+              if (dim == 0) ml[2 * c] = M, ml[2 * c + 1] = L;
             }
+          }
+          if (!final) {                // a column is up to two warps: its threads have read part a's (max, sum) before it changes
+            consumers();
+            if (tid < LC && col_live(tid))
+              *reinterpret_cast<float2*>(part_of(a) + Sh::COLS * HD + 2 * tid) = make_float2(ml[2 * tid], ml[2 * tid + 1]);
           }
         } else {
           float2* part_ml = reinterpret_cast<float2*>(merge);          // [n][cols]
