@@ -235,17 +235,18 @@ __global__ void __launch_bounds__(threads_of<MODE>(), MODE == kFew ? 1 : 2) k_he
   };
   if (MODE != kFew)
     for (int i = tid; i < total; i += THREADS) items[i] = item_of(i);
-  float qw[8];
+  float qw[8], kw = 0.f;
 #pragma unroll
   for (int j = 0; j < 8; j++) qw[j] = 1.f;
-  if (p.norm) {
+  pdl_wait();
+  static_assert(HD <= THREADS, "a thread per weight");
+  if (p.norm) {                      // (the call before may have written the weights)
     if (p.QH > 0) {
       const float4 a = *reinterpret_cast<const float4*>(p.qw + 4 * l), b = *reinterpret_cast<const float4*>(p.qw + HALF + 4 * l);
       qw[0] = a.x, qw[1] = a.y, qw[2] = a.z, qw[3] = a.w, qw[4] = b.x, qw[5] = b.y, qw[6] = b.z, qw[7] = b.w;
     }
-    for (int i = tid; i < HD; i += THREADS) kw64[i] = (double)p.kw[i];
+    if (tid < HD) kw = p.kw[tid];
   }
-  pdl_wait();
   // a CTA's rows are consecutive: they share sequences, pieces and (nearly) angles
   const uint32_t live = live_rows(p.d);
   const uint32_t first_row = blockIdx.x * p.rows_per_cta, end_row = min(live, first_row + p.rows_per_cta);
@@ -297,6 +298,7 @@ __global__ void __launch_bounds__(threads_of<MODE>(), MODE == kFew ? 1 : 2) k_he
       }
   };
   look_up(first_row);
+  if (tid < HD) kw64[tid] = (double)kw;
   form_angles(first_row, 0, 0, true);
   __syncthreads();
   uint32_t turn_no = 0, at_row = 0;                      // at_row: the turn's place in its batch

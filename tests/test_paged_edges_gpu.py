@@ -29,3 +29,29 @@ def test_a_unit_over_more_ctas_than_one_group(e4b, dev, scratch, bits, QH, KVH, 
         assert np.array_equal(dev.read(of, np.uint32, n), first[1].ravel().view(np.uint32))
     assert dev.status() == 0
     c.kv.free()
+
+
+@pytest.mark.parametrize("rows", [2, 900])
+def test_norm_weights_written_by_the_call_before(e4b, dev, rows):
+    """The head prep's weights come out of a GEMV that lets its successor start early: they are read after it is done."""
+    QH, KVH, HD, n_in = 4, 2, 128, 16384
+    rng = np.random.default_rng(rows)
+    raw = dev.upload(e4b.synth.quant_q4_0(e4b.synth.normal_f32(HD * n_in, 5, "w", 0.02)))
+    x = dev.upload(rng.standard_normal((rows, (QH + 2 * KVH) * HD)).astype(F32))
+    vecs = [dev.upload(rng.standard_normal(n_in).astype(F32)) for _ in range(2)]
+    w, bq = dev.alloc(HD * 4), dev.alloc(rows * QH * HD * 4)
+    c = Cache(e4b, dev, [3], [rows], bits=16, page=64, KVH=KVH, HD=HD, ragged=True)
+
+    def prep(vec, wait):
+        e4b.ops.q40mv(dev, vec, raw, None, w, IN=n_in, OUT=HD)
+        if wait:
+            dev.sync()
+        e4b.ops.headprep_paged(dev, c.kv, x, w, w, bq, QH=QH, ROPE_ANGLES=HD // 2, THETA=1e4, ROWS=rows)
+        return [dev.read(bq, F32, rows * QH * HD)] + c.read_rows()
+
+    want = [prep(v, True) for v in vecs]
+    assert not np.array_equal(want[0][0], want[1][0])
+    for i in range(20):
+        for a, b in zip(prep(vecs[i % 2], False), want[i % 2]):
+            assert np.array_equal(a, b)
+    assert dev.status() == 0
