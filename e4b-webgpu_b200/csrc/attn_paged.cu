@@ -680,13 +680,40 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
         }
       }
 
-      // ---- value scales of slots (2t, 2t+1) and (2t+8, 2t+9); one of 2 or more ends the lift of p
+      // ---- the slots (2t, 2t+1) and (2t+8, 2t+9) that the lane's p column sees (keep: masks of
+      // halves), and that some row of the warp sees
+      bool full[N], masked = false;
+      uint32_t keep[N][2], seen[2] = {0u, 0u};
+#pragma unroll
+      for (int nt = 0; nt < N; nt++) {
+        full[nt] = here && t0 + kPieceSlots - 1 <= pos0[nt] &&
+                   (p.window == 0 || pos1[nt] - t0 < p.window || t0 + kPieceSlots <= p.sinks);
+        keep[nt][0] = keep[nt][1] = full[nt] ? 0xffffffffu : 0u;
+        if (!full[nt]) {
+          masked = true;
+#pragma unroll
+          for (int k = 0; k < 4; k++)
+            if (here && slot_visible(t0 + 2 * t + (k & 1) + 8 * (k >> 1), posg[nt], p.window, p.sinks))
+              keep[nt][k >> 1] |= 0xffffu << (16 * (k & 1));
+        }
+        seen[0] |= keep[nt][0], seen[1] |= keep[nt][1];
+      }
+      if (MODE == kRows && masked) {                     // over the columns' rows
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+          seen[k] |= __shfl_xor_sync(0xffffffffu, seen[k], 4);
+          seen[k] |= __shfl_xor_sync(0xffffffffu, seen[k], 8);
+          seen[k] |= __shfl_xor_sync(0xffffffffu, seen[k], 16);
+        }
+      }
+
+      // ---- the value scales that some row sees; one of 2 or more ends the lift of p
       if (BITS == 4) {
         uint32_t any = 0;
 #pragma unroll
         for (int b = 0; b < NB; b += 2) {
           const uint4 d4 = lds128_once(vp + (t * NB + b) * 8);
-          any |= d4.x | d4.y | d4.z | d4.w;
+          any |= ((d4.x | d4.z) & seen[0]) | ((d4.y | d4.w) & seen[1]);
         }
         if (__any_sync(0xffffffffu, (any & 0x40004000u) != 0) && lift != 0.f) {
           lift = slack = 0.f;
@@ -702,12 +729,9 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
       }
 
       // ---- softmax state and p as B fragments
-      uint32_t ph[N][2], pl[N][2], keep[N][2];        // slots (2t, 2t+1), (2t+8, 2t+9); keep: mask of visible halves
-      bool full[N];
+      uint32_t ph[N][2], pl[N][2];                    // slots (2t, 2t+1), (2t+8, 2t+9)
 #pragma unroll
       for (int nt = 0; nt < N; nt++) {
-        full[nt] = here && t0 + kPieceSlots - 1 <= pos0[nt] &&
-                   (p.window == 0 || pos1[nt] - t0 < p.window || t0 + kPieceSlots <= p.sinks);
         float v[4];
         bool see[4] = {true, true, true, true};
 #pragma unroll
@@ -716,13 +740,10 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
           v[k] = s[nt][k] * fac[nt][k & 1];
         }
         if (!full[nt]) {
-          keep[nt][0] = keep[nt][1] = 0;
 #pragma unroll
           for (int k = 0; k < 4; k++) {
             see[k] = here && slot_visible(t0 + g + 8 * (k >> 1), pos[nt][k & 1], p.window, p.sinks);
             if (!see[k]) v[k] = -INFINITY;
-            if (here && slot_visible(t0 + 2 * t + (k & 1) + 8 * (k >> 1), posg[nt], p.window, p.sinks))
-              keep[nt][k >> 1] |= 0xffffu << (16 * (k & 1));
           }
         }
         const bool grow = fmaxf(v[0], v[2]) > top[nt][0] + slack || fmaxf(v[1], v[3]) > top[nt][1] + slack;
@@ -776,23 +797,8 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
       // become zero.  strict: a row does not see a slot that another row sees and that
       // holds an infinity or NaN, so its own mask goes on every operand.
       bool strict[N];
-      uint32_t seen[2] = {0u, 0u};
-      bool masked = false;
 #pragma unroll
-      for (int nt = 0; nt < N; nt++) {
-        strict[nt] = false;
-        if (full[nt]) keep[nt][0] = keep[nt][1] = 0xffffffffu;
-        else masked = true;
-        seen[0] |= keep[nt][0], seen[1] |= keep[nt][1];
-      }
-      if (MODE == kRows && masked) {                     // over the columns' rows
-#pragma unroll
-        for (int k = 0; k < 2; k++) {
-          seen[k] |= __shfl_xor_sync(0xffffffffu, seen[k], 4);
-          seen[k] |= __shfl_xor_sync(0xffffffffu, seen[k], 8);
-          seen[k] |= __shfl_xor_sync(0xffffffffu, seen[k], 16);
-        }
-      }
+      for (int nt = 0; nt < N; nt++) strict[nt] = false;
       uint32_t dv[NB][2];
       if (BITS == 4) {
 #pragma unroll

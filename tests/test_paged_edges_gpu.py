@@ -55,3 +55,43 @@ def test_norm_weights_written_by_the_call_before(e4b, dev, rows):
         for a, b in zip(prep(vecs[i % 2], False), want[i % 2]):
             assert np.array_equal(a, b)
     assert dev.status() == 0
+
+
+def write(c, xs, fill=0xff):
+    """The sequences' keys and values xs[s] [slots][2][KVH][HD] into the pages, `fill` in every other byte; what the pages
+    then stand for."""
+    pools, held = c.pools(fill), []
+    for s, x in enumerate(xs):
+        x, t = x.astype(np.float16), np.arange(len(x))
+        pid = c.table[s, t // c.page].astype(np.int64)
+        for i, pool in enumerate(pools):
+            pool.write_all(pid, t % c.page, x[:, i])
+        held.append([pool.read_all(pid, t % c.page) for pool in pools])
+    for pool, ptr in zip(pools, (c.kv.struct.k, c.kv.struct.v)):
+        c.dev.write(ptr, pool.raw)
+    return held
+
+
+@pytest.mark.parametrize("bits", [4, 16])
+@pytest.mark.parametrize("HD,QH,KVH,lens,counts", [(256, 8, 2, [70, 9, 333, 0], [1] * 4), (128, 4, 1, [70, 9, 333, 0], [1] * 4),
+                                                   (64, 16, 4, [70, 9, 333, 0] * 12, [1] * 48), (256, 4, 1, [70, 9], [3, 20]),
+                                                   (64, 7, 1, [70, 9], [3, 20])])
+def test_bits_do_not_depend_on_hidden_bytes(e4b, dev, scratch, bits, HD, QH, KVH, lens, counts):  # noqa: F811
+    """The rest of a last page, a page that the table does not name, and slots between the sinks and every row's window:
+    zeros, NaN, or values a thousand times the visible ones change no bit of the outputs."""
+    window, sinks, rng = 37, 5, np.random.default_rng(HD + QH)
+    c = Cache(e4b, dev, lens, counts, bits=bits, page=32, KVH=KVH, HD=HD, ragged=max(counts) > 1)
+    xs = [rng.standard_normal((a + b, 2, KVH, HD)) for a, b in zip(lens, counts)]
+    q = (rng.standard_normal((c.n, QH, HD)) * (3.0 / np.sqrt(HD))).astype(F32)
+    got = []
+    for fill, factor in ((0xff, 1.0), (0x00, 1.0), (0x42, 1000.0)):
+        ys = [x.copy() for x in xs]
+        for y, n in zip(ys, lens):
+            y[sinks:max(sinks, n - window + 1)] *= factor
+        held = write(c, ys, fill)
+        got.append(attend(c, scratch, q, QH, window=window, sinks=sinks))
+        assert dev.status() == 0
+    check_rows(c, held, q, got[-1], QH, window, sinks, 1.0)
+    for g in got[1:]:
+        for a, b in zip(g, got[0]):
+            assert np.array_equal(a.view(np.uint8), b.view(np.uint8))
