@@ -33,9 +33,11 @@
 // The MMA aligns a subnormal by its exponent field, which costs it up to 7 of the
 // sum's 24 bits: no loss for 15-bit products of one magnitude (q's), but 6e-6 of
 // the result where p spreads over many, so 4-bit values are decoded to normal f16
-// n - 8.  A value block's scale multiplies p, again as hi + lo; p is lifted by 2^8
-// unless a scale of the piece is 2 or more, so that the lo parts stay clear of
-// f16's subnormals.
+// n - 8.  A value block's scale multiplies p, again as hi + lo.  To keep the lo parts
+// clear of f16's subnormals p is lifted by 2^8, and a block of 32 dims whose visible
+// scales have all been below 2^-7 (2^-14) is held times 2^8 (2^15): a product is off by
+// 2^-20 of itself and 2^-22 of the largest p times the block's largest value at most
+// (2^-16 of that where scales of 2^7 or more stand beside such a block).
 #include <type_traits>
 
 #include "paged.cuh"
@@ -50,8 +52,16 @@ constexpr int kMostParts = 9;        // CTAs that share a unit evenly (10 to 12:
 constexpr uint32_t kLowCodes = 0x000F000Fu, kHighCodes = 0x00F000F0u;
 constexpr float kTwo24 = 16777216.f;
 // p is held as p * 2^8 relative to a maximum that may lag behind the largest score by
-// 2^6, so a rescaling of O is rare and p * d stays below 2^15 for scales d below 2
-constexpr float kLift = 8.f, kSlack = 6.f;
+// 2^6, so a rescaling of O is rare and p * d stays below 2^15 for scales d below 2.
+// A visible scale of 2 or more ends the lag (d below 2^7), one of 2^7 or more leaves a
+// lift of 2^2 (d up to f16's largest, 2^13).
+constexpr float kLift = 8.f, kSlack = 6.f, kLowLift = 2.f;
+// Scale of the values of block b in O and in the products: state c of two bits a block.
+constexpr uint32_t kAllTiny = 0xAAAAAAAAu;               // nothing but zeros seen yet
+E4B_DEV uint32_t scale_state(uint32_t states, int b) { return (states >> (2 * b)) & 3u; }
+E4B_DEV int scale_up(uint32_t c) { return c == 2 ? 15 : (c == 1 ? 8 : 0); }
+E4B_DEV uint32_t scale_half2(uint32_t c) { return c == 2 ? 0x78007800u : (c == 1 ? 0x5C005C00u : 0x3C003C00u); }
+E4B_DEV float scale_pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 
 struct AttnP {
   PagedDev d;
@@ -574,6 +584,7 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
     }
     consumers();
     float top[NT][2], lsum[NT][2], fac[NT][2], lift = kLift, slack = kSlack;  // reference score; sum of p; score factor
+    uint32_t ups = kAllTiny & ((1ull << (2 * NB)) - 1); // the blocks' scales
     uint32_t pos0[NT], pos1[NT], pos[NT][2], posg[NT];   // of the tile's first and last row, the lane's score columns, its p column
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
@@ -707,7 +718,7 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
         }
       }
 
-      // ---- the value scales that some row sees; one of 2 or more ends the lift of p
+      // ---- the value scales that some row sees: what p's lift and the blocks' scales have to be
       if (BITS == 4) {
         uint32_t any = 0;
 #pragma unroll
@@ -715,15 +726,44 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
           const uint4 d4 = lds128_once(vp + (t * NB + b) * 8);
           any |= ((d4.x | d4.z) & seen[0]) | ((d4.y | d4.w) & seen[1]);
         }
-        if (__any_sync(0xffffffffu, (any & 0x40004000u) != 0) && lift != 0.f) {
-          lift = slack = 0.f;
+        const bool big = __any_sync(0xffffffffu, (any & 0x40004000u) != 0) && lift == kLift;   // 2 or more
+        if (__builtin_expect(big || ups != 0, 0)) {
+          uint32_t sizes = 0;        // two bits a block: a scale >= 2^-14, one >= 2^-7; the top one: any >= 2^7
 #pragma unroll
-          for (int nt = 0; nt < N; nt++) {
-            lsum[nt][0] *= 1.f / 256.f, lsum[nt][1] *= 1.f / 256.f;
+          for (int b = 0; b < NB; b++) {
+            const uint2 d = *reinterpret_cast<const uint2*>(vp + (t * NB + b) * 8);
+            const uint32_t w0 = d.x & seen[0], w1 = d.y & seen[1], w = w0 | w1;
+            if (w & 0x7C007C00u) sizes |= 1u << (2 * b);
+            if (w & 0x60006000u) sizes |= 2u << (2 * b);
+            if (big && (w & 0x40004000u)) {
+              const __half2 m = __hmax2(__habs2(*reinterpret_cast<const __half2*>(&w0)), __habs2(*reinterpret_cast<const __half2*>(&w1)));
+              if (!(__low2float(m) < 128.f && __high2float(m) < 128.f)) sizes |= 1u << 31;
+            }
+          }
+          sizes = __reduce_or_sync(0xffffffffu, sizes);
+          int fall = 0;              // of the lift
+          if (big) slack = 0.f;
+          if (sizes >> 31) {
+            fall = (int)(kLift - kLowLift);
+            lift = kLowLift;
+          }
+          const uint32_t were = ups;
 #pragma unroll
-            for (int o = 0; o < OT; o++)
+          for (int b = 0; b < NB; b++) {                 // a block's scale only ever falls, to 1 in the end
+            const uint32_t was = scale_state(were, b), is = min(was, 2u - min(scale_state(sizes, b), 2u));
+            ups ^= (was ^ is) << (2 * b);
+          }
+          if (!fresh && (fall || ups != were)) {
 #pragma unroll
-              for (int k = 0; k < 4; k++) O[nt][o][k] *= 1.f / 256.f;
+            for (int nt = 0; nt < N; nt++) {
+              lsum[nt][0] *= scale_pow2(-fall), lsum[nt][1] *= scale_pow2(-fall);
+#pragma unroll
+              for (int b = 0; b < NB; b++) {
+                const float f = scale_pow2(scale_up(scale_state(ups, b)) - scale_up(scale_state(were, b)) - fall);
+#pragma unroll
+                for (int k = 0; k < 4; k++) O[nt][2 * b][k] *= f, O[nt][2 * b + 1][k] *= f;
+              }
+            }
           }
         }
       }
@@ -806,13 +846,13 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
           const uint4 d4 = lds128(vp + (t * NB + b) * 8);
           dv[b][0] = d4.x, dv[b][1] = d4.y, dv[b + 1][0] = d4.z, dv[b + 1][1] = d4.w;
         }
-        if (masked) {
+        if (__builtin_expect(masked || ups != 0, 0)) {
           bool odd = false;
 #pragma unroll
           for (int b = 0; b < NB; b++)
 #pragma unroll
             for (int k = 0; k < 2; k++) {
-              dv[b][k] &= seen[k];
+              dv[b][k] = hmul2(dv[b][k] & seen[k], scale_half2(scale_state(ups, b)));
               odd |= !finite2(dv[b][k]);
             }
           if (MODE == kRows && __any_sync(0xffffffffu, odd)) {
@@ -919,6 +959,16 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
     }
 
     // ---- the warps' states
+    if (BITS == 4 && ups) {          // the blocks' scales come off
+#pragma unroll
+      for (int b = 0; b < NB; b++) {
+        const float f = scale_pow2(-scale_up(scale_state(ups, b)));
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+          for (int k = 0; k < 4; k++) O[nt][2 * b][k] *= f, O[nt][2 * b + 1][k] *= f;
+      }
+    }
     consumers();                     // the q fragments have been read
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {

@@ -558,9 +558,13 @@ E4B_API int e4b_kvread_paged(e4b_ctx* ctx, const e4b_paged_kv* kv, void* k_out, 
  * the row at position p sees slots t <= p, with window > 0 only those with
  * t > p - window or t < sinks.  q f32 [n_rows][QH][HD]; out_h f16 (fragment order
  * when xfo) and / or out_f f32 [n_rows][QH*HD], lse f32 [n_rows][QH] or NULL; a row
- * that sees nothing gives zeros and lse = -inf.  Products carry f32 precision
- * (q and p as f16 hi + lo), sums are f32; an infinity or NaN in a visible slot
- * gives infinities or NaN in what it reaches.  Pages wholly between the sinks and
+ * that sees nothing gives zeros and lse = -inf.  q and the softmax's p are f16
+ * hi + lo pairs and the sums f32: a product is off by 2^-20 of itself and 2^-22 of
+ * the largest |q| (p) times the largest |k| (|v|) of its 32 dims that the call's
+ * rows see of the sequence (values of an f16 cache below 2^-14 count as 2^-14; 2^-16
+ * for values below 2^-4 beside others above 1024).  An infinity or NaN in a visible
+ * slot gives infinities or NaN in what it reaches; slots that no row sees change no
+ * bit.  Pages wholly between the sinks and
  * the window are not read and need no valid id.  scratch: e4b_paged_scratch_bytes(),
  * zeroed once before its first use (each call leaves it ready for the next) and
  * not shared by calls that may overlap.  q, outputs and scratch 16-byte aligned;

@@ -95,3 +95,45 @@ def test_bits_do_not_depend_on_hidden_bytes(e4b, dev, scratch, bits, HD, QH, KVH
     for g in got[1:]:
         for a, b in zip(g, got[0]):
             assert np.array_equal(a.view(np.uint8), b.view(np.uint8))
+
+
+SIZES = {  # factors of the values' blocks of 32 dims in turn, and whether they change along the sequence
+    "1e-4": ([1e-4], 0), "1e-6": ([1e-6], 0), "far apart": ([1.0, 1e-4, 30.0, 1e-6], 0), "0.01 beside 20": ([0.01, 20.0], 0),
+    "huge beside small": ([5000.0, 1.0, 1e-3], 0), "falling": ([1.0, 1e-3], -1), "growing": ([1e-6, 1e-4, 1.0], 1),
+    "zeros, then small": ([0.0, 1e-5], 1),
+}
+
+
+@pytest.mark.parametrize("HD", [64, 128, 256])
+@pytest.mark.parametrize("QH,counts", [(4, [1, 1, 1]), (3, [9, 1, 0])])
+@pytest.mark.parametrize("name", SIZES)
+def test_4_bit_values_of_any_size(e4b, dev, scratch, name, HD, QH, counts):  # noqa: F811
+    """Every block of 32 dims is as precise relative to its own largest value.  Scores: at most 2^-16 of the sum of
+    |q| 15 d (codes enter as 0..15), which moves an output by twice that of vmax.  Products p d: 2^-22 of the largest p
+    times vmax each (2^-16 beside scales of 2^7 or more), so n / sum(p / max p) of it in the output.  The rest, ex2
+    (2^-22), three roundings of a product (2^-20), 17 addends cut at 2^-23 in each of the two MMAs of a piece (2^-18),
+    f32 sums: 2^-16 altogether."""
+    factors, change = SIZES[name]
+    lens, rng = [700, 45, 3], np.random.default_rng(HD)
+    c = Cache(e4b, dev, lens, counts, bits=4, page=32, KVH=1, HD=HD, ragged=max(counts) > 1)
+    size, xs = np.array([factors[b % len(factors)] for b in range(HD // 32)]).repeat(32), []
+    for n in (a + b for a, b in zip(lens, counts)):
+        x = rng.standard_normal((n, 2, 1, HD))
+        x[:, 1, 0] *= size * 2.0 ** (change * np.linspace(0, 6, n))[:, None]
+        xs.append(x)
+    held = write(c, xs)
+    q = (rng.standard_normal((c.n, QH, HD)) * 2.0 ** -10 / np.sqrt(HD)).astype(F32)
+    of = attend(c, scratch, q, QH)[1]
+    assert dev.status() == 0
+    wide = 2.0 ** -16 if max(factors) * (64 if change > 0 else 1) > 500 else 2.0 ** -22
+    for r in range(c.n):
+        s, p = c.place(r)
+        k, v = (a[:p + 1, 0] for a in held[s])
+        sc = q[r].astype(np.float64) @ k.T                                   # [QH][slots]
+        w = np.exp(sc - sc.max(1, keepdims=True))
+        want = w @ v / w.sum(1, keepdims=True)
+        d15 = 15 / 8 * np.abs(k).reshape(-1, HD // 32, 32).max(-1).repeat(32, -1)
+        ds = 2.0 ** -16 * (np.abs(q[r]).astype(np.float64) @ d15.T).max(1)
+        vmax = np.abs(v).reshape(-1, HD // 32, 32).max((0, 2)).repeat(32)
+        tol = (2 * ds + 2.0 ** -16 + wide * (p + 1) / w.sum(1))[:, None] * vmax
+        assert (np.abs(of[r] - want) <= tol).all(), (r, (np.abs(of[r] - want) / np.maximum(tol, 1e-300)).max())
