@@ -495,10 +495,18 @@ __global__ void __launch_bounds__(128) k_kvread_paged(const PagedDev d, void* k_
   }
 }
 
-__global__ void k_paged_advance(uint32_t* lens, const uint32_t* __restrict__ rows, int nseq) {
+// n_rows: of the call whose rows these are; rows of the table past them were not written.
+__global__ void k_paged_advance(const PagedDev d, uint32_t* lens) {
   pdl_wait();
+  const uint32_t live = live_rows(d);
   const int s = blockIdx.x * blockDim.x + threadIdx.x;
-  if (s < nseq) lens[s] += rows ? rows[s + 1] - rows[s] : 1u;
+  if (s >= d.nseq) return;
+  uint32_t n = 1;
+  if (d.rows) {
+    const uint32_t r0 = min(d.rows[s], live), r1 = min(d.rows[s + 1], live);
+    n = r1 > r0 ? r1 - r0 : 0u;
+  }
+  lens[s] += n;
 }
 
 template <int HD, int MODE>
@@ -583,12 +591,17 @@ E4B_API int e4b_kvread_paged(e4b_ctx* c, const e4b_paged_kv* kv, void* k_out, vo
   return e4b_launch(c, "kvread_paged", kern, grid, dim3(128), 0, paged_dev(c, kv, n_rows), k_out, v_out, out_f32 ? 1 : 0);
 }
 
-E4B_API int e4b_paged_advance(e4b_ctx* c, const e4b_paged_kv* kv) {
+E4B_API int e4b_paged_advance_rows(e4b_ctx* c, const e4b_paged_kv* kv, int n_rows) {
   E4B_CHECK_CTX(c);
   const char* fault = paged_fault(kv);
+  if (!fault) fault = paged_rows_fault(kv, n_rows);
   E4B_REQUIRE(c, !fault, "paged_advance: %s", fault);
   return e4b_launch(c, "paged_advance", k_paged_advance, dim3((kv->nseq + 127) / 128), dim3(128), 0,
-                    const_cast<uint32_t*>(kv->lens), kv->rows, kv->nseq);
+                    paged_dev(c, kv, n_rows), const_cast<uint32_t*>(kv->lens));
+}
+
+E4B_API int e4b_paged_advance(e4b_ctx* c, const e4b_paged_kv* kv) {
+  return e4b_paged_advance_rows(c, kv, kv && !kv->rows ? kv->nseq : kMaxRows);
 }
 
 }  // extern "C"

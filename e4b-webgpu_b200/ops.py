@@ -139,9 +139,12 @@ def attn_paged(dev: Device, kv, q, out_h, out_f, lse, scratch, *, Q_HEADS, WINDO
              XFO, ROWS)
 
 
-def paged_advance(dev: Device, kv):
-    """lens[s] += the rows of the call just made, on the device"""
-    dev.call("e4b_paged_advance", kv.ref)
+def paged_advance(dev: Device, kv, *, ROWS=None):
+    """lens[s] += the rows of the call just made, on the device; with that call's ROWS, those past it do not count"""
+    if ROWS is None:
+        dev.call("e4b_paged_advance", kv.ref)
+    else:
+        dev.call("e4b_paged_advance_rows", kv.ref, ROWS)
 
 
 def geglumul(dev: Device, a, b, y, *, N):

@@ -573,7 +573,10 @@ E4B_API size_t e4b_paged_scratch_bytes(void);
 E4B_API int e4b_attn_paged(e4b_ctx* ctx, const e4b_paged_kv* kv, const float* q, uint16_t* out_h, float* out_f,
                            float* lse, void* scratch, int QH, int window, int sinks, float scale, int xfo, int n_rows);
 /* lens[s] += the sequence's rows of the call (1 without a rows table): the cache
- * is ready for the next rows.  Writes through kv->lens. */
+ * is ready for the next rows.  Writes through kv->lens.  n_rows: the call's; rows of
+ * the table past it, which the call refused and did not write, do not count (the
+ * status bit again).  e4b_paged_advance takes every row of the table as written. */
+E4B_API int e4b_paged_advance_rows(e4b_ctx* ctx, const e4b_paged_kv* kv, int n_rows);
 E4B_API int e4b_paged_advance(e4b_ctx* ctx, const e4b_paged_kv* kv);
 
 /* ------------------------------------------------------------ argmax / feed */

@@ -137,3 +137,37 @@ def test_4_bit_values_of_any_size(e4b, dev, scratch, name, HD, QH, counts):  # n
         vmax = np.abs(v).reshape(-1, HD // 32, 32).max((0, 2)).repeat(32)
         tol = (2 * ds + 2.0 ** -16 + wide * (p + 1) / w.sum(1))[:, None] * vmax
         assert (np.abs(of[r] - want) <= tol).all(), (r, (np.abs(of[r] - want) / np.maximum(tol, 1e-300)).max())
+
+
+def test_lengths_advance_by_the_rows_that_were_written(e4b, dev):
+    """A rows table that claims more rows than the call has: the refused ones do not count, nor do ones out of order."""
+    lens = [5, 0, 9, 2]
+    for counts, n_rows, want, bad in (([2, 3, 1, 4], 10, [7, 3, 10, 6], 0), ([2, 3, 1, 4], 12, [7, 3, 10, 6], 0),
+                                      ([2, 3, 1, 4], 4, [7, 2, 9, 2], 1), ([2, 3, 1, 4], 0, lens, 1)):
+        c = Cache(e4b, dev, lens, counts, bits=16, page=16, KVH=1, HD=64, ragged=True)
+        e4b.ops.paged_advance(dev, c.kv, ROWS=n_rows)
+        assert list(dev.read(c.kv.struct.lens, np.uint32, 4)) == want and dev.status() == bad
+    e4b.ops.paged_advance(dev, c.kv)                     # all of the table's
+    assert list(dev.read(c.kv.struct.lens, np.uint32, 4)) == [7, 3, 10, 6] and dev.status() == 0
+    c.kv.set_tables(lens=lens, rows=dev.upload(np.array([0, 6, 2, 2, 8], np.uint32)).ptr)
+    e4b.ops.paged_advance(dev, c.kv)
+    assert list(dev.read(c.kv.struct.lens, np.uint32, 4)) == [11, 0, 9, 8]
+    c.kv.set_tables(lens=lens, rows=0)
+    e4b.ops.paged_advance(dev, c.kv, ROWS=4)
+    assert list(dev.read(c.kv.struct.lens, np.uint32, 4)) == [6, 1, 10, 3] and dev.status() == 0
+    with pytest.raises(e4b.E4BError, match="paged_advance: "):
+        e4b.ops.paged_advance(dev, c.kv, ROWS=3)         # without a table the call has a row a sequence
+
+
+def test_refused_rows_stay_out_of_sight(e4b, dev, scratch):  # noqa: F811
+    """Append, attention and advance with a row count below the table's: the next call does not see what was not written."""
+    c = Cache(e4b, dev, [0, 0], [3, 5], bits=4, page=16, KVH=1, HD=64, ragged=True)
+    x = np.random.default_rng(1).standard_normal((6, 3 * 64)).astype(F32)
+    bq = dev.alloc(6 * 64 * 4)
+    e4b.ops.headprep_paged(dev, c.kv, dev.upload(x), None, None, bq, QH=1, ROPE_ANGLES=0, THETA=1e4, NORM=0, ROWS=6)
+    e4b.ops.paged_advance(dev, c.kv, ROWS=6)
+    assert list(dev.read(c.kv.struct.lens, np.uint32, 2)) == [3, 3] and dev.status() == 1
+    c.kv.set_tables(lens=[2, 2], rows=0)
+    of = dev.alloc(2 * 64 * 4)
+    e4b.ops.attn_paged(dev, c.kv, bq, None, of, None, scratch, Q_HEADS=1, ROWS=2)
+    assert np.isfinite(dev.read(of, F32, 128)).all() and dev.status() == 0
