@@ -34,17 +34,16 @@ class PagedKV:
         self.dev, self.pool_bytes, self.owned = dev, pool, []
         self.nseq, self.max_pages = SEQS, MAX_PAGES
 
-        def buf(given, nbytes, name):
-            if given is not None:
-                return int(given)
-            self.owned.append(dev.alloc(nbytes, name))
-            return self.owned[-1].ptr
-
-        self.struct = PagedStruct(buf(k, pool, "paged k"), buf(v, pool, "paged v"),
-                                  buf(pages, SEQS * MAX_PAGES * 4, "page table"), buf(lens, SEQS * 4, "lengths"),
-                                  None if rows is None else int(rows), BITS, PAGE, PAGES, MAX_PAGES, SEQS, KV_HEADS,
-                                  HEAD_DIM)
+        self.struct = PagedStruct(None, None, None, None, None if rows is None else int(rows), BITS, PAGE, PAGES,
+                                  MAX_PAGES, SEQS, KV_HEADS, HEAD_DIM)
         self.ref = ctypes.addressof(self.struct)
+        parts = (("k", k, pool, "paged k"), ("v", v, pool, "paged v"),
+                 ("pages", pages, SEQS * MAX_PAGES * 4, "page table"), ("lens", lens, SEQS * 4, "lengths"))
+        for field, given, nbytes, name in parts:
+            if given is None:
+                given = dev.alloc(nbytes, name)
+                self.owned.append((field, given))
+            setattr(self.struct, field, int(given.ptr if hasattr(given, "ptr") else given))
 
     def set_tables(self, pages=None, lens=None, rows=None):
         """Upload the page table [SEQS][MAX_PAGES] and / or the lengths; `rows`: device address of the rows table
@@ -53,16 +52,23 @@ class PagedKV:
             a = np.ascontiguousarray(pages, np.uint32)
             if a.shape != (self.nseq, self.max_pages):
                 raise ValueError(f"paged cache: page table {a.shape}, expected {(self.nseq, self.max_pages)}")
-            self.dev.write(self.struct.pages, a)
+            self._write(self.struct.pages, a)
         if lens is not None:
             a = np.ascontiguousarray(lens, np.uint32)
             if a.shape != (self.nseq,):
                 raise ValueError(f"paged cache: lengths {a.shape}, expected {(self.nseq,)}")
-            self.dev.write(self.struct.lens, a)
+            self._write(self.struct.lens, a)
         if rows is not None:
             self.struct.rows = int(rows) or None
 
+    def _write(self, ptr, a):
+        if not ptr:
+            raise ValueError("paged cache: freed")
+        self.dev.write(ptr, a)
+
     def free(self):
-        for b in self.owned:
+        """Free what the cache allocated; calls on it are refused from then on."""
+        owned, self.owned = self.owned, []
+        for field, b in owned:
+            setattr(self.struct, field, None)
             self.dev.free(b)
-        self.owned = []
