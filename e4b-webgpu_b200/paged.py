@@ -39,11 +39,15 @@ class PagedKV:
         self.ref = ctypes.addressof(self.struct)
         parts = (("k", k, pool, "paged k"), ("v", v, pool, "paged v"),
                  ("pages", pages, SEQS * MAX_PAGES * 4, "page table"), ("lens", lens, SEQS * 4, "lengths"))
-        for field, given, nbytes, name in parts:
-            if given is None:
-                given = dev.alloc(nbytes, name)
-                self.owned.append((field, given))
-            setattr(self.struct, field, int(given.ptr if hasattr(given, "ptr") else given))
+        try:
+            for field, given, nbytes, name in parts:
+                if given is None:
+                    given = dev.alloc(nbytes, name)
+                    self.owned.append((field, given))
+                setattr(self.struct, field, int(given.ptr if hasattr(given, "ptr") else given))
+        except Exception:
+            self.free()                                  # a pool that could not be had leaves none behind
+            raise
 
     def set_tables(self, pages=None, lens=None, rows=None):
         """Upload the page table [SEQS][MAX_PAGES] and / or the lengths; `rows`: device address of the rows table

@@ -45,3 +45,11 @@ def test_free_leaves_the_callers_buffers(e4b):
     kv = e4b.PagedKV(d, **SIZES, k=1 << 30, lens=1 << 31)
     kv.free()
     assert (kv.struct.k, kv.struct.v, kv.struct.pages, kv.struct.lens) == (1 << 30, None, None, 1 << 31)
+
+
+@pytest.mark.parametrize("at", [1, 2, 3, 4])
+def test_a_failed_allocation_leaves_none_behind(e4b, at):
+    d = FakeDevice(fail_at=at)
+    with pytest.raises(RuntimeError, match="memory"):
+        e4b.PagedKV(d, **SIZES)
+    assert not d.live
