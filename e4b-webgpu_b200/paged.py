@@ -14,6 +14,7 @@ import ctypes
 import numpy as np
 
 from ._lib import lib
+from .device import Buffer
 
 
 class PagedStruct(ctypes.Structure):
@@ -44,6 +45,8 @@ class PagedKV:
                 if given is None:
                     given = dev.alloc(nbytes, name)
                     self.owned.append((field, given))
+                elif isinstance(given, Buffer) and given.nbytes < nbytes:
+                    raise ValueError(f"paged cache: {name} has {given.nbytes} bytes, needs {nbytes}")
                 setattr(self.struct, field, int(given.ptr if hasattr(given, "ptr") else given))
         except Exception:
             self.free()                                  # a pool that could not be had leaves none behind

@@ -53,3 +53,16 @@ def test_a_failed_allocation_leaves_none_behind(e4b, at):
     with pytest.raises(RuntimeError, match="memory"):
         e4b.PagedKV(d, **SIZES)
     assert not d.live
+
+
+@pytest.mark.parametrize("field", ["k", "v", "pages", "lens"])
+def test_small_buffers_are_refused(e4b, field):
+    d = FakeDevice()
+    pool = int(e4b.lib().e4b_paged_pool_bytes(4, 16, 5, 1, 64))
+    need = {"k": pool, "v": pool, "pages": 24, "lens": 8}[field]
+    with pytest.raises(ValueError, match="needs"):
+        e4b.PagedKV(d, **SIZES, **{field: e4b.Buffer(None, 1 << 20, need - 4)})
+    assert not d.live
+    kv = e4b.PagedKV(d, **SIZES, **{field: e4b.Buffer(None, 1 << 20, need)})
+    assert getattr(kv.struct, field) == 1 << 20 and kv.ref == ctypes.addressof(kv.struct)
+    kv.set_tables(np.zeros((2, 3)), [0, 0])
