@@ -171,3 +171,32 @@ def test_refused_rows_stay_out_of_sight(e4b, dev, scratch):  # noqa: F811
     of = dev.alloc(2 * 64 * 4)
     e4b.ops.attn_paged(dev, c.kv, bq, None, of, None, scratch, Q_HEADS=1, ROWS=2)
     assert np.isfinite(dev.read(of, F32, 128)).all() and dev.status() == 0
+
+
+@pytest.mark.parametrize("bits,HD,QH,KVH,window,sinks", [(4, 256, 16, 4, 0, 0), (16, 256, 8, 2, 500, 7), (4, 128, 8, 1, 300, 0),
+                                                         (16, 64, 12, 4, 0, 0)])
+def test_prompts_of_thousands_of_rows(e4b, dev, scratch, bits, HD, QH, KVH, window, sinks):  # noqa: F811
+    """Tens of thousands of units, thousands on a CTA, among them one row of a long sequence; every 61st row checked."""
+    rng = np.random.default_rng(HD)
+    c = Cache(e4b, dev, [0, 2000, 40, 700], [2500, 1, 0, 1803], bits=bits, page=64, KVH=KVH, HD=HD, ragged=True, rows_cap=4310)
+    held = c.fill(rng)
+    q = (rng.standard_normal((c.n_rows, QH, HD)) * (3.0 / np.sqrt(HD))).astype(F32)
+    got = attend(c, scratch, q, QH, window=window, sinks=sinks)
+    assert dev.status() == 0
+    check_rows(c, held, q, got, QH, window, sinks, 1.0, rows=sorted({*range(0, c.n, 61), 2499, 2500, 2501, c.n - 1}))
+    c.kv.free()
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.7, 1e-30, 3e5])
+@pytest.mark.parametrize("counts", [[1, 1], [5, 2]])
+def test_scales_of_any_sign_and_size(e4b, dev, scratch, scale, counts):  # noqa: F811
+    QH, HD, rng = 4, 64, np.random.default_rng(4)
+    for bits in (4, 16):
+        c = Cache(e4b, dev, [90, 0], counts, bits=bits, page=16, KVH=2, HD=HD, ragged=max(counts) > 1)
+        held = c.fill(rng)
+        q = (rng.standard_normal((c.n, QH, HD)) * 0.4).astype(F32)
+        if scale > 1:
+            q *= F32(1 / scale)
+        got = attend(c, scratch, q, QH, scale=scale)
+        assert dev.status() == 0
+        check_rows(c, held, q, got, QH, 0, 0, float(F32(scale)))
