@@ -355,15 +355,22 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
   upto += before;
   // Runs of 2 U at least, or a unit's length (no two on a CTA while others idle); an end
   // that falls within U of a unit's start or end moves there, so short units stay whole
-  // and no fragment is shorter than U.  Units of about one length, and nearly as many as
-  // CTAs, are not cut at all: an end then moves to the nearer one (64 sequences of 1035
-  // tokens and 4 KV heads 28.6 us against 32.6 us).
+  // and no fragment is shorter than U.
+  // Units are not cut at all where the longest is at most 3 U, what cutting costs, above a
+  // CTA's even share (f16, bound by memory rather than by the longest CTA: a third of it).
+  // 64 sequences of 1035 tokens and 4 KV heads of 256, whole and cut: 28.8 and 34.4 us, of
+  // 8000 tokens 163 and 153 us, of 1000..1100 29.8 and 35.7 us; f16, 1035 tokens 46.3 and
+  // 52.5 us, 4000 tokens 154 and 163 us.  Under a rows table a run's end then moves to the
+  // nearer end of a unit, which is the right one while the units together are less than half
+  // the longest short of it each.
   // Where the machine has a CTA for every W (or 2 W) pieces of a kRows unit, that many share
   // it evenly, a turn (or two) of their warps, and none takes from two units (3 sequences of
   // 64 query and 8 KV heads of 128, 1024-token windows: 18.9 us -> 14.2 us).  With one row a
   // unit the longer set-up takes back what it gives: one token behind 551 10.6 -> 10.2 us,
   // 64 behind 1034 28.4 -> 29.1 us, one behind 131000 28.5 -> 29.0 us.
-  const bool uncut = units <= gridDim.x && 10 * units >= 7 * gridDim.x && 20 * (uint64_t)longest * units <= 23 * T;
+  const uint64_t most_over = BITS == 16 ? max(3u * U, longest / 3) : 3u * U;
+  const bool uncut = units <= gridDim.x && (uint64_t)longest * gridDim.x <= T + most_over * gridDim.x &&
+                     (!p.d.rows || 2 * ((uint64_t)longest * units - T) < longest);
   const uint64_t want = max(udiv(T, 2 * U), min((uint64_t)units, udiv(T, U)));
   uint32_t C = T == 0 ? 0u : (uncut ? units : (want < 1 ? 1u : (want < gridDim.x ? (uint32_t)want : gridDim.x)));
   bool even = false;
@@ -402,23 +409,33 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
   __shared__ uint64_t run_end, work_all;                 // (read back where they are needed: the loops need the registers)
   __shared__ uint32_t work_ctas;
   __shared__ bool work_uncut;
+  if (uncut && !even && !p.d.rows) { // every sequence has KVH units: CTA c takes unit c (work counted from its sequence)
+    if (tid == 0) {
+      const int s = cta / p.d.KVH;
+      const SeqWork w = seq_work<NT, U, MODE>(p, s);
+      const uint64_t length = w.range.count + U;
+      start.at = (cta - s * p.d.KVH) * length, start.base = 0, start.s = s, start.w = w;
+      run_end = start.at + length;
+    }
+  } else {
 #pragma unroll
-  for (int i = 0; i < 2; i++) {      // an end of the run, formed by the thread whose sequences hold it
-    const uint64_t raw = udiv(T * (cta + i), C);
-    if (upto - mine <= raw && raw < upto) {
-      uint64_t base = upto - mine;
-      int s = tid * per;
-      SeqWork w = own;
-      while (raw >= base + w.cost && s + 1 < p.d.nseq) {
-        base += w.cost;
-        w = seq_work<NT, U, MODE>(p, ++s);
+    for (int i = 0; i < 2; i++) {      // an end of the run, formed by the thread whose sequences hold it
+      const uint64_t raw = udiv(T * (cta + i), C);
+      if (upto - mine <= raw && raw < upto) {
+        uint64_t base = upto - mine;
+        int s = tid * per;
+        SeqWork w = own;
+        while (raw >= base + w.cost && s + 1 < p.d.nseq) {
+          base += w.cost;
+          w = seq_work<NT, U, MODE>(p, ++s);
+        }
+        const uint64_t length = MODE == kRows && even ? w.parts : w.range.count + U, unit0 = base + udiv(raw - base, length) * length, unit1 = unit0 + length;
+        const uint64_t reach = reach_of(length, even, uncut), at = raw - unit0 < reach ? unit0 : (unit1 - raw < reach ? unit1 : raw);
+        if (i == 1) run_end = at;
+        else start.at = at, start.base = base, start.s = s, start.w = w;
+      } else if (i == 1 && raw == T && tid == 0) {
+        run_end = T;
       }
-      const uint64_t length = MODE == kRows && even ? w.parts : w.range.count + U, unit0 = base + udiv(raw - base, length) * length, unit1 = unit0 + length;
-      const uint64_t reach = reach_of(length, even, uncut), at = raw - unit0 < reach ? unit0 : (unit1 - raw < reach ? unit1 : raw);
-      if (i == 1) run_end = at;
-      else start.at = at, start.base = base, start.s = s, start.w = w;
-    } else if (i == 1 && raw == T && tid == 0) {
-      run_end = T;
     }
   }
   if (tid == 0) work_all = T, work_ctas = C, work_uncut = uncut;

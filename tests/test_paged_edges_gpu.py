@@ -200,3 +200,28 @@ def test_scales_of_any_sign_and_size(e4b, dev, scratch, scale, counts):  # noqa:
         got = attend(c, scratch, q, QH, scale=scale)
         assert dev.status() == 0
         check_rows(c, held, q, got, QH, 0, 0, float(F32(scale)))
+
+
+WHOLE = {  # lens, QH, KVH: about as many units as CTAs, of nearly one length
+    "64 of 1000..1100": (lambda r: [int(x) for x in r.integers(1000, 1101, 64)], 16, 4),
+    "falling": (lambda r: list(range(1100, 1000, -2)), 15, 5),
+    "37 x 4": (lambda r: [int(x) for x in r.integers(150, 200, 37)], 16, 4),
+    "74 x 4": (lambda r: [int(x) for x in r.integers(150, 200, 74)], 4, 4),
+    "8 heads": (lambda r: [int(x) for x in r.integers(1000, 1101, 36)], 32, 4),
+    "some empty": (lambda r: [0, 40] * 36, 6, 2),
+}
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (90, 3)])
+@pytest.mark.parametrize("bits,HD", [(4, 256), (16, 256), (4, 64), (16, 128)])
+def test_units_that_stay_whole(e4b, dev, scratch, bits, HD, window, sinks):  # noqa: F811
+    for name, (lens, QH, KVH) in WHOLE.items():
+        rng = np.random.default_rng(HD)
+        lens = lens(rng)
+        c = Cache(e4b, dev, lens, [1] * len(lens), bits=bits, page=32, KVH=KVH, HD=HD, ragged=False)
+        held = c.fill(rng)
+        q = (rng.standard_normal((c.n, QH, HD)) * (3.0 / np.sqrt(HD))).astype(F32)
+        got = attend(c, scratch, q, QH, window=window, sinks=sinks)
+        assert dev.status() == 0, name
+        check_rows(c, held, q, got, QH, window, sinks, 1.0, rows=range(0, c.n, 3))
+        c.kv.free()
