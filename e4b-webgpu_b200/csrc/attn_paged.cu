@@ -11,15 +11,19 @@
 // A unit cut between CTAs leaves partials in the scratch, which the last CTA to
 // arrive merges in CTA order (the same bits every time).
 //
-// Bounds and measurements (B200; a call's bytes at the copy rate, 6.45 TB/s, is its floor):
-// long caches in 4 bits are bound by the instructions, some 650 for a piece of 4.6 KB, of
-// which 12 warps issue one in 55 % of the cycles: 32 sequences of 8000..16000 tokens, 16
-// query and 4 KV heads of 256, 100 us = 4.1 TB/s (floor 63 us).  64 sequences of 1035 tokens take 28.6 us (floor 12 us)
-// and one of 131001 tokens and 2 KV heads 28.9 us (11.7 us): set-up, first pieces, merges
-// and the join of the parts, 6 to 8 us one after the other, come beside it; one token
-// behind 551 takes 10.3 us of them alone.  f16, 64 windows of 1024: 28.9 us (15.3 us).
-// Several rows a sequence (8 x 1..64 rows behind 300..4000 tokens, windows of 1024): 77 us,
-// bound by the latency of the products on 8 warps (tensor pipe 20 % busy).
+// Bounds and measurements (B200; a call's bytes at the copy rate, 6.45 TB/s, is its floor;
+// replayed calls, one at a time in the stream):
+// long caches in 4 bits are bound by the latency of a warp's chain (loads, products,
+// shuffles, exponents, products), 660 instructions for a piece of 4.6 KB: three warps a
+// scheduler issue in 54 % of the cycles, with neither memory (45 %) nor the tensor pipe
+// (21 %) near its limit.  32 sequences of 8000..16000 tokens, 16 query and 4 KV heads of 256,
+// 102 us = 4.0 TB/s (floor 63 us; 107 us among calls on other caches).  64 sequences of 1035
+// tokens take 28.8 us (floor 12 us) and one of 131001 tokens and 2 KV heads 29.8 us (11.7
+// us): set-up, first pieces, merges and the join of the parts, 6 to 8 us one after the other,
+// come beside it; one token behind 551 takes 10.4 us of them alone.  f16, 64 windows of 1024:
+// 29.4 us (15.3 us).  Several rows a sequence (8 x 1..64 rows behind 300..4000 tokens, windows
+// of 1024): 81 us, bound by the latency of the products on 8 warps (tensor pipe 20 % busy),
+// each piece decoded once for 16 columns; 16 prompts of 1..1000 rows 1450 us.
 //
 // Products, per piece and 8 MMA columns (m16n8k16, f32 accumulators):
 //   S[slot][col]  = K[slot][:] . q[:][col]      A = keys,   B = q
@@ -100,7 +104,10 @@ struct Shape {
   // warps (a warp then never waits for a phase before the stage's last one is done)
   static constexpr int S = W * (BITS == 16 ? (HD == 256 ? 1 : (HD == 128 ? 2 : 4)) :
                                 MODE == kRows ? (HD == 256 ? 2 : (HD == 128 ? 4 : 8)) : (HD == 256 ? 3 : (HD == 128 ? 5 : 8)));
-  // what a unit costs beside its pieces (q, the merge, the outputs), in pieces
+  // what a unit costs beside its pieces (q, the merge, the outputs), in pieces.  Half of it
+  // and twice it (us, as is in the middle): 48 ragged sequences, 4 bits 15.9 / 13.1 / 18.2,
+  // f16 22.4 / 15.7 / 12.6; 8 x 1..64 rows 91 / 81 / 80; 300 of 1..400 tokens 16.3 / 17.6 /
+  // 17.5, f16 19.2 / 15.1 / 16.8; 32 of 8000..16000 tokens 104 / 103 / 101
   static constexpr int U = MODE == kRows ? 16 : (BITS == 16 ? (HD == 256 ? 6 : (HD == 128 ? 8 : 12)) : (HD == 256 ? 12 : 16));
   static constexpr int LN = S <= 32 ? S : (W == 11 ? 11 : (W == 5 ? (S == 40 ? 20 : 25) : 32));   // producer lanes; S is a multiple
   static constexpr int THREADS = MODE == kRows ? 384 : 32 * (W + 1), CT = 32 * W;
@@ -365,7 +372,7 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
   // the longest short of it each.
   // Where the machine has a CTA for every W (or 2 W) pieces of a kRows unit, that many share
   // it evenly, a turn (or two) of their warps, and none takes from two units (3 sequences of
-  // 64 query and 8 KV heads of 128, 1024-token windows: 18.9 us -> 14.2 us).  With one row a
+  // 64 query and 8 KV heads of 128, 1024-token windows: 20.6 us -> 15.2 us).  With one row a
   // unit the longer set-up takes back what it gives: one token behind 551 10.6 -> 10.2 us,
   // 64 behind 1034 28.4 -> 29.1 us, one behind 131000 28.5 -> 29.0 us.
   const uint64_t most_over = BITS == 16 ? max(3u * U, longest / 3) : 3u * U;
@@ -1254,10 +1261,10 @@ template <int BITS, int HD>
 int launch_mode(e4b_ctx* c, const AttnP& p) {
   if (p.G > 4 || p.d.rows) return launch<BITS, HD, kRows>(c, p);
   // few units: all of an SM's warps on one (kWide against kNarrow, 4 bits, heads of 256: a
-  // sequence of 131001 tokens and 2 KV heads 28.9 against 36.0 us, 32 of 8000..16000 tokens
-  // and 4 KV heads 100 against 109 us); more units than SMs: two CTAs per SM (64 of 1035
-  // tokens and 4 KV heads 28.6 against 34.4 us; f16, windows of 1024 in 1..8000 tokens 28.9
-  // against 43.0 us)
+  // sequence of 131001 tokens and 2 KV heads 29.9 against 37.5 us, 32 of 8000..16000 tokens
+  // and 4 KV heads 102 against 111 us); more units than SMs: two CTAs per SM (kNarrow against
+  // kWide, 64 of 1035 tokens and 4 KV heads 28.9 against 35.7 us; f16, windows of 1024 in
+  // 1..8000 tokens 29.3 against 42.7 us)
   if (p.d.nseq * p.d.KVH <= c->sm_count) return launch<BITS, HD, kWide>(c, p);
   return launch<BITS, HD, kNarrow>(c, p);
 }

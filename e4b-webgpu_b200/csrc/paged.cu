@@ -174,14 +174,16 @@ E4B_DEV RowPlace place_one(const PagedDev& d, uint32_t row) {          // a thre
 // pair (p, p + HD/2) and a group of four codes sit in one lane and a 32-dim block in 8
 // neighbouring lanes.  The rotation's angles are formed once per row for all its heads,
 // in 64 bits (a position of 10^6 times a frequency leaves f32 no fraction).  q is
-// computed in f32.  Keys and values are formed in 64 bits: what is stored is then the
-// rounding of the exact value whatever the order of the sums, so the 4-bit codes do not
-// depend on it.  Bound by memory for many rows (per row of 16 q + 2 x 4 heads of 256:
+// computed in f32.  Keys and values are formed in 64 bits and rounded through f32 to f16:
+// what is stored is the exact value's rounding (but within 2^-24 of a border between two
+// f16, where the first rounding may decide) whatever the order of the sums, so neither the
+// f16 rows nor the 4-bit codes of them depend on it.  Bound by memory for many rows (per row of 16 q + 2 x 4 heads of 256:
 // 24.6 KB read, 16.4 KB of q and 2.3 KB of 4-bit cache written): prompts of 16 x 1..1000
-// such rows with their read-back as f16 take 81 us, 4.3 TB/s (floor 55 us).  f16 rows whose
-// values are their keys, 8 x 1..500 into an f16 cache, 25 us (floor 12 us), are bound by the
-// lanes' conversions and 64-bit products between barriers (issue slots 53 % busy); one row,
-// 4.9 us, and 64, 6.3 us, by latency: two launches with their chains of loads.
+// such rows take 69 us and their read-back as f16 12.8 us, 4.3 TB/s together (floor 55 us).
+// f16 rows whose values are their keys, 8 x 1..500 into an f16 cache, 20 and 4.1 us (floor
+// 12 us together), are bound by the lanes' conversions and 64-bit products between barriers
+// (issue slots 53 % busy); one row, 2.9 and 1.9 us, and 64, 3.9 and 2.1 us, by latency: a
+// chain of loads each.
 // A head of a turn: where its elements are, and where it goes.
 struct Item {
   uint32_t src;                      // bytes from the turn's first row (rows row_bytes apart: kStaged), or of its row
