@@ -74,7 +74,8 @@ class PagedKV:
         self.dev.write(ptr, a)
 
     def free(self):
-        """Free what the cache allocated; calls on it are refused from then on."""
+        """Free what the cache allocated; calls on it are refused from then on (a recorded plan of such calls is to be
+        destroyed before)."""
         owned, self.owned = self.owned, []
         for field, b in owned:
             setattr(self.struct, field, None)

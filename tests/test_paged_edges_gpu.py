@@ -225,3 +225,38 @@ def test_units_that_stay_whole(e4b, dev, scratch, bits, HD, window, sinks):  # n
         assert dev.status() == 0, name
         check_rows(c, held, q, got, QH, window, sinks, 1.0, rows=range(0, c.n, 3))
         c.kv.free()
+
+
+BORDERS = [2.0 ** -24, 2.0 ** -14 - 2.0 ** -24, 2.0 ** -14, 2.0 ** -7 - 2.0 ** -18, 2.0 ** -7, 2 - 2.0 ** -10, 2.0, 128 - 2.0 ** -4, 128.0, 8188.0]
+
+
+@pytest.mark.parametrize("first,second", [(a, b) for i, a in enumerate(BORDERS) for b in (a, BORDERS[-1 - i], BORDERS[(i + 1) % 10])])
+@pytest.mark.parametrize("QH,count", [(4, 1), (8, 1), (2, 7)])
+def test_scales_at_the_borders_under_growing_scores(e4b, dev, scratch, QH, count, first, second):  # noqa: F811
+    """Value scales at the borders of the kernel's classes, two blocks of one size and then of another, while the scores
+    grow by 2^5.5 from turn to turn of the warps, so that p is as large as it may be: nothing overflows."""
+    HD, n = 64, 900
+    c = Cache(e4b, dev, [n - count, n - count], [count, count], bits=4, page=32, KVH=1, HD=HD, ragged=count > 1)
+    t = np.arange(n)
+    xs = []
+    for turn in (5, 11):
+        x = np.zeros((n, 2, 1, HD))
+        x[:, 0, 0, 0] = np.minimum(5.5 * (t // (16 * turn)), 22.0)
+        d = np.where(t < n // 2, first, second)
+        x[:, 1, 0] = d[:, None] * np.random.default_rng(turn).integers(-8, 8, (n, HD))
+        x[:, 1, 0, ::32] = -8 * d[:, None]
+        xs.append(x)
+    held = write(c, xs)
+    assert np.array_equal(held[0][0], xs[0][:, 0]) and np.array_equal(held[0][1], xs[0][:, 1])
+    q = np.zeros((c.n, QH, HD), F32)
+    q[..., 0] = np.log(2.0)
+    _, of, lse = attend(c, scratch, q, QH)
+    assert dev.status() == 0
+    for r in range(c.n):
+        s, p = c.place(r)
+        k, v = (a[:p + 1, 0] for a in held[s])
+        sc = q[r].astype(np.float64) @ k.T
+        w = np.exp(sc - sc.max(1, keepdims=True))
+        # scores: 2^-16 of |q| 15 d (see test_4_bit_values_of_any_size)
+        tol = (2 * 2.0 ** -16 * 15 / 8 * sc.max() + 2.0 ** -16 + 2.0 ** -16 * (p + 1) / w.sum(1))[:, None] * np.abs(v).max()
+        assert (np.abs(of[r] - w @ v / w.sum(1, keepdims=True)) <= tol).all()
