@@ -177,8 +177,9 @@ E4B_DEV RowPlace place_one(const PagedDev& d, uint32_t row) {          // a thre
 // computed in f32.  Keys and values are formed in 64 bits and rounded through f32 to f16:
 // what is stored is the exact value's rounding (but within 2^-24 of a border between two
 // f16, where the first rounding may decide) whatever the order of the sums, so neither the
-// f16 rows nor the 4-bit codes of them depend on it.  Bound by memory for many rows (per row of 16 q + 2 x 4 heads of 256:
-// 24.6 KB read, 16.4 KB of q and 2.3 KB of 4-bit cache written): prompts of 16 x 1..1000
+// f16 rows nor the 4-bit codes of them depend on it.  Bound by memory for many rows (per
+// row of 16 q + 2 x 4 heads of 256: 24.6 KB read, 16.4 KB of q and 2.3 KB of 4-bit cache
+// written): prompts of 16 x 1..1000
 // such rows take 69 us and their read-back as f16 12.8 us, 4.3 TB/s together (floor 55 us).
 // f16 rows whose values are their keys, 8 x 1..500 into an f16 cache, 20 and 4.1 us (floor
 // 12 us together), are bound by the lanes' conversions and 64-bit products between barriers
