@@ -14,30 +14,27 @@
 // Bounds and measurements (B200; a call's bytes at the copy rate, 6.45 TB/s, is its floor;
 // replayed calls, one at a time in the stream):
 // long caches in 4 bits are bound by the latency of a warp's chain (loads, products,
-// shuffles, exponents, products), 660 instructions for a piece of 4.6 KB: three warps a
-// scheduler issue in 54 % of the cycles, with neither memory (45 %) nor the tensor pipe
-// (21 %) near its limit.  32 sequences of 8000..16000 tokens, 16 query and 4 KV heads of 256,
-// 102 us = 4.0 TB/s (floor 63 us; 107 us among calls on other caches).  64 sequences of 1035
-// tokens take 28.8 us (floor 12 us) and one of 131001 tokens and 2 KV heads 29.8 us (11.7
+// shuffles, exponents, products), 717 instructions for a piece of 4.6 KB: three warps a
+// scheduler issue in 56 % of the cycles, with neither memory (44 %) nor the tensor pipe
+// (20 %) near its limit.  32 sequences of 8000..16000 tokens, 16 query and 4 KV heads of 256,
+// 107 us = 3.8 TB/s (floor 63 us; 109 us among calls on other caches).  64 sequences of 1035
+// tokens take 30.2 us (floor 12 us) and one of 131001 tokens and 2 KV heads 30.8 us (11.7
 // us): set-up, first pieces, merges and the join of the parts, 6 to 8 us one after the other,
-// come beside it; one token behind 551 takes 10.4 us of them alone.  f16, 64 windows of 1024:
-// 29.4 us (15.3 us).  Several rows a sequence (8 x 1..64 rows behind 300..4000 tokens, windows
+// come beside it; one token behind 551 takes 10.8 us of them alone.  f16, 64 windows of 1024:
+// 29.2 us (15.3 us).  Several rows a sequence (8 x 1..64 rows behind 300..4000 tokens, windows
 // of 1024): 81 us, bound by the latency of the products on 8 warps (tensor pipe 20 % busy),
-// each piece decoded once for 16 columns; 16 prompts of 1..1000 rows 1450 us.
+// each piece decoded once for 16 columns; 16 prompts of 1..1000 rows 1440 us.
 //
 // Products, per piece and 8 MMA columns (m16n8k16, f32 accumulators):
 //   S[slot][col]  = K[slot][:] . q[:][col]      A = keys,   B = q
 //   O[dim][col]  += V[slot][dim] p[slot][col]   A = values, B = p
 // The 8 columns are 4 query heads of one row as f16 hi and lo parts (columns 0-3,
 // 4-7), so q and p carry f32 precision at the MMA cost of one f16 pass.
-// 4-bit keys: A holds the codes n as f16 subnormals, n * 2^-24 (a code in the low
-// bits of a half) or 16 n * 2^-24 (one place up; q is divided by 16 there), so
-// decoding is one AND per pair; a block's scale d multiplies its dot product in
-// f32, and the code's -8 is one more MMA per piece, sum_b d_b (-8 sum q_b).
-// The MMA aligns a subnormal by its exponent field, which costs it up to 7 of the
-// sum's 24 bits: no loss for 15-bit products of one magnitude (q's), but 6e-6 of
-// the result where p spreads over many, so 4-bit values are decoded to normal f16
-// n - 8.  A value block's scale multiplies p, again as hi + lo.  To keep the lo parts
+// 4-bit keys and values: A holds n - 8, two instructions per pair of codes; a key
+// block's scale multiplies its dot product in f32.  (Codes n as f16 subnormals, n * 2^-24
+// by one AND, with the -8 taken off by one more MMA, make 4 % of long caches' time, but the
+// MMA aligns a subnormal by its exponent field and sums larger numbers: f32 outputs were
+// 0.7e-6 to 1.8e-6 off in place of 0.1e-6 to 0.8e-6.)  A value block's scale multiplies p, again as hi + lo.  To keep the lo parts
 // clear of f16's subnormals p is lifted by 2^8, and a block of 32 dims whose visible
 // scales have all been below 2^-7 (2^-14) is held times 2^8 (2^15): a product is off by
 // 2^-20 of itself and 2^-22 of the largest p times the block's largest value at most
@@ -54,7 +51,6 @@ constexpr int kMaxCtas = 320;
 constexpr int kGroup = 12;           // CTAs whose parts are merged first
 constexpr int kMostParts = 9;        // CTAs that share a unit evenly (10 to 12: merging them costs more than equal runs, 17.3 us against 15.1 us)
 constexpr uint32_t kLowCodes = 0x000F000Fu, kHighCodes = 0x00F000F0u;
-constexpr float kTwo24 = 16777216.f;
 // p is held as p * 2^8 relative to a maximum that may lag behind the largest score by
 // 2^6, so a rescaling of O is rare and p * d stays below 2^15 for scales d below 2.
 // A visible scale of 2 or more ends the lag (d below 2^7), one of 2^7 or more leaves a
@@ -105,9 +101,9 @@ struct Shape {
   static constexpr int S = W * (BITS == 16 ? (HD == 256 ? 1 : (HD == 128 ? 2 : 4)) :
                                 MODE == kRows ? (HD == 256 ? 2 : (HD == 128 ? 4 : 8)) : (HD == 256 ? 3 : (HD == 128 ? 5 : 8)));
   // what a unit costs beside its pieces (q, the merge, the outputs), in pieces.  Half of it
-  // and twice it (us, as is in the middle): 48 ragged sequences, 4 bits 15.9 / 13.1 / 18.2,
-  // f16 22.4 / 15.7 / 12.6; 8 x 1..64 rows 91 / 81 / 80; 300 of 1..400 tokens 16.3 / 17.6 /
-  // 17.5, f16 19.2 / 15.1 / 16.8; 32 of 8000..16000 tokens 104 / 103 / 101
+  // and twice it (us, as is in the middle): 48 ragged sequences, 4 bits 15.3 / 13.3 / 18.8,
+  // f16 21.2 / 15.6 / 12.9; 8 x 1..64 rows 91 / 81 / 80; 300 of 1..400 tokens 16.2 / 17.3 /
+  // 17.2, f16 19.1 / 15.3 / 16.9; 32 of 8000..16000 tokens 108 / 107 / 105
   static constexpr int U = MODE == kRows ? 16 : (BITS == 16 ? (HD == 256 ? 6 : (HD == 128 ? 8 : 12)) : (HD == 256 ? 12 : 16));
   static constexpr int LN = S <= 32 ? S : (W == 11 ? 11 : (W == 5 ? (S == 40 ? 20 : 25) : 32));   // producer lanes; S is a multiple
   static constexpr int THREADS = MODE == kRows ? 384 : 32 * (W + 1), CT = 32 * W;
@@ -299,7 +295,6 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
   __shared__ uint64_t warp_sum_[Sh::THREADS / 32];
   __shared__ uint32_t warp_units[Sh::THREADS / 32], warp_longest[Sh::THREADS / 32];
   __shared__ uint2 warp_parts[Sh::THREADS / 32];
-  __shared__ uint2 qzero[BITS == 4 ? Sh::TILES * 32 : 32];               // B of the -8 term: -8 sum q per block, hi and lo
   __shared__ float qfac[Sh::TILES * TC];
   __shared__ float ml[W * LC * 2];
   __shared__ int last_one, more_units;
@@ -313,8 +308,6 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
     mbar_init(&freed[tid], 1);
   }
   if (tid == 0) fence_barrier_init();
-  if constexpr (BITS == 4)
-    for (int i = tid; i < Sh::TILES * 32; i += Sh::THREADS) qzero[i] = make_uint2(0u, 0u);
   pdl_wait();
 
   // ---- the run of this CTA: the work of all units, cut evenly
@@ -365,14 +358,14 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
   // and no fragment is shorter than U.
   // Units are not cut at all where the longest is at most 3 U, what cutting costs, above a
   // CTA's even share (f16, bound by memory rather than by the longest CTA: a third of it).
-  // 64 sequences of 1035 tokens and 4 KV heads of 256, whole and cut: 28.8 and 34.4 us, of
-  // 8000 tokens 163 and 153 us, of 1000..1100 29.8 and 35.7 us; f16, 1035 tokens 46.3 and
-  // 52.5 us, 4000 tokens 154 and 163 us.  Under a rows table a run's end then moves to the
+  // 64 sequences of 1035 tokens and 4 KV heads of 256, whole and cut: 30.2 and 35.8 us, of
+  // 8000 tokens 173 and 162 us, of 1000..1100 31.4 and 36.9 us; f16, 1035 tokens 46.3 and
+  // 52.3 us, 4000 tokens 154 and 164 us.  Under a rows table a run's end then moves to the
   // nearer end of a unit, which is the right one while the units together are less than half
   // the longest short of it each.
   // Where the machine has a CTA for every W (or 2 W) pieces of a kRows unit, that many share
   // it evenly, a turn (or two) of their warps, and none takes from two units (3 sequences of
-  // 64 query and 8 KV heads of 128, 1024-token windows: 20.6 us -> 15.2 us).  With one row a
+  // 64 query and 8 KV heads of 128, 1024-token windows: 20.0 us -> 14.7 us).  With one row a
   // unit the longer set-up takes back what it gives: one token behind 551 10.6 -> 10.2 us,
   // 64 behind 1034 28.4 -> 29.1 us, one behind 131000 28.5 -> 29.0 us.
   const uint64_t most_over = BITS == 16 ? max(3u * U, longest / 3) : 3u * U;
@@ -568,21 +561,17 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
         const int e = (int)(__float_as_uint(m) >> 23);   // biased exponent; 0: zero or subnormal, 255: inf
         const int up = e == 255 ? 0 : min(14 + 127 - e, 120);
         const float f = __uint_as_float((uint32_t)(up + 127) << 23);
-        float hi[8], lo[8], sum = 0.f;
+        float hi[8], lo[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) {
           const float v = x[i] * f;
           hi[i] = __half2float(__float2half_rn(v));
           lo[i] = __half2float(__float2half_rn(v - hi[i]));
-          sum += v;
         }
         uint4 fh, fl;
         if constexpr (BITS == 4) {
-          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-          constexpr float r = 1.f / 16.f;
-          fh = make_uint4(pack2(hi[0], hi[4]), pack2(hi[2], hi[6]), pack2(hi[1] * r, hi[5] * r), pack2(hi[3] * r, hi[7] * r));
-          fl = make_uint4(pack2(lo[0], lo[4]), pack2(lo[2], lo[6]), pack2(lo[1] * r, lo[5] * r), pack2(lo[3] * r, lo[7] * r));
+          fh = make_uint4(pack2(hi[0], hi[4]), pack2(hi[2], hi[6]), pack2(hi[1], hi[5]), pack2(hi[3], hi[7]));
+          fl = make_uint4(pack2(lo[0], lo[4]), pack2(lo[2], lo[6]), pack2(lo[1], lo[5]), pack2(lo[3], lo[7]));
         } else {
           fh = make_uint4(pack2(hi[0], hi[1]), pack2(hi[2], hi[3]), pack2(hi[4], hi[5]), pack2(hi[6], hi[7]));
           fl = make_uint4(pack2(lo[0], lo[1]), pack2(lo[2], lo[3]), pack2(lo[4], lo[5]), pack2(lo[6], lo[7]));
@@ -592,15 +581,6 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
           uint4* at = qfrag + ((size_t)(tile * NB + blk) * QP) * 32 + cc * 4 + tt;
           at[0] = fh;
           at[MODE == kRows ? 32 : 16] = fl;
-          if constexpr (BITS == 4) {
-            // B[k][col] of -8 sum q / 2^8: k = block (hi part), 8 + block (lo part); the rest stays zero
-            if (tt == 0) {
-              uint16_t* z = reinterpret_cast<uint16_t*>(qzero + tile * 32 + cc * 4 + blk / 2) + (blk & 1);
-              const float v = sum * (-8.f / 256.f);
-              z[0] = f2h(v);
-              z[2] = f2h(v - h2f(z[0]));
-            }
-          }
           if (l == 0)
             qfac[c] = p.scale * 1.4426950408889634f * __uint_as_float((uint32_t)(127 - up) << 23);
         }
@@ -643,21 +623,15 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
       constexpr int N = decltype(tiles)::value;
       // ---- scores
       float s[N][4];
+#pragma unroll
+      for (int nt = 0; nt < N; nt++)
+#pragma unroll
+        for (int k = 0; k < 4; k++) s[nt][k] = 0.f;
       if (BITS == 4) {
         constexpr int RUN = NB < 4 ? NB : 4;
         uint32_t da[NB / 2], db[NB / 2];                 // scales of slots g, g + 8
         lds_words<NB / 2>(da, kp + g * NB * 2);
         lds_words<NB / 2>(db, kp + (g + 8) * NB * 2);
-        float z[N][4];
-        const uint32_t dz0 = t < NB / 2 ? *reinterpret_cast<const uint32_t*>(kp + g * NB * 2 + t * 4) : 0u;
-        const uint32_t dz1 = t < NB / 2 ? *reinterpret_cast<const uint32_t*>(kp + (g + 8) * NB * 2 + t * 4) : 0u;
-#pragma unroll
-        for (int nt = 0; nt < N; nt++) {
-          const uint2 zb = qzero[nt * 32 + lane];
-          mma16816_zero(z[nt], dz0, dz1, dz0, dz1, zb.x, zb.y);
-#pragma unroll
-          for (int k = 0; k < 4; k++) s[nt][k] = 0.f;
-        }
 #pragma unroll
         for (int r = 0; r < NB / RUN; r++) {
           uint32_t wa[RUN], wb[RUN];
@@ -668,16 +642,18 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
             const int b = r * RUN + q;
             const uint32_t sa = wa[q] >> 8, sb = wb[q] >> 8;
             const float d0 = half_of(da[b / 2], b & 1), d1 = half_of(db[b / 2], b & 1);
+            const uint32_t al[4] = {low_codes(wa[q]), low_codes(wb[q]), low_codes(sa), low_codes(sb)};
+            const uint32_t ah[4] = {high_codes(wa[q]), high_codes(wb[q]), high_codes(sa), high_codes(sb)};
 #pragma unroll
             for (int nt = 0; nt < N; nt++) {
               const uint4 qb = qf[(nt * NB + b) * QP * 32];
               float acc[4];
-              mma16816_zero(acc, wa[q] & kLowCodes, wb[q] & kLowCodes, sa & kLowCodes, sb & kLowCodes, qb.x, qb.y);
-              mma16816(acc, wa[q] & kHighCodes, wb[q] & kHighCodes, sa & kHighCodes, sb & kHighCodes, qb.z, qb.w);
+              mma16816_zero(acc, al[0], al[1], al[2], al[3], qb.x, qb.y);
+              mma16816(acc, ah[0], ah[1], ah[2], ah[3], qb.z, qb.w);
               if (MODE == kRows) {
                 const uint4 ql = qf[((nt * NB + b) * QP + 1) * 32];
-                mma16816(acc, wa[q] & kLowCodes, wb[q] & kLowCodes, sa & kLowCodes, sb & kLowCodes, ql.x, ql.y);
-                mma16816(acc, wa[q] & kHighCodes, wb[q] & kHighCodes, sa & kHighCodes, sb & kHighCodes, ql.z, ql.w);
+                mma16816(acc, al[0], al[1], al[2], al[3], ql.x, ql.y);
+                mma16816(acc, ah[0], ah[1], ah[2], ah[3], ql.z, ql.w);
               }
               s[nt][0] = fmaf(d0, acc[0], s[nt][0]);
               s[nt][1] = fmaf(d0, acc[1], s[nt][1]);
@@ -686,15 +662,7 @@ __global__ void __launch_bounds__(Shape<BITS, HD, MODE>::THREADS, Shape<BITS, HD
             }
           }
         }
-#pragma unroll
-        for (int nt = 0; nt < N; nt++)
-#pragma unroll
-          for (int k = 0; k < 4; k++) s[nt][k] = fmaf(s[nt][k], kTwo24, z[nt][k] * 256.f);
       } else {
-#pragma unroll
-        for (int nt = 0; nt < N; nt++)
-#pragma unroll
-          for (int k = 0; k < 4; k++) s[nt][k] = 0.f;
 #pragma unroll
         for (int b = 0; b < NB; b++) {
           const uint4 wa = lds128(kp + (b * 16 + g) * 64 + t * 16), wb = lds128(kp + (b * 16 + g + 8) * 64 + t * 16);
@@ -1261,10 +1229,10 @@ template <int BITS, int HD>
 int launch_mode(e4b_ctx* c, const AttnP& p) {
   if (p.G > 4 || p.d.rows) return launch<BITS, HD, kRows>(c, p);
   // few units: all of an SM's warps on one (kWide against kNarrow, 4 bits, heads of 256: a
-  // sequence of 131001 tokens and 2 KV heads 29.9 against 37.5 us, 32 of 8000..16000 tokens
-  // and 4 KV heads 102 against 111 us); more units than SMs: two CTAs per SM (kNarrow against
-  // kWide, 64 of 1035 tokens and 4 KV heads 28.9 against 35.7 us; f16, windows of 1024 in
-  // 1..8000 tokens 29.3 against 42.7 us)
+  // sequence of 131001 tokens and 2 KV heads 31.0 against 38.6 us, 32 of 8000..16000 tokens
+  // and 4 KV heads 107 against 116 us); more units than SMs: two CTAs per SM (kNarrow against
+  // kWide, 64 of 1035 tokens and 4 KV heads 30.3 against 36.7 us; f16, windows of 1024 in
+  // 1..8000 tokens 29.3 against 42.9 us)
   if (p.d.nseq * p.d.KVH <= c->sm_count) return launch<BITS, HD, kWide>(c, p);
   return launch<BITS, HD, kNarrow>(c, p);
 }

@@ -3,7 +3,9 @@
 Scores: one visible slot, so lse is the score.  q = 2^j (1 + 2^-11), which f16 rounds to 2^j everywhere; keys 1 and 1/2,
 which both caches hold exactly.  Every product and partial sum is a multiple of 2^-14 below 2^9, so f32 holds the sum
 exactly in any order; what remains is the factor scale * log2(e) (three roundings with the product), the reference score
-less 2^3, the sum with log2(2^8) (an ulp, 2^-20) and the factor log(2): 2^-20 (1 + |s|).  Without the lo parts s is off by 2^-11 s, of one 32-dim block by 2^-14 s or more.
+less 2^3, the sum with log2(2^8) (an ulp, 2^-20) and the factor log(2): 2^-20 (1 + |s|).  Without the lo parts s is off
+by 2^-11 s, of one 32-dim block by 2^-14 s or more.  The same holds beside elements of q of 2^14 where the key is zero:
+they add nothing, unless codes enter uncentred, as 8 d 2^14 that is taken off again.
 
 Weights: scores that are exact multiples of 2^-10 below 4, 1 to 16 slots (one piece).  ex2 of a difference below 8 (2^-21
 with its argument's roundings), p as hi + lo (2^-22), its product with a scale (2^-20), 17 addends cut at 2^-23 in each of
@@ -14,12 +16,14 @@ import numpy as np
 F32, F64 = np.float32, np.float64
 
 
-def score_case(HD, n_rows, QH):
-    """q [n_rows][QH][HD], keys and values [1][2][1][HD] of the one slot."""
+def score_case(HD, n_rows, QH, large=0.0):
+    """q [n_rows][QH][HD], keys and values [1][2][1][HD] of the one slot; large: every 16th element of q, where the key is 0."""
     j = (np.arange(n_rows)[:, None, None] + np.arange(QH)[None, :, None] + np.arange(HD)) % 3
     q = (2.0 ** -j * (1 + 2.0 ** -11)).astype(F32)
     x = np.ones((1, 2, 1, HD))
     x[0, 0, 0, 1::2] = 0.5
+    if large:
+        q[..., 5::16], x[0, 0, 0, 5::16] = large, 0.0
     return q, x
 
 

@@ -109,7 +109,7 @@ SIZES = {  # factors of the values' blocks of 32 dims in turn, and whether they 
 @pytest.mark.parametrize("name", SIZES)
 def test_4_bit_values_of_any_size(e4b, dev, scratch, name, HD, QH, counts):  # noqa: F811
     """Every block of 32 dims is as precise relative to its own largest value.  Scores: at most 2^-16 of the sum of
-    |q| 15 d (codes enter as 0..15), which moves an output by twice that of vmax.  Products p d: 2^-22 of the largest p
+    |q| times the block's largest |k|, which moves an output by twice that of vmax.  Products p d: 2^-22 of the largest p
     times vmax each (2^-16 beside scales of 2^7 or more), so n / sum(p / max p) of it in the output.  The rest, ex2
     (2^-22), three roundings of a product (2^-20), 17 addends cut at 2^-23 in each of the two MMAs of a piece (2^-18),
     f32 sums: 2^-16 altogether."""
@@ -132,8 +132,8 @@ def test_4_bit_values_of_any_size(e4b, dev, scratch, name, HD, QH, counts):  # n
         sc = q[r].astype(np.float64) @ k.T                                   # [QH][slots]
         w = np.exp(sc - sc.max(1, keepdims=True))
         want = w @ v / w.sum(1, keepdims=True)
-        d15 = 15 / 8 * np.abs(k).reshape(-1, HD // 32, 32).max(-1).repeat(32, -1)
-        ds = 2.0 ** -16 * (np.abs(q[r]).astype(np.float64) @ d15.T).max(1)
+        kmax = np.abs(k).reshape(-1, HD // 32, 32).max(-1).repeat(32, -1)
+        ds = 2.0 ** -16 * (np.abs(q[r]).astype(np.float64) @ kmax.T).max(1)
         vmax = np.abs(v).reshape(-1, HD // 32, 32).max((0, 2)).repeat(32)
         tol = (2 * ds + 2.0 ** -16 + wide * (p + 1) / w.sum(1))[:, None] * vmax
         assert (np.abs(of[r] - want) <= tol).all(), (r, (np.abs(of[r] - want) / np.maximum(tol, 1e-300)).max())
@@ -257,6 +257,6 @@ def test_scales_at_the_borders_under_growing_scores(e4b, dev, scratch, QH, count
         k, v = (a[:p + 1, 0] for a in held[s])
         sc = q[r].astype(np.float64) @ k.T
         w = np.exp(sc - sc.max(1, keepdims=True))
-        # scores: 2^-16 of |q| 15 d (see test_4_bit_values_of_any_size)
-        tol = (2 * 2.0 ** -16 * 15 / 8 * sc.max() + 2.0 ** -16 + 2.0 ** -16 * (p + 1) / w.sum(1))[:, None] * np.abs(v).max()
+        # scores: 2^-16 of |q k| (see test_4_bit_values_of_any_size)
+        tol = (2 * 2.0 ** -16 * sc.max() + 2.0 ** -16 + 2.0 ** -16 * (p + 1) / w.sum(1))[:, None] * np.abs(v).max()
         assert (np.abs(of[r] - w @ v / w.sum(1, keepdims=True)) <= tol).all()

@@ -2,7 +2,7 @@
 does not."""
 import numpy as np
 import pytest
-from paged_precision import F64, hi, score_bound, score_case, weight_bound, weight_case
+from paged_precision import F32, F64, hi, score_bound, score_case, weight_bound, weight_case
 
 from oracle import paged as op
 
@@ -27,11 +27,19 @@ def test_scores_without_lo_parts_break_the_bound(HD, bits):
         one = q.copy()
         one[..., 32 * b:32 * b + 32] = hi(q)[..., 32 * b:32 * b + 32]
         assert (np.abs(one @ k - s) > 10 * score_bound(s)).all()
-    if bits == 4:                                        # codes n (0 and 4) times d, and the -8: either of the two
-        n = k / -0.125 + 8
-        assert (np.abs((hi(q) - q) @ n * -0.125) > 50 * score_bound(s)).all()
-        total = q.reshape(5, 4, -1, 32).sum(-1)
-        assert np.abs((total.astype(np.float16).astype(F64) - total).sum(-1)).max() > 50 * score_bound(s).max()
+
+
+@pytest.mark.parametrize("HD", [64, 128, 256])
+def test_uncentred_codes_break_the_bound(HD):
+    """Codes 0..15 summed in f32 beside q of 2^14, the 8 taken off at the end; centred, every sum is exact."""
+    q, x = score_case(HD, 5, 4, 2.0 ** 14)
+    k = held(x, 4)[0, 0, 0]
+    assert np.array_equal(k, x[0, 0, 0])
+    s = q.astype(F64) @ k
+    n = (k / -0.125 + 8).astype(F32)
+    sums = np.cumsum((q * n).astype(F32), -1, dtype=F32)[..., -1] - 8 * np.cumsum(q, -1, dtype=F32)[..., -1]
+    assert (np.abs(sums * F32(-0.125) - s) > 4 * score_bound(s)).all()
+    assert np.array_equal(np.cumsum((q * (n - 8)).astype(F32), -1, dtype=F32)[..., -1] * F32(-0.125), s)
 
 
 @pytest.mark.parametrize("slots", [2, 3, 7, 16])

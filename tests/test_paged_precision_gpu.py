@@ -13,11 +13,12 @@ FORMS = {"a row each": (3, 1, 4), "many sequences": (200, 1, 3), "8 heads": (3, 
 @pytest.mark.parametrize("HD", [64, 128, 256])
 @pytest.mark.parametrize("bits", [4, 16])
 @pytest.mark.parametrize("form", FORMS)
-def test_scores(e4b, dev, scratch, form, bits, HD):  # noqa: F811
+@pytest.mark.parametrize("large", [0.0, 2.0 ** 14])
+def test_scores(e4b, dev, scratch, large, form, bits, HD):  # noqa: F811
     """Rows that see one slot (a window of 1 where there are several rows): lse is the score, o the value."""
     nseq, rows, QH = FORMS[form]
     c = Cache(e4b, dev, [0] * nseq, [rows] * nseq, bits=bits, page=16, KVH=1, HD=HD, ragged=rows > 1)
-    q, x = score_case(HD, c.n, QH)
+    q, x = score_case(HD, c.n, QH, large)
     k, v = write(c, [x.repeat(rows, 0)] * nseq)[0]
     assert np.array_equal(k[0], x[0, 0])
     _, of, lse = attend(c, scratch, q, QH, window=1 if rows > 1 else 0)
