@@ -32,13 +32,14 @@
 // 4-7), so q and p carry f32 precision at the MMA cost of one f16 pass.
 // 4-bit keys and values: A holds n - 8, two instructions per pair of codes; a key
 // block's scale multiplies its dot product in f32.  (Codes n as f16 subnormals, n * 2^-24
-// by one AND, with the -8 taken off by one more MMA, make 4 % of long caches' time, but the
-// MMA aligns a subnormal by its exponent field and sums larger numbers: f32 outputs were
-// 0.7e-6 to 1.8e-6 off in place of 0.1e-6 to 0.8e-6.)  A value block's scale multiplies p, again as hi + lo.  To keep the lo parts
-// clear of f16's subnormals p is lifted by 2^8, and a block of 32 dims whose visible
-// scales have all been below 2^-7 (2^-14) is held times 2^8 (2^15): a product is off by
-// 2^-20 of itself and 2^-22 of the largest p times the block's largest value at most
-// (2^-16 of that where scales of 2^7 or more stand beside such a block).
+// by one AND, with the -8 taken off by one more MMA, take 4 % less time on long caches, but
+// the MMA aligns a subnormal by its exponent field and sums larger numbers: f32 outputs
+// were 0.7e-6 to 1.8e-6 off in place of 0.1e-6 to 0.8e-6.)  A value block's scale
+// multiplies p, again as hi + lo.  To keep the lo parts clear of f16's subnormals p is
+// lifted by 2^8, and a block of 32 dims whose visible scales have all been below 2^-7
+// (2^-14) is held times 2^8 (2^15): a product is off by 2^-20 of itself and 2^-22 of the
+// largest p times the block's largest value at most (2^-16 of that where scales of 2^7 or
+// more stand beside such a block).
 #include <type_traits>
 
 #include "paged.cuh"

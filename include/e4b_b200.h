@@ -561,10 +561,10 @@ E4B_API int e4b_kvread_paged(e4b_ctx* ctx, const e4b_paged_kv* kv, void* k_out, 
  * that sees nothing gives zeros and lse = -inf.  q and the softmax's p are f16
  * hi + lo pairs and the sums f32: a product is off by 2^-20 of itself and 2^-22 of
  * the largest |q| (p) times the largest |k| (|v|) of its 32 dims that the call's
- * rows see of the sequence (below 2^-14 that counts as 2^-14, except for 4-bit
- * values; there 2^-16 where |v| is below 2^-4 and others are above 1024).  An
- * infinity or NaN in a visible slot gives infinities or NaN in what it reaches;
- * slots that no row sees change no bit.  Pages wholly between the sinks and
+ * rows see of the sequence (f16: below 2^-14 that counts as 2^-14; 4 bits: 2^-16
+ * where |v| is below 2^-4 and others are above 1024).  An infinity or NaN in a
+ * visible slot gives infinities or NaN in what it reaches; slots that no row sees
+ * change no bit.  Pages wholly between the sinks and
  * the window are not read and need no valid id.  scratch: e4b_paged_scratch_bytes(),
  * zeroed once before its first use (each call leaves it ready for the next) and
  * not shared by calls that may overlap.  q, outputs and scratch 16-byte aligned;
